@@ -68,6 +68,16 @@ class TurboPrefillParams(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """glq_paged_cache (include/glorcq_hip.h), field for field."""
+    _fields_ = [
+        *[(n, _vp) for n in ("k_pages", "v_pages", "k_scales", "v_scales", "page_table",
+                             "lengths")],
+        *[(n, _i64) for n in ("seqs", "max_pages", "table_stride", "pages", "kv_heads",
+                              "head_dim", "page_size")],
+    ]
+
+
 # name -> (restype, argtypes); must match include/glorcq_hip.h exactly.
 SIGNATURES = {
     "glq_version": (_c_int, []),
@@ -225,6 +235,19 @@ SIGNATURES = {
         _vp, ctypes.c_float, _vp,       # len, scale, advance
         _vp, _vp, _i64, _vp,            # out, U, rank, parts
         _vp, _i64, _vp,                 # workspace, bytes, stream
+    ]),
+    "glq_paged_append": (_c_int, [
+        ctypes.POINTER(PagedCache), _vp, _i64,  # cache, starts, tokens
+        _vp, _i64, _vp, _i64,           # k, k_stride, v, v_stride
+        _vp, _i64, _i64, _i64,          # q, q_heads, q_stride, q_item_rows
+        _vp, _vp, ctypes.c_float,       # q_norm_w, k_norm_w, eps
+        _vp, _vp, _i64, _vp, _vp,       # cos, sin, cs_stride, q_out, stream
+    ]),
+    "glq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "glq_paged_attention": (_c_int, [
+        ctypes.POINTER(PagedCache), _vp, _i64,  # cache, starts, tokens
+        _vp, _i64, ctypes.c_float, _i64,        # q, q_heads, scale, window
+        _vp, _vp, _i64, _vp,                    # out, workspace, bytes, stream
     ]),
 }
 

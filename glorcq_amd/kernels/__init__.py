@@ -1061,3 +1061,11 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         workspace.data_ptr(), workspace.numel(), _lib.stream_handle(q.device)),
         "glq_decode_attention")
     return out
+
+
+# the paged key/value cache (it uses the checks and workspaces above)
+from .paged import (paged_append, paged_attention, paged_attention_workspace,  # noqa: E402
+                    paged_cache_tensors)
+
+__all__ += ["paged_append", "paged_attention", "paged_attention_workspace",
+            "paged_cache_tensors"]

@@ -728,6 +728,88 @@ int glq_decode_attention_xu(const void* q, const void* k_cache, const void* v_ca
                             void* out, const void* U, int64_t rank, float* parts,
                             void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * ---- Paged key/value cache ----
+ * For sequences of lengths of their own; no reference counterpart (its model
+ * path keeps one static cache a batch, inference/graph_wrapper.py:69-149).
+ *
+ * One layer's cache: a pool of pages of page_size tokens (a power of two in
+ * [16, 1024]); page page_table[b * table_stride + i] of the pool holds
+ * positions [i page_size, (i + 1) page_size) of sequence b.  head_dim 64 or
+ * 128.  In blocks of 16 tokens:
+ *   k_pages (pages, kv_heads, page_size, head_dim)
+ *   v_pages (pages, kv_heads, page_size / 16, head_dim, 16)
+ * of fp16 values (k_scales and v_scales NULL), or of e4m3 codes (OCP FP8:
+ * largest value 448, NaN, no infinities) with
+ *   k_scales, v_scales (pages, kv_heads, page_size / 16) e8m0 bytes,
+ * a block's values being code * 2^(byte - 127) (byte 255: NaN).
+ *
+ * A batch brings `tokens` new tokens as rows of q, k and v: rows
+ * [starts[b], starts[b + 1]) (seqs + 1 int32 on the device, ascending) are
+ * sequence b's, or, with starts NULL, tokens / seqs rows each.  lengths[b]
+ * (int32, device) counts the sequence's tokens with the new ones, which sit at
+ * the last positions.  Rows behind starts[seqs] are neither read nor written.
+ * Everything on the device is checked there: positions below 0 or past the
+ * page table and page ids outside [0, pages) are not written; what they would
+ * have held is NaN to the rows that see them.
+ */
+typedef struct glq_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  void* k_scales;  /* NULL with v_scales: fp16 pages */
+  void* v_scales;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  int64_t seqs;
+  int64_t max_pages;     /* entries of a page table row; * page_size <= 2^30 */
+  int64_t table_stride;  /* entries between rows */
+  int64_t pages;         /* of the pool */
+  int64_t kv_heads;
+  int64_t head_dim;
+  int64_t page_size;
+} glq_paged_cache;
+
+/*
+ * Appends the new tokens' keys and values, and rotates their queries, in one
+ * launch: for each head of q and k,
+ *   x' = rope(x rsqrt(mean(x^2) + eps) w),  rope(y) = y cos + rotate_half(y) sin
+ * (norm weights of head_dim fp16, NULL: no norm; cos/sin rows of head_dim fp16,
+ * one a token, cs_stride apart, 0 for one row for all, NULL: no rotation), in
+ * fp32, rounded once: q' to q_out (tokens, q_heads, head_dim) fp16, k' and v to
+ * their places in the pages.  q may be NULL (nothing is rotated).  8-bit pages:
+ * a block's scale is the smallest 2^e >= amax / 448 (e >= -32) of its finite
+ * values that no token before it needed larger; a block that had tokens keeps
+ * a larger scale, and is scaled down by the power of two where the new ones
+ * need more (e4m3 subnormals are then rounded again).  Infinities and NaN are
+ * stored as NaN.  What lies behind a sequence's last token in its block
+ * becomes zero.  Rows of k, v and q are k_stride, v_stride and q_stride values
+ * apart (multiples of 8); with q_item_rows > 0, q is item-major as in
+ * glq_qk_norm_rope.  Pages that get tokens must belong to one sequence.
+ */
+int glq_paged_append(const glq_paged_cache* cache, const int32_t* starts, int64_t tokens,
+                     const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                     const void* q, int64_t q_heads, int64_t q_stride, int64_t q_item_rows,
+                     const void* q_norm_w, const void* k_norm_w, float eps, const void* cos,
+                     const void* sin, int64_t cs_stride, void* q_out, void* stream);
+
+/*
+ * Causal attention of the new tokens over the cache (after glq_paged_append):
+ * the row of q at position p of its sequence attends to positions
+ * (p - window, p], window 0: [0, p]:
+ *   out[t][h*D + d] = fp16(sum_p softmax_p(scale * q.k_p) v_p[d]),
+ * KV head h / (q_heads / kv_heads), fp32 scores, softmax and sums.  A row
+ * without positions (p < 0) is 0; one past the page table NaN.  q (tokens,
+ * q_heads, head_dim) fp16, out (tokens, q_heads * head_dim).  workspace:
+ * glq_paged_attention_workspace_bytes, 256-byte aligned, zero-filled
+ * before its first use (each call leaves its counters zero); calls that share
+ * it must not overlap.
+ */
+int64_t glq_paged_attention_workspace_bytes(int64_t seqs, int64_t tokens, int64_t q_heads,
+                                            int64_t kv_heads, int64_t head_dim);
+int glq_paged_attention(const glq_paged_cache* cache, const int32_t* starts, int64_t tokens,
+                        const void* q, int64_t q_heads, float scale, int64_t window, void* out,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -421,3 +421,61 @@ def test_moe_prefill_token_tile(lib, monkeypatch, mean, tile):
         monkeypatch.setenv("GLQ_PF_MOE_TM", str(tm))
         forced[tm] = size()
     assert mine == forced[tile] and len(set(forced.values())) >= 2
+
+
+def _paged(**kw):
+    p = 1 << 12
+    c = dict(k_pages=p, v_pages=p, k_scales=p, v_scales=p, page_table=p, lengths=p, seqs=2,
+             max_pages=4, table_stride=4, pages=8, kv_heads=2, head_dim=128, page_size=64)
+    return ctypes.byref(_lib.PagedCache(**{**c, **kw}))
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(head_dim=96), b"head_dim"), (dict(page_size=48), b"page_size"),
+    (dict(page_size=8), b"page_size"), (dict(page_size=2048), b"page_size"),
+    (dict(kv_heads=0), b"kv_heads"), (dict(seqs=-1), b"seqs"), (dict(pages=1 << 31), b"pages"),
+    (dict(max_pages=1 << 25), b"max_pages"), (dict(table_stride=3), b"table_stride"),
+    (dict(pages=0), b"no pages"), (dict(k_pages=None), b"null"), (dict(lengths=None), b"null"),
+    (dict(v_scales=None), b"come together"), (dict(v_pages=8), b"aligned"),
+    (dict(seqs=3), b"same number"),
+])
+def test_paged_cache_checks(lib, kw, what):
+    """A cache descriptor that does not fit is refused on the host by both
+    entry points, before any launch."""
+    p, nul = 1 << 12, None
+    rc = lib.glq_paged_append(_paged(**kw), nul, 2, p, 256, p, 256, nul, 0, 0, 0, nul, nul, 1e-6,
+                              nul, nul, 0, nul, nul)
+    assert rc == 1 and what in lib.glq_last_error()
+    rc = lib.glq_paged_attention(_paged(**kw), nul, 2, p, 8, 1.0, 0, p, p, 1 << 30, nul)
+    assert rc == 1 and what in lib.glq_last_error()
+
+
+def test_paged_entry_points_check_arguments(lib):
+    p, nul = 1 << 12, None
+
+    def append(k=p, ks=256, vs=256, q=nul, Hq=0, qs=0, item=0, cos=nul, sin=nul, cs=0, qo=nul):
+        return lib.glq_paged_append(_paged(), nul, 2, k, ks, p, vs, q, Hq, qs, item, nul, nul,
+                                    1e-6, cos, sin, cs, qo, nul)
+
+    for rc, what in [
+        (append(k=nul), b"null"), (append(k=p + 8), b"aligned"), (append(ks=250), b"strides"),
+        (append(vs=260), b"strides"), (append(cos=p), b"cos and sin"),
+        (append(cos=p, sin=p, cs=64), b"cs_stride"), (append(q=p, Hq=3, qs=512, qo=p), b"q_heads"),
+        (append(q=p, Hq=4, qs=512), b"q_out"), (append(q=p, Hq=4, qs=256, qo=p), b"row stride"),
+        (append(q=p, Hq=4, item=96, qo=p), b"q_item_rows"),
+    ]:
+        assert rc == 1, what
+    assert append(q=p, Hq=4, item=96, qo=p) == 1 and b"q_item_rows" in lib.glq_last_error()
+
+    def attend(q=p, Hq=8, window=0, out=p):
+        return lib.glq_paged_attention(_paged(), nul, 2, q, Hq, 1.0, window, out, p, 1 << 30, nul)
+
+    assert attend(Hq=7) == 1 and b"q_heads" in lib.glq_last_error()
+    assert attend(window=-1) == 1 and b"window" in lib.glq_last_error()
+    assert attend(out=nul) == 1 and attend(q=p + 2) == 1 and b"aligned" in lib.glq_last_error()
+    # no tokens: nothing is looked at
+    c = _paged(k_pages=None, pages=0)
+    assert lib.glq_paged_attention(c, nul, 0, nul, 8, 1.0, 0, nul, nul, 0, nul) == 0
+    assert lib.glq_paged_append(c, nul, 0, nul, 0, nul, 0, nul, 0, 0, 0, nul, nul, 1e-6, nul, nul,
+                                0, nul, nul) == 0
+    assert lib.glq_paged_attention_workspace_bytes(-1, 1, 1, 1, 128) == -1
