@@ -78,6 +78,26 @@ class PagedCache(ctypes.Structure):
     ]
 
 
+class PagedAppendParams(ctypes.Structure):
+    """glq_paged_append_params (include/glorcq_hip.h), field for field."""
+    _fields_ = [
+        ("cache", PagedCache), ("starts", _vp), ("tokens", _i64),
+        *[(n, _vp) for n in ("k", "v", "q")],
+        *[(n, _i64) for n in ("k_stride", "v_stride", "q_stride", "q_heads", "q_item_rows")],
+        *[(n, _vp) for n in ("q_norm_w", "k_norm_w", "cos", "sin")],
+        ("cs_stride", _i64), ("q_out", _vp), ("eps", ctypes.c_float), ("reserved", ctypes.c_int32),
+    ]
+
+
+class PagedAttentionParams(ctypes.Structure):
+    """glq_paged_attention_params (include/glorcq_hip.h), field for field."""
+    _fields_ = [
+        ("cache", PagedCache), ("starts", _vp), ("tokens", _i64), ("q", _vp), ("out", _vp),
+        ("q_heads", _i64), ("window", _i64), ("workspace", _vp), ("workspace_bytes", _i64),
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); must match include/glorcq_hip.h exactly.
 SIGNATURES = {
     "glq_version": (_c_int, []),
@@ -236,19 +256,11 @@ SIGNATURES = {
         _vp, _vp, _i64, _vp,            # out, U, rank, parts
         _vp, _i64, _vp,                 # workspace, bytes, stream
     ]),
-    "glq_paged_append": (_c_int, [
-        ctypes.POINTER(PagedCache), _vp, _i64,  # cache, starts, tokens
-        _vp, _i64, _vp, _i64,           # k, k_stride, v, v_stride
-        _vp, _i64, _i64, _i64,          # q, q_heads, q_stride, q_item_rows
-        _vp, _vp, ctypes.c_float,       # q_norm_w, k_norm_w, eps
-        _vp, _vp, _i64, _vp, _vp,       # cos, sin, cs_stride, q_out, stream
-    ]),
-    "glq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
-    "glq_paged_attention": (_c_int, [
-        ctypes.POINTER(PagedCache), _vp, _i64,  # cache, starts, tokens
-        _vp, _i64, ctypes.c_float, _i64,        # q, q_heads, scale, window
-        _vp, _vp, _i64, _vp,                    # out, workspace, bytes, stream
-    ]),
+    # (params as c_void_p: a pointer to one of the structures above, or its bytes)
+    "glq_paged_append": (_c_int, [_vp, _vp]),            # params, stream
+    "glq_paged_attention_scratch_bytes": (_i64, []),
+    "glq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "glq_paged_attention": (_c_int, [_vp, _vp]),         # params, stream
 }
 
 _lib = None

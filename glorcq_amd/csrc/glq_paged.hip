@@ -24,31 +24,37 @@ struct AppendArgs {
   float eps;
 };
 
+__device__ __forceinline__ float rsqrt_of(float x) { return rsqrtf(x); }
+__device__ __forceinline__ double rsqrt_of(double x) { return rsqrt(x); }
+
 // A head's D values on D / 8 lanes, 8 each (lane `c` of them: 8 c .. + 8).
 //   x -> x rsqrt(mean(x^2) + eps) w   (w != null)
 //     -> x cos + rotate_half(x) sin   (cos != null)
-// in fp32; the caller rounds once.
-template <int D>
-__device__ __forceinline__ void head_norm_rope(float (&x)[8], const f16x8* w, const f16x8* cos,
+// The caller rounds once.  q: in fp32.  k: in fp64, since a value that fp32
+// leaves on the wrong side of a border between two e4m3 codes is off by a
+// whole step of 2^-3 for as long as the cache lives; the vector fp64 rate is
+// half of fp32's, and k has a share Hk / Hq of the work.
+template <int D, class F>
+__device__ __forceinline__ void head_norm_rope(F (&x)[8], const f16x8* w, const f16x8* cos,
                                                const f16x8* sin, int c, float eps) {
   constexpr int L = D / 8;
   if (w) {
-    float ss = 0.f;
+    F ss = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
 #pragma unroll
     for (int o = 1; o < L; o <<= 1) ss += __shfl_xor(ss, o);
-    const float r = rsqrtf(ss / (float)D + eps);
+    const F r = rsqrt_of(ss / (F)D + (F)eps);
     const f16x8 wv = *w;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (float)wv[e];
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (F)wv[e];
   }
   if (cos) {
     const f16x8 cv = *cos, sv = *sin;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_xor(x[e], L / 2);  // the value D / 2 away
-      x[e] = fmaf(x[e], (float)cv[e], (c < L / 2 ? -other : other) * (float)sv[e]);
+      const F other = __shfl_xor(x[e], L / 2);  // the value D / 2 away
+      x[e] = x[e] * (F)cv[e] + (c < L / 2 ? -other : other) * (F)sv[e];
     }
   }
 }
@@ -162,12 +168,24 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(AppendArgs a)
     fresh[p] = pos >= lo && pos < hi;
     const int64_t t = fresh[p] ? s0 + (pos - first) : s0;
     const f16x8 v = fresh[p] ? ((const f16x8*)(src + t * stride + h * D))[li] : f16x8{};
+    if (isv) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[p][e] = (float)v[e];
-    if (!isv)
-      head_norm_rope<D>(x[p], a.kw ? (const f16x8*)a.kw + li : nullptr,
+      for (int e = 0; e < 8; ++e) x[p][e] = (float)v[e];
+    } else {
+      double y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = (double)v[e];
+      head_norm_rope<D>(y, a.kw ? (const f16x8*)a.kw + li : nullptr,
                         a.cos ? (const f16x8*)(a.cos + t * a.cs_stride) + li : nullptr,
                         a.cos ? (const f16x8*)(a.sin + t * a.cs_stride) + li : nullptr, li, a.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // to fp32, and from there to the pages' type, as torch converts fp64
+        // (the asm keeps the compiler from making one conversion of the two)
+        x[p][e] = (float)y[e];
+        asm("" : "+v"(x[p][e]));
+      }
+    }
   }
   if constexpr (FP8) {
     float amax = 0.f;
@@ -310,14 +328,18 @@ int paged_view(const glq_paged_cache* c, const int32_t* starts, int64_t tokens, 
 
 }  // namespace glq
 
-extern "C" int glq_paged_append(const glq_paged_cache* cache, const int32_t* starts,
-                                int64_t tokens, const void* k, int64_t k_stride, const void* v,
-                                int64_t v_stride, const void* q, int64_t q_heads,
-                                int64_t q_stride, int64_t q_item_rows, const void* q_norm_w,
-                                const void* k_norm_w, float eps, const void* cos, const void* sin,
-                                int64_t cs_stride, void* q_out, void* stream) {
+extern "C" int glq_paged_append(const glq_paged_append_params* p, void* stream) {
   using namespace glq;
   clear_error();
+  GLQ_CHECK(p != nullptr, "null params");
+  const glq_paged_cache* cache = &p->cache;
+  const int32_t* starts = p->starts;
+  const int64_t tokens = p->tokens, k_stride = p->k_stride, v_stride = p->v_stride;
+  const int64_t q_heads = p->q_heads, q_stride = p->q_stride, q_item_rows = p->q_item_rows;
+  const int64_t cs_stride = p->cs_stride;
+  const void *k = p->k, *v = p->v, *q = p->q, *cos = p->cos, *sin = p->sin;
+  const void *q_norm_w = p->q_norm_w, *k_norm_w = p->k_norm_w;
+  void* q_out = p->q_out;
   AppendArgs a{};
   if (int rc = paged_view(cache, starts, tokens, a.c)) return rc;
   const int64_t D = cache->head_dim, Hk = cache->kv_heads;
@@ -346,7 +368,7 @@ extern "C" int glq_paged_append(const glq_paged_cache* cache, const int32_t* sta
   a.q_item = (int)q_item_rows;
   a.qw = (const __half*)q_norm_w; a.kw = (const __half*)k_norm_w;
   a.cos = (const __half*)cos; a.sin = (const __half*)sin; a.cs_stride = cs_stride;
-  a.q_out = (__half*)q_out; a.Hq = q ? (int)q_heads : 0; a.eps = eps;
+  a.q_out = (__half*)q_out; a.Hq = q ? (int)q_heads : 0; a.eps = p->eps;
   // blocks: a sequence's n new tokens touch at most (n + 14) / 16 + 1 of them
   a.units = (int)((a.c.each + kBlkTokens - 2) / kBlkTokens + 1);
   const int64_t slots = starts ? tokens / kBlkTokens + 2 * cache->seqs : cache->seqs * a.units;

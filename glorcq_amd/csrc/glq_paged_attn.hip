@@ -3,19 +3,24 @@
 
 #include <algorithm>
 
+#include "glq_handoff.h"
 #include "glq_paged.h"
 
 namespace glq {
 namespace {
 
-constexpr int kPaThreads = 256;
+constexpr int kPaThreads = 512;
+constexpr int kPaWaves = kPaThreads / 64;
 constexpr int kPaRows = 16;  // query rows (tokens x the KV head's q heads) of a unit
+constexpr int kPaGrid = 256;
 
 struct PagedAttnArgs {
   PagedView c;
   const __half* q;  // (T, Hq, D)
   __half* out;      // (T, Hq D)
-  int rep, window, tiles_each;
+  float* part;      // [workgroup][2][kPaRows][D + 4]: o, m, l
+  unsigned* count;  // [unit], zero between calls
+  int rep, window, tiles_each, rows;
   float scale2;     // scale log2(e)
 };
 
@@ -39,6 +44,7 @@ struct RowAttention {
   static constexpr int TP = FP8 ? 64 : 32, P = TP / 4, NT = TP / 16, NM = P / 8;
   static constexpr int KL = FP8 ? D / 64 : D / 32;  // 16-byte pieces of a K row and lane
   static constexpr int NC = D / 16;
+  static constexpr int S = FP8 ? 1 : 2;             // bytes of a value
 
   struct Tile {
     u32x4 k[NT][KL], v[NC];
@@ -47,7 +53,7 @@ struct RowAttention {
   };
 
   const PagedView& c;
-  int b, g, li, kb;
+  int b, g, li, kb, rep, window;
   float scale2;
   RowSet r;
   f16x8 q[D / 32];
@@ -59,7 +65,7 @@ struct RowAttention {
     kb = (threadIdx.x >> 4) & 3;
   }
 
-  __device__ void begin(const __half* qp, int rep, int Hq) {
+  __device__ void begin(const __half* qp, int Hq) {
     const int t = r.s0 + r.row / rep, h = g * rep + r.row % rep;
     const f16x8* src = (const f16x8*)(qp + ((int64_t)t * Hq + h) * D);
 #pragma unroll
@@ -71,36 +77,44 @@ struct RowAttention {
     for (int i = 0; i < NC; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // Block of 16 tokens -> its place in the pool; pages out of range read page 0.
-  __device__ int64_t place(int blk, bool& bad) const {
-    const int bps = c.page_shift - 4;
-    const int i = blk >> bps;
-    const int p = c.table[b * c.table_stride + min(i, c.max_pages - 1)];
-    bad = p < 0 || p >= c.pages;
-    return ((int64_t)(bad ? 0 : p) * c.Hk + g) * (1 << bps) + (blk & ((1 << bps) - 1));
+  // Page ids of a tile's blocks as a lane needs them, for k's rows and for v
+  // (and the scales, which are the blocks' of v's lanes).
+  struct Ids {
+    int k, v;
+  };
+  __device__ Ids ids(int tile) const {
+    const int bps = c.page_shift - 4, b0 = tile * (TP / 16);
+    const int* row = c.table + b * c.table_stride;
+    return {row[min((b0 + (FP8 ? li >> 2 : li >> 3)) >> bps, c.max_pages - 1)],
+            row[min((b0 + (FP8 ? kb : kb >> 1)) >> bps, c.max_pages - 1)]};
   }
 
-  __device__ void load(Tile& x, int tile) const {
-    constexpr int S = FP8 ? 1 : 2;
-    bool ignore;
+  // A block's place in the pool; ids out of range read page 0.
+  __device__ int64_t place(int p, int blk) const {
+    const int bpp = 1 << (c.page_shift - 4);
+    return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g) * bpp + (blk & (bpp - 1));
+  }
+  __device__ void load_k(Tile& x, int tile, Ids id) const {
     const int b0 = tile * (TP / 16);
-    const int64_t kblk = place(b0 + (FP8 ? li >> 2 : li >> 3), ignore);
-    const int64_t vblk = place(b0 + (FP8 ? kb : kb >> 1), x.bad);
-    const char* kp = (const char*)c.k + kblk * (16 * D * S);
-    const char* vp = (const char*)c.v + vblk * (16 * D * S);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int row = (FP8 ? 0 : 8 * ((li >> 2) & 1)) + 4 * i + (li & 3);
-#pragma unroll
-      for (int t = 0; t < KL; ++t) x.k[i][t] = *(const u32x4*)(kp + row * D * S + 64 * t + 16 * kb);
-    }
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-      x.v[i] = *(const u32x4*)(vp + (16 * i + li) * 16 * S + (FP8 ? 0 : 16 * (kb & 1)));
     if constexpr (FP8) {
+      const int64_t vblk = place(id.v, b0 + kb);
       x.ks = c.ks[vblk];
       x.vs = c.vs[vblk];
     }
+    x.bad = (unsigned)id.v >= (unsigned)c.pages;
+    const char* p = (const char*)c.k + place(id.k, b0 + (FP8 ? li >> 2 : li >> 3)) * (16 * D * S) +
+                    ((FP8 ? 0 : 8 * ((li >> 2) & 1)) + (li & 3)) * D * S + 16 * kb;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int t = 0; t < KL; ++t) x.k[i][t] = *(const u32x4*)(p + 4 * i * D * S + 64 * t);
+  }
+  __device__ void load_v(Tile& x, int tile, Ids id) const {
+    const char* p = (const char*)c.v +
+                    place(id.v, tile * (TP / 16) + (FP8 ? kb : kb >> 1)) * (16 * D * S) +
+                    li * 16 * S + (FP8 ? 0 : 16 * (kb & 1));
+#pragma unroll
+    for (int i = 0; i < NC; ++i) x.v[i] = *(const u32x4*)(p + 16 * i * 16 * S);
   }
 
   __device__ static f16x8 k_frag(const Tile& x, int i, int s) {
@@ -111,18 +125,20 @@ struct RowAttention {
       return __builtin_bit_cast(f16x8, x.k[i][s]);
     }
   }
-  __device__ static f16x8 v_frag(const Tile& x, int i, int mm) {
+  __device__ static f16x8 v_frag(u32x4 v, int mm) {
     if constexpr (FP8)
-      return fp8x8_to_f16(x.v[i][2 * mm], x.v[i][2 * mm + 1]);
+      return fp8x8_to_f16(v[2 * mm], v[2 * mm + 1]);
     else
-      return __builtin_bit_cast(f16x8, x.v[i]);
+      return __builtin_bit_cast(f16x8, v);
   }
 
   // Online softmax over the tile's positions.  The scale 2^e of a V block goes
   // into the exponent: w = 2^(t + e - m) with m the largest t + e so far, so
   // that w (fp16 for the product) keeps its bits where the block's share of
   // the result is largest; the denominator sums w 2^-e in fp32.
-  __device__ void step(const Tile& x, int tile) {
+  // `next_k`: fetches the next tile's k into x, whose k has been used by then.
+  template <class Next>
+  __device__ void step(Tile& x, int tile, Next next_k) {
     const int p0 = tile * TP + P * kb;
     const bool edge = tile * TP < r.lo_all || (tile + 1) * TP > r.hi_all;
     float t[NT][4];
@@ -146,6 +162,7 @@ struct RowAttention {
 #pragma unroll
       for (int j = 0; j < 4; ++j) mx = fmaxf(mx, t[i][j]);
     }
+    next_k();
     mx = fmaxf(mx, __shfl_xor(mx, 16));
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     const float mf = mx == -__builtin_inff() ? 0.f : mx;
@@ -169,46 +186,53 @@ struct RowAttention {
     // (a block that the row does not see may hold any scale)
     l = ls == 0.f ? l : fmaf(ls, __builtin_amdgcn_exp2f(-ev), l);
     // weight 0 times an inf or a NaN behind a row's positions is not 0
-    bool odd = false;
-    if (edge) {
+    if (!edge || __builtin_amdgcn_ballot_w64(odd(x)) == 0) {
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int mm = 0; mm < NM; ++mm) {
-          const u32x4 u = __builtin_bit_cast(u32x4, v_frag(x, i, mm));
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            odd |= (u[e] & 0x7C00u) == 0x7C00u || (u[e] & 0x7C000000u) == 0x7C000000u;
-        }
-      odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-    }
-    if (!odd) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int mm = 0; mm < NM; ++mm) o[i] = mfma_16x16x32(v_frag(x, i, mm), w[mm], o[i]);
+        for (int mm = 0; mm < NM; ++mm) o[i] = mfma_16x16x32(v_frag(x.v[i], mm), w[mm], o[i]);
     } else {
-      // a position at a time, and only into the rows that see it
-#pragma unroll
-      for (int e = 0; e < P; ++e)
+      // a token's rows at a time, with zeros for the positions that it does
+      // not see
+      const int tok = r.row / rep, last = __builtin_amdgcn_readlane(tok, 15);
 #pragma nounroll
-        for (int k4 = 0; k4 < 4; ++k4) {
-          const bool mine = kb == k4;
-          const int p = tile * TP + P * k4 + e;
-          const bool sees = p >= r.lo && p < r.hi;
-          f16x8 wp{};
-          wp[e & 7] = mine ? w[e >> 3][e & 7] : (_Float16)0.f;
+      for (int k = __builtin_amdgcn_readfirstlane(tok); k <= last; ++k) {
+        const int pos = r.first + k, hi = pos + 1, lo = window > 0 ? pos - window + 1 : 0;
+        const int n0 = min(max(lo - p0, 0), P), n1 = min(max(hi - p0, 0), P);
+        constexpr int E = FP8 ? 4 : 2;  // values of a word
+        auto below = [](int n) {        // the bits of its first n values
+          return n <= 0 ? 0u : n >= E ? ~0u : (1u << (32 / E * n)) - 1u;
+        };
+        u32x4 keep;
 #pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            const f16x8 vf = v_frag(x, i, e >> 3);
-            f16x8 vp{};
-            vp[e & 7] = mine ? vf[e & 7] : (_Float16)0.f;
-            const f32x4 on = mfma_16x16x32(vp, wp, o[i]);
+        for (int e = 0; e < 4; ++e) keep[e] = below(n1 - E * e) & ~below(n0 - E * e);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = sees ? on[j] : o[i][j];
-          }
+        for (int i = 0; i < NC; ++i) {
+          const u32x4 v = x.v[i] & keep;
+          f32x4 on = o[i];
+#pragma unroll
+          for (int mm = 0; mm < NM; ++mm) on = mfma_16x16x32(v_frag(v, mm), w[mm], on);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][j] = tok == k ? on[j] : o[i][j];
         }
+      }
     }
+  }
+
+  // Whether this lane's part of V holds an infinity or a NaN.
+  __device__ static bool odd(const Tile& x) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // the largest exponent field carries into the sign's place
+        if constexpr (FP8)
+          any |= (x.v[i][e] & 0x7F7F7F7Fu) + 0x01010101u;
+        else
+          any |= (x.v[i][e] & 0x7FFF7FFFu) + 0x04000400u;
+      }
+    return (any & (FP8 ? 0x80808080u : 0x80008000u)) != 0;
   }
 };
 
@@ -233,93 +257,353 @@ __device__ __forceinline__ void set_rows(RowSet& r, const PagedView& c, int b, i
   r.hi_any = hi(r.first + r1 / rep);
 }
 
+// Tiles of each of a sequence's units, 0 for a sequence without new tokens (the
+// rows of others are written even where they see nothing: at least 1).
+template <int TP>
+__device__ __forceinline__ int sequence_tiles(const RowSet& r, int window) {
+  if (r.n == 0) return 0;
+  const int lo = window > 0 ? max(r.first - window + 1, 0) : 0;
+  const int hi = min(max(r.first + r.n, 0), r.cap);
+  return max((hi + TP - 1) / TP - lo / TP, 1);
+}
+
+// Merges pieces (m, l, o) of a row's attention, 4 columns a thread.
+struct Merge {
+  float M = -__builtin_inff(), den = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  __device__ void add(float m, float l, f32x4 v) {
+    const float Mn = fmaxf(M, m), Mf = Mn == -__builtin_inff() ? 0.f : Mn;
+    const float fo = __builtin_amdgcn_exp2f(M - Mf), fn = __builtin_amdgcn_exp2f(m - Mf);
+    den = den * fo + l * fn;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * fo + v[e] * fn;
+    M = Mn;
+  }
+};
+
+// 4 columns of a row's result to memory.
+__device__ __forceinline__ void store_row(__half* dst, f32x4 v, float den, int pos, int cap) {
+  const float inv = 1.f / den;
+  f16x2 y[2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    y[e >> 1][e & 1] = (_Float16)(pos < 0 ? 0.f : pos >= cap ? __builtin_nanf("") : v[e] * inv);
+  *(uint2*)dst = uint2{__builtin_bit_cast(uint32_t, y[0]), __builtin_bit_cast(uint32_t, y[1])};
+}
+
+// The batch's work is a line of tiles: sequence by sequence, unit by unit (KV
+// head fastest), the unit's positions.  It is cut into equal pieces, one a
+// wave, whatever the lengths: 256 workgroups of 8 waves, a wave's piece running
+// over as many units as it does.  A unit inside a piece is written by its wave;
+// one that crosses waves is merged by their workgroup through LDS; one that
+// crosses workgroups goes through memory, and the last one to arrive (an
+// arrival counter, data handed over coherently) merges its parts in order.  So
+// a result's sums depend on the lengths alone, and the workspace holds two
+// parts a workgroup, not a cache's length of them.
+//
+// Where every unit fits a workgroup with at most kPaShort tiles a wave, a unit
+// gets a workgroup of its own, and nothing goes through memory.
+constexpr int kPaShort = 4;
+
 template <int D, bool FP8>
 __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a) {
   using RA = RowAttention<D, FP8>;
-  constexpr int W = kPaThreads / 64;
-  __shared__ float sm[W][kPaRows], sl[W][kPaRows];
-  __shared__ __align__(16) float so[W][kPaRows][D + 4];
+  constexpr int TP = RA::TP, PS = D + 4;
+  struct Seg {  // a unit's piece that did not stay within its wave
+    int b, unit, ended;
+  };
+  extern __shared__ __align__(16) float parts[];  // [wave][2][rows][PS]
+  __shared__ long long scan[kPaWaves];
+  __shared__ int most[kPaWaves], units_sum[kPaWaves];
+  __shared__ long long at_off[kPaWaves];
+  __shared__ int at_seq[kPaWaves];
+  __shared__ Seg seg[kPaWaves][2];
+  __shared__ int flag;
   const PagedView& c = a.c;
-  int slot = blockIdx.x, b;
-  if (c.starts) {
-    b = slot_sequence(c, a.rep, kPaRows, 1, slot);
-    if (slot < 0) return;
-  } else {
-    b = slot / a.tiles_each;
-    slot -= b * a.tiles_each;
-  }
-  const int wave = threadIdx.x >> 6;
-  RA x(c);
-  x.b = b;
-  x.g = blockIdx.y;
-  x.scale2 = a.scale2;
-  set_rows(x.r, c, b, slot, a.rep, a.window, x.li);
-  if (slot * kPaRows >= x.r.n * a.rep) return;  // uniform
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int Hq = c.Hk * a.rep;
-  x.begin(a.q, a.rep, Hq);
-  for (int t = x.r.lo_any / RA::TP + wave; t * RA::TP < x.r.hi_any; t += W) {
-    typename RA::Tile tile;
-    x.load(tile, t);
-    x.step(tile, t);
+
+  // the line: each thread sums a run of sequences
+  const int per = (c.B + kPaThreads - 1) / kPaThreads, b0 = tid * per, b1 = min(b0 + per, c.B);
+  auto weigh = [&](int b, int& tiles, int& units) {
+    RowSet r;
+    r.s0 = c.start(b);
+    r.n = max((c.starts ? c.start(b + 1) : r.s0 + c.each) - r.s0, 0);
+    r.first = c.length(b) - r.n;
+    r.cap = c.max_pages << c.page_shift;
+    tiles = sequence_tiles<TP>(r, a.window);
+    units = (r.n * a.rep + kPaRows - 1) / kPaRows * c.Hk;
+  };
+  long long total = 0, sum = 0;
+  int widest = 0, n_units = 0;
+  for (int b = b0; b < b1; ++b) {
+    int tiles, units;
+    weigh(b, tiles, units);
+    sum += (long long)tiles * units;
+    widest = max(widest, tiles);
+    n_units += units;
   }
-  x.l += __shfl_xor(x.l, 16);
-  x.l += __shfl_xor(x.l, 32);
-  if (x.kb == 0) {
-    sm[wave][x.li] = x.m;
-    sl[wave][x.li] = x.l;
-  }
+  // every unit in a workgroup of its own, or an even cut: `quota` tiles a wave,
+  // a unit's tiles rounded up to `align` of them
+  auto scan_line = [&](long long mine, long long& before) {
+    long long v = mine;
 #pragma unroll
-  for (int i = 0; i < RA::NC; ++i) *(f32x4*)&so[wave][x.li][16 * i + 4 * x.kb] = x.o[i];
-  __syncthreads();
-  // thread (row, 4 columns a step)
-  const int row = threadIdx.x >> 4, r = slot * kPaRows + row;
-  if (r >= x.r.n * a.rep) return;
-  float M = -__builtin_inff();
-#pragma unroll
-  for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w][row]);
-  const float Mf = M == -__builtin_inff() ? 0.f : M;
-  float f[W], den = 0.f;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    f[w] = __builtin_amdgcn_exp2f(sm[w][row] - Mf);
-    den = fmaf(sl[w][row], f[w], den);
-  }
-  const int tok = r / a.rep, pos = x.r.first + tok;
-  const bool none = pos < 0, beyond = pos >= x.r.cap;
-  const float inv = 1.f / den;
-  __half* dst = a.out + ((int64_t)(x.r.s0 + tok) * Hq + x.g * a.rep + r % a.rep) * D;
-  for (int d = 4 * (threadIdx.x & 15); d < D; d += 64) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const f32x4 ow = *(const f32x4*)&so[w][row][d];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(ow[e], f[w], v[e]);
+    for (int o = 1; o < 64; o <<= 1) {
+      const long long u = __shfl_up(v, o);
+      if (lane >= o) v += u;
     }
-    f16x2 y[2];
+    __syncthreads();
+    if (lane == 63) scan[wave] = v;
+    __syncthreads();
+    before = v - mine;
+    long long all = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      y[e >> 1][e & 1] = (_Float16)(none ? 0.f : beyond ? __builtin_nanf("") : v[e] * inv);
-    *(uint2*)(dst + d) = uint2{__builtin_bit_cast(uint32_t, y[0]), __builtin_bit_cast(uint32_t, y[1])};
+    for (int w = 0; w < kPaWaves; ++w) {
+      if (w < wave) before += scan[w];
+      all += scan[w];
+    }
+    return all;
+  };
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    widest = max(widest, __shfl_xor(widest, o));
+    n_units += __shfl_xor(n_units, o);
+  }
+  if (lane == 0) {
+    most[wave] = widest;
+    units_sum[wave] = n_units;
+  }
+  long long before;
+  total = scan_line(sum, before);
+  widest = n_units = 0;
+#pragma unroll
+  for (int w = 0; w < kPaWaves; ++w) {
+    widest = max(widest, most[w]);
+    n_units += units_sum[w];
+  }
+  const bool own = n_units <= (int)gridDim.x && widest <= kPaShort * kPaWaves;
+  const long long waves = (long long)gridDim.x * kPaWaves;
+  long long quota = own ? (widest + kPaWaves - 1) / kPaWaves
+                        : (total + waves - 1) / waves;
+  const int align = own ? (int)quota * kPaWaves : 1;
+  auto rounded = [&](int tiles) { return (tiles + align - 1) / align * align; };
+  if (own) {
+    sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      int tiles, units;
+      weigh(b, tiles, units);
+      sum += (long long)rounded(tiles) * units;
+    }
+    total = scan_line(sum, before);
+  }
+  const long long wg_quota = quota * kPaWaves, wg0 = blockIdx.x * wg_quota;
+  if (wg0 >= total) return;  // uniform
+  // where each wave's piece begins
+  if (tid < kPaWaves) at_seq[tid] = -1;
+  __syncthreads();
+  for (int b = b0; b < b1; ++b) {
+    int tiles, units;
+    weigh(b, tiles, units);
+    const long long w = (long long)rounded(tiles) * units;
+#pragma unroll
+    for (int v = 0; v < kPaWaves; ++v) {
+      const long long p = wg0 + v * quota;
+      if (p >= before && p < before + w) {
+        at_seq[v] = b;
+        at_off[v] = p - before;
+      }
+    }
+    before += w;
+  }
+  if (tid < 2 * kPaWaves) seg[tid >> 1][tid & 1].unit = -1;
+  __syncthreads();
+
+  RA x(c);
+  x.scale2 = a.scale2;
+  x.rep = a.rep;
+  x.window = a.window;
+  {
+    int b = __builtin_amdgcn_readfirstlane(at_seq[wave]);
+    auto uniform = [](long long v) {
+      return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                         (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+    };
+    long long off = b >= 0 ? uniform(at_off[wave]) : 0, left = uniform(quota);
+    while (b >= 0 && b < c.B && left > 0) {  // (bounded: b grows, or off to its end)
+      int tiles, units;
+      weigh(b, tiles, units);
+      const int size = rounded(tiles);
+      if (off >= (long long)size * units) {
+        ++b;
+        off = 0;
+        continue;
+      }
+      const int unit = (int)(off / size), t0 = (int)(off - (long long)unit * size);
+      const int run = (int)min((long long)(size - t0), left), t1 = min(t0 + run, tiles);
+      off += run;
+      left -= run;
+      if (t0 >= t1) continue;
+      const int qt = unit / c.Hk;
+      x.b = b;
+      x.g = unit - qt * c.Hk;
+      set_rows(x.r, c, b, qt, a.rep, a.window, x.li);
+      x.begin(a.q, Hq);
+      const int first = (a.window > 0 ? max(x.r.first - a.window + 1, 0) : 0) / TP;
+      // k and v of the next tile are fetched as soon as the present one's have
+      // been used, page ids a tile before them
+      {
+        const int e = first + t1;
+        int t = first + t0;
+        typename RA::Tile tile;
+        typename RA::Ids id = x.ids(t), ahead = x.ids(t + 1);
+        x.load_k(tile, t, id);
+        x.load_v(tile, t, id);
+        for (; t < e; ++t) {
+          x.step(tile, t, [&] {
+            if (t + 1 < e) {
+              id = ahead;
+              ahead = x.ids(t + 2);
+              x.load_k(tile, t + 1, id);
+            }
+          });
+          if (t + 1 < e) x.load_v(tile, t + 1, id);
+        }
+      }
+      x.l += __shfl_xor(x.l, 16);
+      x.l += __shfl_xor(x.l, 32);
+      if (t0 == 0 && t1 == tiles) {
+        if (x.r.live) {
+          const int tok = x.r.row / a.rep;
+          __half* dst = a.out + ((int64_t)(x.r.s0 + tok) * Hq + x.g * a.rep + x.r.row % a.rep) * D;
+#pragma unroll
+          for (int i = 0; i < RA::NC; ++i)
+            store_row(dst + 16 * i + 4 * x.kb, x.o[i], x.l, x.r.first + tok, x.r.cap);
+        }
+      } else {
+        const int s = t0 == 0;
+        if (x.li < a.rows) {
+          float* mine = parts + ((wave * 2 + s) * a.rows + x.li) * PS;
+#pragma unroll
+          for (int i = 0; i < RA::NC; ++i) *(f32x4*)(mine + 16 * i + 4 * x.kb) = x.o[i];
+          if (x.kb == 0) {
+            mine[D] = x.m;
+            mine[D + 1] = x.l;
+          }
+        }
+        if (lane == 0) seg[wave][s] = Seg{b, unit, t1 == tiles};
+      }
+    }
+  }
+  __syncthreads();
+  // Chains of pieces of one unit: the one that the workgroup begins in, and
+  // those that begin in a wave.  Thread (row, 4 columns).
+  const int row = tid / (D / 4), d4 = 4 * (tid % (D / 4));
+  for (int v = -1; v < kPaWaves; ++v) {  // uniform
+    const int v0 = max(v, 0), s0 = v < 0 ? 0 : 1;
+    const Seg head = seg[v0][s0];
+    if (head.unit < 0) continue;
+    const bool began = v >= 0;
+    bool ended = head.ended;
+    int v1 = v0 + 1;
+    while (!ended && v1 < kPaWaves && seg[v1][0].unit >= 0) ended = seg[v1++][0].ended;
+    RowSet r;
+    const int qt = head.unit / c.Hk, g = head.unit - qt * c.Hk;
+    set_rows(r, c, head.b, qt, a.rep, a.window, row & 15);
+    const bool mine = row < kPaRows && r.live;
+    Merge acc;
+    if (mine) {
+      for (int w = v0; w < v1; ++w) {
+        const float* p = parts + ((w * 2 + (w == v0 ? s0 : 0)) * a.rows + row) * PS;
+        acc.add(p[D], p[D + 1], *(const f32x4*)(p + d4));
+      }
+    }
+    if (!(began && ended)) {
+      // to memory; the last workgroup of the unit merges its parts in order
+      float* my = a.part + ((int64_t)(blockIdx.x * 2 + began) * kPaRows + row) * PS;
+      if (mine) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) handoff_put(my + d4 + e, acc.o[e]);
+        if (d4 == 0) {
+          handoff_put(my + D, acc.M);
+          handoff_put(my + D + 1, acc.den);
+        }
+      }
+      int tiles, units;
+      weigh(head.b, tiles, units);
+      // the unit's place on the line, from a piece of this workgroup's
+      const long long base = wg0 + v0 * quota - at_off[v0];  // (at_seq[v0] begins here)
+      long long u0;
+      if (at_seq[v0] == head.b) {
+        u0 = base + (long long)head.unit * tiles;
+      } else {  // the sequence begins inside wave v0's piece
+        u0 = base;
+        for (int b = at_seq[v0]; b < head.b; ++b) {
+          int t, u;
+          weigh(b, t, u);
+          u0 += (long long)t * u;
+        }
+        u0 += (long long)head.unit * tiles;
+      }
+      const int w0 = (int)(u0 / wg_quota), w1 = (int)((u0 + tiles - 1) / wg_quota);
+      const int slot = c.starts ? (int)((int64_t)r.s0 * a.rep / kPaRows) + head.b
+                                : head.b * a.tiles_each;
+      unsigned* cnt = a.count + (int64_t)(slot + qt) * c.Hk + g;
+      if (!handoff_arrive(cnt, (unsigned)(w1 - w0 + 1), &flag)) continue;
+      acc = Merge();
+      const float* p0 = a.part + (int64_t)(row & 15) * PS;
+      for (int w = w0; w <= w1; w += 8) {
+        float m[8], l[8];
+        f32x4 o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int ww = min(w + j, w1);
+          const float* p = p0 + (int64_t)(ww * 2 + (ww == w0)) * (kPaRows * PS);
+          m[j] = handoff_get(p + D);
+          l[j] = handoff_get(p + D + 1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j][e] = handoff_get(p + d4 + e);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (w + j <= w1) acc.add(m[j], l[j], o[j]);
+      }
+      if (tid == 0) handoff_reset(cnt);
+    }
+    if (mine) {
+      const int tok = r.row / a.rep;
+      store_row(a.out + ((int64_t)(r.s0 + tok) * Hq + g * a.rep + r.row % a.rep) * D + d4, acc.o,
+                acc.den, r.first + tok, r.cap);
+    }
   }
 }
 
 }  // namespace
 }  // namespace glq
 
-extern "C" int64_t glq_paged_attention_workspace_bytes(int64_t seqs, int64_t tokens,
-                                                       int64_t q_heads, int64_t kv_heads,
-                                                       int64_t head_dim) {
-  if (seqs < 0 || tokens < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0) return -1;
-  return 256;
+extern "C" int64_t glq_paged_attention_scratch_bytes(void) {
+  using namespace glq;
+  return (int64_t)kPaGrid * 2 * kPaRows * (128 + 4) * 4;
 }
 
-extern "C" int glq_paged_attention(const glq_paged_cache* cache, const int32_t* starts,
-                                   int64_t tokens, const void* q, int64_t q_heads, float scale,
-                                   int64_t window, void* out, void* workspace,
-                                   int64_t workspace_bytes, void* stream) {
+extern "C" int64_t glq_paged_attention_workspace_bytes(int64_t seqs, int64_t tokens,
+                                                       int64_t q_heads, int64_t kv_heads) {
+  using namespace glq;
+  if (seqs < 0 || tokens < 0 || q_heads <= 0 || kv_heads <= 0) return -1;
+  // a counter a unit: at most rows / 16 + 1 units a sequence and KV head
+  const int64_t rep = (q_heads + kv_heads - 1) / kv_heads;
+  const int64_t units = (tokens * rep / kPaRows + seqs) * kv_heads;
+  return glq_paged_attention_scratch_bytes() + align_up(4 * units, 256);
+}
+
+extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* stream) {
   using namespace glq;
   clear_error();
+  GLQ_CHECK(p != nullptr, "null params");
+  const glq_paged_cache* cache = &p->cache;
+  const int32_t* starts = p->starts;
+  const int64_t tokens = p->tokens, q_heads = p->q_heads, window = p->window;
+  const void* q = p->q;
+  void* out = p->out;
   PagedAttnArgs a{};
   if (int rc = paged_view(cache, starts, tokens, a.c)) return rc;
   const int64_t D = cache->head_dim, Hk = cache->kv_heads;
@@ -330,22 +614,27 @@ extern "C" int glq_paged_attention(const glq_paged_cache* cache, const int32_t* 
   GLQ_CHECK(q && out && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0,
             "q and out must be non-null and 16-byte aligned");
   const int64_t need =
-      glq_paged_attention_workspace_bytes(cache->seqs, tokens, q_heads, Hk, D);
-  GLQ_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0,
+      glq_paged_attention_workspace_bytes(cache->seqs, tokens, q_heads, Hk);
+  GLQ_CHECK(p->workspace && p->workspace_bytes >= need && ((uintptr_t)p->workspace & 255) == 0,
             "a 256-byte aligned workspace of %lld bytes needed (got %lld)", (long long)need,
-            (long long)workspace_bytes);
+            (long long)p->workspace_bytes);
   a.q = (const __half*)q;
   a.out = (__half*)out;
   a.rep = (int)(q_heads / Hk);
   a.window = window >= cache->max_pages * cache->page_size ? 0 : (int)window;
-  a.scale2 = scale * 1.44269504088896f;
+  a.scale2 = p->scale * 1.44269504088896f;
   GLQ_CHECK(tokens * a.rep < (1ll << 30), "batch of too many (token, head) rows");
-  a.tiles_each = (int)(((int64_t)a.c.each * a.rep + kPaRows - 1) / kPaRows);
-  const int64_t slots = starts ? tokens * a.rep / kPaRows + cache->seqs : cache->seqs * a.tiles_each;
-  GLQ_CHECK(slots < (1ll << 24) && Hk <= 65535, "batch of too many query rows");
+  const int64_t rows_each = (int64_t)a.c.each * a.rep;
+  a.tiles_each = (int)((rows_each + kPaRows - 1) / kPaRows);
+  a.rows = !starts && rows_each <= 8 ? 8 : kPaRows;
+  a.part = (float*)p->workspace;
+  a.count = (unsigned*)((char*)p->workspace + glq_paged_attention_scratch_bytes());
+  const size_t lds = (size_t)kPaWaves * 2 * a.rows * (D + 4) * 4;
   auto kern = D == 128 ? (a.c.ks ? paged_rows_kernel<128, true> : paged_rows_kernel<128, false>)
                        : (a.c.ks ? paged_rows_kernel<64, true> : paged_rows_kernel<64, false>);
-  kern<<<dim3((unsigned)slots, (unsigned)Hk), dim3(kPaThreads), 0, (hipStream_t)stream>>>(a);
+  static size_t attr[4] = {64 * 1024, 64 * 1024, 64 * 1024, 64 * 1024};
+  if (int rc = set_lds_limit(kern, lds, attr[(D == 64) * 2 + !a.c.ks])) return rc;
+  kern<<<dim3(kPaGrid), dim3(kPaThreads), lds, (hipStream_t)stream>>>(a);
   GLQ_LAUNCH_CHECK("paged_rows_kernel");
   return GLQ_OK;
 }

@@ -22,6 +22,7 @@ replays of a captured graph.  Rows behind starts[B] are left as they were.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -30,8 +31,19 @@ from . import _require, _zeroed_buffer
 
 BLOCK = 16  # tokens of a scale block
 
+_FP8, _FP16, _E8M0 = torch.float8_e4m3fn, torch.float16, torch.float8_e8m0fnu
+
+# The C ABI's parameter structures, packed in one go (a ctypes.Structure costs
+# about 4 us of host time a call, this 1): glq_paged_cache, then the call's own.
+_CACHE = "6P7q"
+_append_params = struct.Struct(_CACHE + "Pq3P5q4PqPfi").pack
+_attention_params = struct.Struct(_CACHE + "Pq2P2qPqfi").pack
+assert struct.calcsize(_CACHE + "Pq3P5q4PqPfi") == ctypes.sizeof(_lib.PagedAppendParams)
+assert struct.calcsize(_CACHE + "Pq2P2qPqfi") == ctypes.sizeof(_lib.PagedAttentionParams)
+
 # attention workspaces: (device index, stream handle) -> zero-filled uint8 tensor
 _workspaces: dict = {}
+_ws_bytes: dict = {}
 
 
 def paged_cache_tensors(pages: int, kv_heads: int, head_dim: int = 128, page_size: int = 64,
@@ -58,73 +70,99 @@ def paged_cache_tensors(pages: int, kv_heads: int, head_dim: int = 128, page_siz
     return k, v, ks, vs
 
 
-def _same_device(dev, named) -> None:
-    for t, n in named:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{n} is on {t.device}, the pages on {dev}")
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _check(t, name, dev, dtype) -> None:
+    """A contiguous tensor of the pages' device and this type (the common case
+    first: the checks are on the path of every decode step)."""
+    if type(t) is torch.Tensor and t.get_device() == dev and t.dtype is dtype \
+            and t.is_contiguous():
+        return
+    _require(t, name, dtype)
+    if t.get_device() != dev:
+        raise RuntimeError(f"{name} is on {t.device}, the pages on cuda:{dev}")
 
 
 def _cache_view(k_pages, v_pages, k_scales, v_scales, page_table, lengths, starts, T):
-    """The C ABI's cache descriptor, checked; (descriptor, heads, head_dim)."""
-    _require(k_pages, "k_pages")
-    if k_pages.dtype not in (torch.float16, torch.float8_e4m3fn):
-        raise RuntimeError(f"k_pages must be float16 or float8_e4m3fn (got {k_pages.dtype})")
-    _require(v_pages, "v_pages", k_pages.dtype)
-    if k_pages.dim() != 4:
+    """The cache's checks: the C ABI's descriptor (its 13 values), the pages'
+    device index, KV heads and head width."""
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
         raise RuntimeError("k_pages must be (pages, Hk, page, D)")
+    dtype, dev = k_pages.dtype, k_pages.get_device()
+    if dtype is not _FP8 and dtype is not _FP16:
+        raise RuntimeError(f"k_pages must be float16 or float8_e4m3fn (got {dtype})")
+    if dev < 0:
+        raise RuntimeError("k_pages must be a GPU tensor (glorcq_amd runs on the GPU only)")
+    _check(k_pages, "k_pages", dev, dtype)
+    _check(v_pages, "v_pages", dev, dtype)
     pages, Hk, page, D = k_pages.shape
+    blocks = page // BLOCK
     if page < BLOCK or page > 1024 or page & (page - 1):
         raise RuntimeError(f"a page holds a power of two of tokens in [16, 1024] (got {page})")
-    if tuple(v_pages.shape) != (pages, Hk, page // BLOCK, D, BLOCK):
-        raise RuntimeError(f"v_pages must be ({pages}, {Hk}, {page // BLOCK}, {D}, {BLOCK})")
-    if k_pages.dtype == torch.float16:
+    if v_pages.shape != (pages, Hk, blocks, D, BLOCK):
+        raise RuntimeError(f"v_pages must be ({pages}, {Hk}, {blocks}, {D}, {BLOCK})")
+    if dtype is _FP16:
         if k_scales is not None or v_scales is not None:
             raise RuntimeError("fp16 pages have no scales")
     else:
         for s, n in ((k_scales, "k_scales"), (v_scales, "v_scales")):
             if s is None:
                 raise RuntimeError(f"8-bit pages need {n}")
-            _require(s, n, torch.float8_e8m0fnu)
-            if tuple(s.shape) != (pages, Hk, page // BLOCK):
-                raise RuntimeError(f"{n} must be ({pages}, {Hk}, {page // BLOCK})")
-    if not isinstance(page_table, torch.Tensor) or not page_table.is_cuda \
-            or page_table.dtype != torch.int32 or page_table.dim() != 2 \
-            or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise RuntimeError("page_table must be a GPU int32 tensor (B, n) of contiguous rows")
-    _require(lengths, "lengths", torch.int32)
+            _check(s, n, dev, _E8M0)
+            if s.shape != (pages, Hk, blocks):
+                raise RuntimeError(f"{n} must be ({pages}, {Hk}, {blocks})")
+    if not isinstance(page_table, torch.Tensor) or page_table.get_device() != dev \
+            or page_table.dtype is not torch.int32 or page_table.dim() != 2:
+        raise RuntimeError(f"page_table must be an int32 tensor (B, n) on cuda:{dev}")
     B, n = page_table.shape
-    if tuple(lengths.shape) != (B,):
+    stride, one = page_table.stride()
+    if B <= 1:
+        stride = n
+    if (one != 1 and n > 1) or stride < n:
+        raise RuntimeError("page_table must have contiguous rows that do not overlap")
+    _check(lengths, "lengths", dev, torch.int32)
+    if lengths.shape != (B,):
         raise RuntimeError(f"lengths must be ({B},)")
     if starts is not None:
-        _require(starts, "starts", torch.int32)
-        if tuple(starts.shape) != (B + 1,):
+        _check(starts, "starts", dev, torch.int32)
+        if starts.shape != (B + 1,):
             raise RuntimeError(f"starts must be ({B + 1},)")
     elif T % B if B else T:
         raise RuntimeError(f"{T} rows do not divide over {B} sequences (give starts)")
-    _same_device(k_pages.device, ((v_pages, "v_pages"), (k_scales, "k_scales"),
-                                  (v_scales, "v_scales"), (page_table, "page_table"),
-                                  (lengths, "lengths"), (starts, "starts")))
-    stride = page_table.stride(0) if B > 1 else n
-    if stride < n:
-        raise RuntimeError("page_table rows overlap")
-    return _lib.PagedCache(
-        k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(k_scales), _lib.ptr(v_scales),
-        page_table.data_ptr(), lengths.data_ptr(), B, n, stride, pages, Hk, D, page), Hk, D
+    return (k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+            page_table.data_ptr(), lengths.data_ptr(), B, n, stride, pages, Hk, D, page), dev, Hk, D
 
 
-def _rows(t, name, width):
-    """(T, ...) rows of `width` values, each contiguous: (T, row stride)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float16:
-        raise RuntimeError(f"{name} must be a GPU float16 tensor")
-    if t.dim() == 3 and t.shape[1] * t.shape[2] == width:  # (T, heads, D)
-        if t.numel() and t.shape[1] > 1 and t.stride(1) != t.shape[2]:
+def _rows(t, name, width, dev):
+    """(T, width) rows, or (T, heads, D) ones, each contiguous: T, row stride."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype is not _FP16:
+        raise RuntimeError(f"{name} must be a float16 tensor on the pages' GPU, cuda:{dev}")
+    nd = t.dim()
+    if nd == 3 and t.shape[1] * t.shape[2] == width:
+        T, heads, D = t.shape
+        stride, head, one = t.stride()
+        if T and heads > 1 and head != D:
             raise RuntimeError(f"{name}'s heads must be contiguous within a row")
-    elif t.dim() != 2 or t.shape[1] != width:
+    elif nd == 2 and t.shape[1] == width:
+        T = t.shape[0]
+        stride, one = t.stride()
+    else:
         raise RuntimeError(f"{name} must be (T, {width}) (got {tuple(t.shape)})")
-    if t.stride(-1) != 1 and t.numel():
+    if one != 1 and T:
         raise RuntimeError(f"{name} must have contiguous rows")
-    T = t.shape[0]
-    return T, t.stride(0) if T > 1 else width
+    return T, stride if T > 1 else width
+
+
+def _launch(fn, name, params, dev) -> None:
+    if torch.cuda.current_device() == dev:
+        rc = fn(params, _lib.stream_handle(torch.device("cuda", dev)))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(params, _lib.stream_handle(torch.device("cuda", dev)))
+    if rc:
+        _lib.check(rc, name)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -136,89 +174,100 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                  eps: float = 1e-6, q_out: torch.Tensor | None = None):
     """Writes the new tokens' k (T, Hk*D) and v into their positions' pages,
     one launch (glq_paged_append): each k head normalized (k_norm_w (D,), None:
-    not) and rotated (cos/sin (T or 1, D), None: not) in fp32 and rounded once
-    to the pages' type; with q (T, Hq*D) -- or item-major (n, T, R), a batched
-    GEMV's output over R-row slices -- its heads likewise, returned as q_out
-    (T, Hq, D) fp16 (else None).  Rows of k, v and q may be slices of a wider
-    matrix.  8-bit pages: a block's scale is the smallest power of two that
-    takes its values to e4m3's 448; tokens that a block already had are scaled
-    along when it grows.  Infinities and NaN are stored as NaN."""
+    not) and rotated (cos/sin (T or 1, D), None: not) and rounded once to the
+    pages' type; with q (T, Hq*D) -- or item-major (n, T, R), a batched GEMV's
+    output over R-row slices -- its heads likewise, returned as q_out (T, Hq, D)
+    fp16 (else None).  Rows of k, v and q may be slices of a wider matrix.
+    8-bit pages: a block's scale is the smallest power of two that takes its
+    values to e4m3's 448; tokens that a block already had are scaled along when
+    it grows.  Infinities and NaN are stored as NaN.  Pages that get tokens must
+    belong to one sequence."""
     lib = _lib.load()
-    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
-        raise RuntimeError("k_pages must be (pages, Hk, page, D)")
-    width = k_pages.shape[1] * k_pages.shape[3]
-    T, k_stride = _rows(k, "k", width)
-    Tv, v_stride = _rows(v, "v", width)
+    if not isinstance(k, torch.Tensor):
+        raise RuntimeError("k must be a tensor")
+    T = k.shape[0] if k.dim() else 0
+    cache, dev, Hk, D = _cache_view(k_pages, v_pages, k_scales, v_scales, page_table, lengths,
+                                    starts, T)
+    T, k_stride = _rows(k, "k", Hk * D, dev)
+    Tv, v_stride = _rows(v, "v", Hk * D, dev)
     if Tv != T:
         raise RuntimeError(f"k has {T} rows, v {Tv}")
-    view, Hk, D = _cache_view(k_pages, v_pages, k_scales, v_scales, page_table, lengths, starts, T)
-    for w, n in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
-        if w is not None:
-            _require(w, n, torch.float16)
-            if tuple(w.shape) != (D,):
-                raise RuntimeError(f"{n} must be ({D},)")
+    if k_norm_w is not None:
+        _check(k_norm_w, "k_norm_w", dev, _FP16)
+        if k_norm_w.shape != (D,):
+            raise RuntimeError(f"k_norm_w must be ({D},)")
     if (cos is None) != (sin is None):
         raise RuntimeError("cos and sin come together")
     cs_stride = 0
     if cos is not None:
-        _require(cos, "cos", torch.float16)
-        _require(sin, "sin", torch.float16)
-        if cos.shape[-1] != D or sin.shape != cos.shape or cos.numel() // D not in (1, T):
+        _check(cos, "cos", dev, _FP16)
+        _check(sin, "sin", dev, _FP16)
+        n = cos.numel()
+        if cos.shape[-1:] != (D,) or sin.shape != cos.shape or (n != D and n != T * D):
             raise RuntimeError(f"cos and sin must hold 1 or {T} rows of {D}")
-        cs_stride = D if cos.numel() // D > 1 else 0
+        cs_stride = D if n > D else 0
     Hq = item_rows = q_stride = 0
     if q is not None:
         if not isinstance(q, torch.Tensor) or q.dim() not in (2, 3):
             raise RuntimeError("q must be (T, Hq*D), (T, Hq, D) or item-major (n, T, R)")
         if q.dim() == 3 and q.shape[2] != D and q.shape[1] == T:  # item-major
-            _require(q, "q", torch.float16)
+            _check(q, "q", dev, _FP16)
             item_rows = q.shape[2]
             if item_rows % D:
                 raise RuntimeError(f"q's items must be of whole heads ({D})")
             Hq = q.shape[0] * item_rows // D
         else:
-            Hq = q.shape[1:].numel() // D
-            Tq, q_stride = _rows(q, "q", Hq * D)
+            Hq = (q.shape[1] if q.dim() == 2 else q.shape[1] * q.shape[2]) // D
+            Tq, q_stride = _rows(q, "q", Hq * D, dev)
             if Tq != T:
                 raise RuntimeError(f"k has {T} rows, q {Tq}")
         if Hq == 0 or Hq % Hk:
             raise RuntimeError(f"q's heads ({Hq}) must be a multiple of the KV heads ({Hk})")
+        if q_norm_w is not None:
+            _check(q_norm_w, "q_norm_w", dev, _FP16)
+            if q_norm_w.shape != (D,):
+                raise RuntimeError(f"q_norm_w must be ({D},)")
         if q_out is None:
-            q_out = torch.empty(T, Hq, D, dtype=torch.float16, device=k.device)
+            q_out = q.new_empty((T, Hq, D))
         else:
-            _require(q_out, "q_out", torch.float16)
+            _check(q_out, "q_out", dev, _FP16)
             if q_out.numel() != T * Hq * D:
                 raise RuntimeError(f"q_out must be ({T}, {Hq}, {D})")
     elif q_out is not None or q_norm_w is not None:
         raise RuntimeError("q_out and q_norm_w need a q")
-    dev = k_pages.device
-    _same_device(dev, ((k, "k"), (v, "v"), (q, "q"), (cos, "cos"), (sin, "sin"),
-                       (q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w"), (q_out, "q_out")))
-    with torch.cuda.device(dev):
-        _lib.check(lib.glq_paged_append(
-            ctypes.byref(view), _lib.ptr(starts), T, k.data_ptr(), k_stride, v.data_ptr(),
-            v_stride, _lib.ptr(q), Hq, q_stride, item_rows, _lib.ptr(q_norm_w),
-            _lib.ptr(k_norm_w), float(eps), _lib.ptr(cos), _lib.ptr(sin), cs_stride,
-            _lib.ptr(q_out), _lib.stream_handle(dev)), "glq_paged_append")
+    _launch(lib.glq_paged_append, "glq_paged_append", _append_params(
+        *cache, _ptr(starts), T, k.data_ptr(), v.data_ptr(), _ptr(q), k_stride, v_stride, q_stride,
+        Hq, item_rows, _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos), _ptr(sin), cs_stride,
+        _ptr(q_out), eps, 0), dev)
     return q_out
+
+
+def _workspace_bytes(B, T, Hq, Hk) -> int:
+    """glq_paged_attention_workspace_bytes, memoized (a function of its sizes)."""
+    n = _ws_bytes.get((B, T, Hq, Hk))
+    if n is None:
+        n = _lib.load().glq_paged_attention_workspace_bytes(B, T, Hq, Hk)
+        if n < 0:
+            raise RuntimeError("invalid paged attention shapes")
+        n = _ws_bytes[(B, T, Hq, Hk)] = max(int(n), 256)
+    return n
+
+
+def _new_workspace(n: int, dev: int) -> torch.Tensor:
+    """A workspace whose counters, the part behind its scratch, are zero."""
+    ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", dev))
+    ws[_lib.load().glq_paged_attention_scratch_bytes():].zero_()
+    return ws
 
 
 def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor,
                               page_table: torch.Tensor) -> torch.Tensor:
-    """A zeroed workspace for paged_attention at these shapes (keep it for the
-    calls that follow: every call leaves its counters zero, and calls that
-    share it must not overlap)."""
-    D = k_pages.shape[3]
-    n = _workspace_bytes(page_table.shape[0], q.shape[0], q.shape[1:].numel() // D,
-                         k_pages.shape[1], D)
-    return torch.zeros(n, dtype=torch.uint8, device=k_pages.device)
-
-
-def _workspace_bytes(B, T, Hq, Hk, D) -> int:
-    n = _lib.load().glq_paged_attention_workspace_bytes(B, T, Hq, Hk, D)
-    if n < 0:
-        raise RuntimeError("invalid paged attention shapes")
-    return max(int(n), 256)
+    """A workspace for paged_attention at these shapes (keep it for the calls
+    that follow: every call leaves its counters zero, and calls that share it
+    must not overlap)."""
+    return _new_workspace(_workspace_bytes(page_table.shape[0], q.shape[0],
+                                           q.shape[1:].numel() // k_pages.shape[3],
+                                           k_pages.shape[1]), k_pages.get_device())
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -235,37 +284,35 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     capture one of the call's own, so that graphs may be replayed on several
     streams."""
     lib = _lib.load()
-    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
-        raise RuntimeError("k_pages must be (pages, Hk, page, D)")
-    _require(q, "q", torch.float16)
-    D = k_pages.shape[3]
-    if q.dim() not in (2, 3) or (q.dim() == 3 and q.shape[2] != D) or q.shape[1:].numel() % D:
+    if not isinstance(q, torch.Tensor) or q.dim() not in (2, 3):
+        raise RuntimeError("q must be (T, Hq, D) or (T, Hq*D)")
+    T = q.shape[0]
+    cache, dev, Hk, D = _cache_view(k_pages, v_pages, k_scales, v_scales, page_table, lengths,
+                                    starts, T)
+    _check(q, "q", dev, _FP16)
+    width = q.shape[1] if q.dim() == 2 else q.shape[1] * q.shape[2]
+    if width % D or (q.dim() == 3 and q.shape[2] != D):
         raise RuntimeError(f"q must be (T, Hq, {D}) or (T, Hq*{D})")
-    T, Hq = q.shape[0], q.shape[1:].numel() // D
-    view, Hk, D = _cache_view(k_pages, v_pages, k_scales, v_scales, page_table, lengths, starts, T)
+    Hq = width // D
     if Hq == 0 or Hq % Hk:
         raise RuntimeError(f"q's heads ({Hq}) must be a multiple of the KV heads ({Hk})")
     if window < 0:
         raise RuntimeError("window must be >= 0 (0: none)")
-    dev = k_pages.device
     if out is None:
-        out = torch.empty(T, Hq * D, dtype=torch.float16, device=dev)
+        out = q.new_empty((T, width))
     else:
-        _require(out, "out", torch.float16)
-        if out.numel() != T * Hq * D or out.shape[0] != T:
-            raise RuntimeError(f"out must be ({T}, {Hq * D})")
-    _same_device(dev, ((q, "q"), (out, "out"), (workspace, "workspace")))
-    with torch.cuda.device(dev):
-        if workspace is None:
-            n = _workspace_bytes(view.seqs, T, Hq, Hk, D)
-            if torch.cuda.is_current_stream_capturing():
-                workspace = torch.zeros(n, dtype=torch.uint8, device=dev)
-            else:
-                workspace = _zeroed_buffer(_workspaces, dev, n)
+        _check(out, "out", dev, _FP16)
+        if out.dim() == 0 or out.shape[0] != T or out.numel() != T * width:
+            raise RuntimeError(f"out must be ({T}, {width})")
+    if workspace is None:
+        n = _workspace_bytes(cache[6], T, Hq, Hk)
+        if torch.cuda.is_current_stream_capturing():
+            workspace = _new_workspace(n, dev)
         else:
-            _require(workspace, "workspace", torch.uint8)
-        _lib.check(lib.glq_paged_attention(
-            ctypes.byref(view), _lib.ptr(starts), T, q.data_ptr(), Hq, float(scale), int(window),
-            out.data_ptr(), workspace.data_ptr(), workspace.numel(), _lib.stream_handle(dev)),
-            "glq_paged_attention")
+            workspace = _zeroed_buffer(_workspaces, torch.device("cuda", dev), n)
+    else:
+        _check(workspace, "workspace", dev, torch.uint8)
+    _launch(lib.glq_paged_attention, "glq_paged_attention", _attention_params(
+        *cache, _ptr(starts), T, q.data_ptr(), out.data_ptr(), Hq, window, workspace.data_ptr(),
+        workspace.numel(), scale, 0), dev)
     return out

@@ -774,23 +774,34 @@ typedef struct glq_paged_cache {
  * launch: for each head of q and k,
  *   x' = rope(x rsqrt(mean(x^2) + eps) w),  rope(y) = y cos + rotate_half(y) sin
  * (norm weights of head_dim fp16, NULL: no norm; cos/sin rows of head_dim fp16,
- * one a token, cs_stride apart, 0 for one row for all, NULL: no rotation), in
- * fp32, rounded once: q' to q_out (tokens, q_heads, head_dim) fp16, k' and v to
- * their places in the pages.  q may be NULL (nothing is rotated).  8-bit pages:
- * a block's scale is the smallest 2^e >= amax / 448 (e >= -32) of its finite
- * values that no token before it needed larger; a block that had tokens keeps
- * a larger scale, and is scaled down by the power of two where the new ones
- * need more (e4m3 subnormals are then rounded again).  Infinities and NaN are
- * stored as NaN.  What lies behind a sequence's last token in its block
+ * one a token, cs_stride apart, 0 for one row for all, NULL: no rotation), k in
+ * fp64, q in fp32, rounded once: q' to q_out (tokens, q_heads, head_dim) fp16,
+ * k' and v to their places in the pages.  q may be NULL (nothing is rotated).
+ * 8-bit pages: a block's scale is the smallest 2^e >= amax / 448 (e >= -32) of
+ * its finite values that no token before it needed larger; a block that had
+ * tokens keeps a larger scale, and is scaled down by the power of two where the
+ * new ones need more (e4m3 subnormals are then rounded again).  Infinities and
+ * NaN are stored as NaN.  What lies behind a sequence's last token in its block
  * becomes zero.  Rows of k, v and q are k_stride, v_stride and q_stride values
  * apart (multiples of 8); with q_item_rows > 0, q is item-major as in
  * glq_qk_norm_rope.  Pages that get tokens must belong to one sequence.
  */
-int glq_paged_append(const glq_paged_cache* cache, const int32_t* starts, int64_t tokens,
-                     const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                     const void* q, int64_t q_heads, int64_t q_stride, int64_t q_item_rows,
-                     const void* q_norm_w, const void* k_norm_w, float eps, const void* cos,
-                     const void* sin, int64_t cs_stride, void* q_out, void* stream);
+typedef struct glq_paged_append_params {
+  glq_paged_cache cache;
+  const int32_t* starts;
+  int64_t tokens;
+  const void *k, *v, *q;
+  int64_t k_stride, v_stride, q_stride;
+  int64_t q_heads, q_item_rows;
+  const void *q_norm_w, *k_norm_w;
+  const void *cos, *sin;
+  int64_t cs_stride;
+  void* q_out;
+  float eps;
+  int32_t reserved;
+} glq_paged_append_params;
+
+int glq_paged_append(const glq_paged_append_params* p, void* stream);
 
 /*
  * Causal attention of the new tokens over the cache (after glq_paged_append):
@@ -799,16 +810,30 @@ int glq_paged_append(const glq_paged_cache* cache, const int32_t* starts, int64_
  *   out[t][h*D + d] = fp16(sum_p softmax_p(scale * q.k_p) v_p[d]),
  * KV head h / (q_heads / kv_heads), fp32 scores, softmax and sums.  A row
  * without positions (p < 0) is 0; one past the page table NaN.  q (tokens,
- * q_heads, head_dim) fp16, out (tokens, q_heads * head_dim).  workspace:
- * glq_paged_attention_workspace_bytes, 256-byte aligned, zero-filled
- * before its first use (each call leaves its counters zero); calls that share
- * it must not overlap.
+ * q_heads, head_dim) fp16, out (tokens, q_heads * head_dim).  workspace: of
+ * glq_paged_attention_workspace_bytes (negative: invalid sizes), 256-byte
+ * aligned; what lies behind its first glq_paged_attention_scratch_bytes are
+ * counters, zero before its first use and left zero by each call.  Calls that
+ * share it must not overlap.
  */
+typedef struct glq_paged_attention_params {
+  glq_paged_cache cache;
+  const int32_t* starts;
+  int64_t tokens;
+  const void* q;
+  void* out;
+  int64_t q_heads;
+  int64_t window;
+  void* workspace;
+  int64_t workspace_bytes;
+  float scale;
+  int32_t reserved;
+} glq_paged_attention_params;
+
+int64_t glq_paged_attention_scratch_bytes(void);
 int64_t glq_paged_attention_workspace_bytes(int64_t seqs, int64_t tokens, int64_t q_heads,
-                                            int64_t kv_heads, int64_t head_dim);
-int glq_paged_attention(const glq_paged_cache* cache, const int32_t* starts, int64_t tokens,
-                        const void* q, int64_t q_heads, float scale, int64_t window, void* out,
-                        void* workspace, int64_t workspace_bytes, void* stream);
+                                            int64_t kv_heads);
+int glq_paged_attention(const glq_paged_attention_params* p, void* stream);
 
 #ifdef __cplusplus
 }

@@ -423,11 +423,25 @@ def test_moe_prefill_token_tile(lib, monkeypatch, mean, tile):
     assert mine == forced[tile] and len(set(forced.values())) >= 2
 
 
-def _paged(**kw):
-    p = 1 << 12
-    c = dict(k_pages=p, v_pages=p, k_scales=p, v_scales=p, page_table=p, lengths=p, seqs=2,
+P = 1 << 12  # a pointer that no call may follow
+
+
+def _paged_cache(**kw):
+    c = dict(k_pages=P, v_pages=P, k_scales=P, v_scales=P, page_table=P, lengths=P, seqs=2,
              max_pages=4, table_stride=4, pages=8, kv_heads=2, head_dim=128, page_size=64)
-    return ctypes.byref(_lib.PagedCache(**{**c, **kw}))
+    return _lib.PagedCache(**{**c, **kw})
+
+
+def _append(lib, cache={}, **kw):
+    a = dict(tokens=2, k=P, v=P, k_stride=256, v_stride=256, eps=1e-6)
+    p = _lib.PagedAppendParams(cache=_paged_cache(**cache), **{**a, **kw})
+    return lib.glq_paged_append(ctypes.byref(p), None), lib.glq_last_error()
+
+
+def _attend(lib, cache={}, **kw):
+    a = dict(tokens=2, q=P, out=P, q_heads=8, scale=1.0, workspace=P, workspace_bytes=1 << 30)
+    p = _lib.PagedAttentionParams(cache=_paged_cache(**cache), **{**a, **kw})
+    return lib.glq_paged_attention(ctypes.byref(p), None), lib.glq_last_error()
 
 
 @pytest.mark.parametrize("kw,what", [
@@ -442,40 +456,39 @@ def _paged(**kw):
 def test_paged_cache_checks(lib, kw, what):
     """A cache descriptor that does not fit is refused on the host by both
     entry points, before any launch."""
-    p, nul = 1 << 12, None
-    rc = lib.glq_paged_append(_paged(**kw), nul, 2, p, 256, p, 256, nul, 0, 0, 0, nul, nul, 1e-6,
-                              nul, nul, 0, nul, nul)
-    assert rc == 1 and what in lib.glq_last_error()
-    rc = lib.glq_paged_attention(_paged(**kw), nul, 2, p, 8, 1.0, 0, p, p, 1 << 30, nul)
-    assert rc == 1 and what in lib.glq_last_error()
+    for rc, msg in (_append(lib, kw), _attend(lib, kw)):
+        assert rc == 1 and what in msg
 
 
-def test_paged_entry_points_check_arguments(lib):
-    p, nul = 1 << 12, None
+@pytest.mark.parametrize("kw,what", [
+    (dict(k=None), b"null"), (dict(k=P + 8), b"aligned"), (dict(k_stride=250), b"strides"),
+    (dict(v_stride=260), b"strides"), (dict(cos=P), b"cos and sin"),
+    (dict(cos=P, sin=P, cs_stride=64), b"cs_stride"),
+    (dict(q=P, q_heads=3, q_stride=512, q_out=P), b"q_heads"),
+    (dict(q=P, q_heads=4, q_stride=512), b"q_out"),
+    (dict(q=P, q_heads=4, q_stride=256, q_out=P), b"row stride"),
+    (dict(q=P, q_heads=4, q_item_rows=96, q_out=P), b"q_item_rows"),
+    (dict(tokens=1 << 25), b"tokens"), (dict(tokens=3), b"same number"),
+])
+def test_paged_append_checks(lib, kw, what):
+    rc, msg = _append(lib, **kw)
+    assert rc == 1 and what in msg
 
-    def append(k=p, ks=256, vs=256, q=nul, Hq=0, qs=0, item=0, cos=nul, sin=nul, cs=0, qo=nul):
-        return lib.glq_paged_append(_paged(), nul, 2, k, ks, p, vs, q, Hq, qs, item, nul, nul,
-                                    1e-6, cos, sin, cs, qo, nul)
 
-    for rc, what in [
-        (append(k=nul), b"null"), (append(k=p + 8), b"aligned"), (append(ks=250), b"strides"),
-        (append(vs=260), b"strides"), (append(cos=p), b"cos and sin"),
-        (append(cos=p, sin=p, cs=64), b"cs_stride"), (append(q=p, Hq=3, qs=512, qo=p), b"q_heads"),
-        (append(q=p, Hq=4, qs=512), b"q_out"), (append(q=p, Hq=4, qs=256, qo=p), b"row stride"),
-        (append(q=p, Hq=4, item=96, qo=p), b"q_item_rows"),
-    ]:
-        assert rc == 1, what
-    assert append(q=p, Hq=4, item=96, qo=p) == 1 and b"q_item_rows" in lib.glq_last_error()
+@pytest.mark.parametrize("kw,what", [
+    (dict(q_heads=7), b"q_heads"), (dict(window=-1), b"window"), (dict(out=None), b"null"),
+    (dict(q=P + 2), b"aligned"), (dict(workspace=None), b"workspace"),
+    (dict(workspace_bytes=100), b"workspace"), (dict(workspace=P + 64), b"workspace"),
+])
+def test_paged_attention_checks(lib, kw, what):
+    rc, msg = _attend(lib, **kw)
+    assert rc == 1 and what in msg
 
-    def attend(q=p, Hq=8, window=0, out=p):
-        return lib.glq_paged_attention(_paged(), nul, 2, q, Hq, 1.0, window, out, p, 1 << 30, nul)
 
-    assert attend(Hq=7) == 1 and b"q_heads" in lib.glq_last_error()
-    assert attend(window=-1) == 1 and b"window" in lib.glq_last_error()
-    assert attend(out=nul) == 1 and attend(q=p + 2) == 1 and b"aligned" in lib.glq_last_error()
-    # no tokens: nothing is looked at
-    c = _paged(k_pages=None, pages=0)
-    assert lib.glq_paged_attention(c, nul, 0, nul, 8, 1.0, 0, nul, nul, 0, nul) == 0
-    assert lib.glq_paged_append(c, nul, 0, nul, 0, nul, 0, nul, 0, 0, 0, nul, nul, 1e-6, nul, nul,
-                                0, nul, nul) == 0
-    assert lib.glq_paged_attention_workspace_bytes(-1, 1, 1, 1, 128) == -1
+def test_paged_no_tokens(lib):
+    """No tokens: nothing is looked at."""
+    assert lib.glq_paged_append(None, None) == 1 and lib.glq_paged_attention(None, None) == 1
+    c = dict(k_pages=None, pages=0)
+    assert _append(lib, c, tokens=0, k=None)[0] == 0
+    assert _attend(lib, c, tokens=0, q=None, workspace=None)[0] == 0
+    assert lib.glq_paged_attention_workspace_bytes(-1, 1, 1, 1) == -1

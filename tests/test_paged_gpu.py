@@ -57,23 +57,23 @@ class Cache:
                 e = getattr(self.model, "e" + which)[b]
                 L = x.shape[0]
                 self.lengths[b] = L
+                pos = torch.arange(L)
+                pg, at = self.cpu_table[b, pos // self.page], pos % self.page
+                if self.fp8:
+                    x = x * torch.exp2(-e.T[pos // 16].double())[..., None]
+                val = x.float().to(pages.dtype)
                 host = pages.cpu()
-                sh = scales.cpu().view(torch.uint8) if self.fp8 else None
-                for p in range(L):
-                    pg, at = int(self.cpu_table[b, p // self.page]), p % self.page
-                    blk, j = at // 16, at % 16
-                    val = x[p] * torch.exp2(-e[:, p // 16].double())[:, None] if self.fp8 else x[p]
-                    val = val.float().to(pages.dtype).view(torch.uint8 if self.fp8 else FP16)
-                    hv = host.view(torch.uint8) if self.fp8 else host
-                    if which == "k":
-                        hv[pg, :, at] = val
-                    else:
-                        hv[pg, :, blk, :, j] = val
-                    if self.fp8:
-                        sh[pg, :, blk] = (e[:, p // 16] + 127).to(torch.uint8)
+                raw = host.view(torch.uint8) if self.fp8 else host
+                val = val.view(torch.uint8) if self.fp8 else val
+                if which == "k":
+                    raw[pg, :, at] = val
+                else:
+                    raw[pg, :, at // 16, :, at % 16] = val
                 pages.view(torch.uint8).copy_(host.view(torch.uint8))
                 if self.fp8:
-                    scales.view(torch.uint8).copy_(sh)
+                    host = scales.cpu().view(torch.uint8)
+                    host[pg, :, at // 16] = (e.T[pos // 16] + 127).to(torch.uint8)
+                    scales.view(torch.uint8).copy_(host)
 
     def tokens(self, b, L):
         """(k, v, ek, ev) that the pages hold of sequence b: (L, Hk, D) values,
@@ -291,6 +291,25 @@ def test_attention(gpu, dtype, D, page, Hq, Hk, news, past):
     c.fill([n + p for n, p in zip(news, past)])
     q = (torch.randn(sum(news), Hq, D, generator=c.g) * 2).half().to(gpu)
     check_attend(c, q, news, D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+@pytest.mark.parametrize("D,page,Hq,Hk,news,past,window", [
+    (128, 64, 8, 1, [1], [9000], 0),                    # one unit over many workgroups
+    (64, 16, 2, 2, [1] * 3, [6000, 17, 4100], 0),       # units that share workgroups
+    (128, 32, 4, 2, [2, 3, 1], [5000, 0, 2300], 1500),
+    (64, 64, 3, 3, [1] * 130, list(range(130)), 0),     # more units than workgroups
+    (128, 128, 40, 2, [1, 1], [2500, 100], 0),          # more rows than a unit holds
+    (64, 32, 1, 1, [1] * 600, [i % 70 for i in range(600)], 0),  # more sequences than threads
+])
+def test_attention_split(gpu, dtype, D, page, Hq, Hk, news, past, window):
+    """The units' pieces over waves and workgroups, and their merging; twice,
+    since a call leaves its counters zero."""
+    c = Cache(gpu, len(news), Hk, D, page, dtype, max(past) + page, 28)
+    c.fill([n + p for n, p in zip(news, past)])
+    q = (torch.randn(sum(news), Hq, D, generator=c.g) * 2).half().to(gpu)
+    y = check_attend(c, q, news, D ** -0.5, window=window)
+    assert torch.equal(y, check_attend(c, q, news, D ** -0.5, window=window))
 
 
 @pytest.mark.parametrize("dtype", [FP8, FP16])
@@ -559,7 +578,7 @@ def test_refusals(gpu):
         ("rows", lambda: append(v=k[:1])),
         ("do not divide", lambda: append(k=torch.cat([k, k[:1]]), v=torch.cat([k, k[:1]]))),
         ("multiples of 8", lambda: append(k=torch.zeros(2, 132, dtype=FP16, device=gpu)[:, :128])),
-        ("float16", lambda: append(k=k.float())),
+        ("float16", lambda: append(k=k.float(), v=k)),
         ("cos and sin", lambda: append(cos=k[:1, :64].contiguous())),
         ("rows of 64", lambda: append(cos=k, sin=k)),
         ("k_norm_w", lambda: append(k_norm_w=k[0])),
@@ -575,6 +594,8 @@ def test_refusals(gpu):
         ("workspace", lambda: attend(workspace=torch.zeros(8, dtype=torch.uint8, device=gpu))),
         ("q must be", lambda: attend(q=q[..., :32].contiguous())),
         ("GPU", lambda: attend(q=q.cpu())),
+        ("pages' GPU", lambda: append(v=k.cpu())),
+        ("GPU", lambda: append(kp=kp.cpu())),
     ]:
         with pytest.raises(RuntimeError, match=what):
             call()
