@@ -305,27 +305,13 @@ __device__ __forceinline__ void store_row(__half* dst, f32x4 v, float den, int p
 // gets a workgroup of its own, and nothing goes through memory.
 constexpr int kPaShort = 4;
 
-template <int D, bool FP8>
-__global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a) {
-  using RA = RowAttention<D, FP8>;
-  constexpr int TP = RA::TP, PS = D + 4;
-  struct Seg {  // a unit's piece that did not stay within its wave
-    int b, unit, ended;
-  };
-  extern __shared__ __align__(16) float parts[];  // [wave][2][rows][PS]
-  __shared__ long long scan[kPaWaves];
-  __shared__ int most[kPaWaves], units_sum[kPaWaves];
-  __shared__ long long at_off[kPaWaves];
-  __shared__ int at_seq[kPaWaves];
-  __shared__ Seg seg[kPaWaves][2];
-  __shared__ int flag;
-  const PagedView& c = a.c;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int Hq = c.Hk * a.rep;
+// The line, as every wave works it out for itself: 64 sequences a step.
+template <int TP>
+struct Line {
+  int total, quota, align;
 
-  // the line: each thread sums a run of sequences
-  const int per = (c.B + kPaThreads - 1) / kPaThreads, b0 = tid * per, b1 = min(b0 + per, c.B);
-  auto weigh = [&](int b, int& tiles, int& units) {
+  __device__ static void weigh(const PagedAttnArgs& a, int b, int& tiles, int& units) {
+    const PagedView& c = a.c;
     RowSet r;
     r.s0 = c.start(b);
     r.n = max((c.starts ? c.start(b + 1) : r.s0 + c.each) - r.s0, 0);
@@ -333,121 +319,110 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
     r.cap = c.max_pages << c.page_shift;
     tiles = sequence_tiles<TP>(r, a.window);
     units = (r.n * a.rep + kPaRows - 1) / kPaRows * c.Hk;
-  };
-  long long total = 0, sum = 0;
-  int widest = 0, n_units = 0;
-  for (int b = b0; b < b1; ++b) {
-    int tiles, units;
-    weigh(b, tiles, units);
-    sum += (long long)tiles * units;
-    widest = max(widest, tiles);
-    n_units += units;
   }
-  // every unit in a workgroup of its own, or an even cut: `quota` tiles a wave,
-  // a unit's tiles rounded up to `align` of them
-  auto scan_line = [&](long long mine, long long& before) {
-    long long v = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const long long u = __shfl_up(v, o);
-      if (lane >= o) v += u;
+  __device__ int rounded(int tiles) const { return (tiles + align - 1) / align * align; }
+
+  __device__ Line(const PagedAttnArgs& a) : align(1) {
+    const int lane = threadIdx.x & 63;
+    int sum = 0, widest = 0, units = 0;
+    for (int b = lane; b < a.c.B; b += 64) {
+      int t, u;
+      weigh(a, b, t, u);
+      sum += t * u;
+      units += u;
+      if (u) widest = max(widest, t);
     }
-    __syncthreads();
-    if (lane == 63) scan[wave] = v;
-    __syncthreads();
-    before = v - mine;
-    long long all = 0;
 #pragma unroll
-    for (int w = 0; w < kPaWaves; ++w) {
-      if (w < wave) before += scan[w];
-      all += scan[w];
+    for (int o = 32; o >= 1; o >>= 1) {
+      sum += __shfl_xor(sum, o);
+      units += __shfl_xor(units, o);
+      widest = max(widest, __shfl_xor(widest, o));
     }
-    return all;
-  };
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    widest = max(widest, __shfl_xor(widest, o));
-    n_units += __shfl_xor(n_units, o);
-  }
-  if (lane == 0) {
-    most[wave] = widest;
-    units_sum[wave] = n_units;
-  }
-  long long before;
-  total = scan_line(sum, before);
-  widest = n_units = 0;
-#pragma unroll
-  for (int w = 0; w < kPaWaves; ++w) {
-    widest = max(widest, most[w]);
-    n_units += units_sum[w];
-  }
-  const bool own = n_units <= (int)gridDim.x && widest <= kPaShort * kPaWaves;
-  const long long waves = (long long)gridDim.x * kPaWaves;
-  long long quota = own ? (widest + kPaWaves - 1) / kPaWaves
-                        : (total + waves - 1) / waves;
-  const int align = own ? (int)quota * kPaWaves : 1;
-  auto rounded = [&](int tiles) { return (tiles + align - 1) / align * align; };
-  if (own) {
-    sum = 0;
-    for (int b = b0; b < b1; ++b) {
-      int tiles, units;
-      weigh(b, tiles, units);
-      sum += (long long)rounded(tiles) * units;
+    sum = __builtin_amdgcn_readfirstlane(sum);
+    units = __builtin_amdgcn_readfirstlane(units);
+    widest = __builtin_amdgcn_readfirstlane(widest);
+    const int waves = (int)gridDim.x * kPaWaves;
+    if (units <= (int)gridDim.x && widest <= kPaShort * kPaWaves) {
+      quota = max((widest + kPaWaves - 1) / kPaWaves, 1);
+      align = quota * kPaWaves;
+      total = units * align;
+    } else {
+      quota = (sum + waves - 1) / waves;
+      total = sum;
     }
-    total = scan_line(sum, before);
   }
-  const long long wg_quota = quota * kPaWaves, wg0 = blockIdx.x * wg_quota;
-  if (wg0 >= total) return;  // uniform
-  // where each wave's piece begins
-  if (tid < kPaWaves) at_seq[tid] = -1;
-  __syncthreads();
-  for (int b = b0; b < b1; ++b) {
-    int tiles, units;
-    weigh(b, tiles, units);
-    const long long w = (long long)rounded(tiles) * units;
+
+  // Sequence of the line's tile p, and p's place from its first one; -1 past the end.
+  __device__ int find(const PagedAttnArgs& a, int p, int& off) const {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0, before = 0; base < a.c.B; base += 64) {
+      int t = 0, u = 0;
+      if (base + lane < a.c.B) weigh(a, base + lane, t, u);
+      const int w = rounded(t) * u;
+      int upto = w;
 #pragma unroll
-    for (int v = 0; v < kPaWaves; ++v) {
-      const long long p = wg0 + v * quota;
-      if (p >= before && p < before + w) {
-        at_seq[v] = b;
-        at_off[v] = p - before;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(upto, o);
+        if (lane >= o) upto += v;
       }
+      const int at = p - (before + upto - w);
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(at >= 0 && at < w);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        off = __builtin_amdgcn_readlane(at, l);
+        return base + l;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
     }
-    before += w;
+    return -1;
   }
-  if (tid < 2 * kPaWaves) seg[tid >> 1][tid & 1].unit = -1;
-  __syncthreads();
+};
+
+template <int D, bool FP8>
+__global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a) {
+  using RA = RowAttention<D, FP8>;
+  constexpr int TP = RA::TP, PS = D + 4;
+  struct Seg {  // a unit's piece that did not stay within its wave
+    int b, unit, tiles, ended, line;  // line: of the unit's first tile
+  };
+  extern __shared__ __align__(16) float parts[];  // [wave][2][rows][PS]
+  __shared__ Seg seg[kPaWaves][2];
+  __shared__ int flag;
+  const PagedView& c = a.c;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int Hq = c.Hk * a.rep;
+  const Line<TP> line(a);
+  const int wg_quota = line.quota * kPaWaves, wg0 = blockIdx.x * wg_quota;
+  if (wg0 >= line.total) return;  // uniform
+  if (lane < 2) seg[wave][lane].unit = -1;
 
   RA x(c);
   x.scale2 = a.scale2;
   x.rep = a.rep;
   x.window = a.window;
   {
-    int b = __builtin_amdgcn_readfirstlane(at_seq[wave]);
-    auto uniform = [](long long v) {
-      return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
-                         (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
-    };
-    long long off = b >= 0 ? uniform(at_off[wave]) : 0, left = uniform(quota);
-    while (b >= 0 && b < c.B && left > 0) {  // (bounded: b grows, or off to its end)
+    int off = 0, left = line.quota, pos = wg0 + wave * line.quota;
+    int b = line.find(a, pos, off);
+    while (b >= 0 && b < c.B && left > 0) {  // (b grows, or off to its end)
       int tiles, units;
-      weigh(b, tiles, units);
-      const int size = rounded(tiles);
-      if (off >= (long long)size * units) {
+      line.weigh(a, b, tiles, units);
+      const int size = line.rounded(tiles);
+      if (off >= size * units) {
         ++b;
         off = 0;
         continue;
       }
-      const int unit = (int)(off / size), t0 = (int)(off - (long long)unit * size);
-      const int run = (int)min((long long)(size - t0), left), t1 = min(t0 + run, tiles);
+      const int unit = off / size, t0 = off - unit * size;
+      const int run = min(size - t0, left), t1 = min(t0 + run, tiles);
+      const int at = pos - t0;
       off += run;
+      pos += run;
       left -= run;
       if (t0 >= t1) continue;
       const int qt = unit / c.Hk;
       x.b = b;
       x.g = unit - qt * c.Hk;
       set_rows(x.r, c, b, qt, a.rep, a.window, x.li);
-      x.begin(a.q, Hq);
       const int first = (a.window > 0 ? max(x.r.first - a.window + 1, 0) : 0) / TP;
       // k and v of the next tile are fetched as soon as the present one's have
       // been used, page ids a tile before them
@@ -456,6 +431,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
         int t = first + t0;
         typename RA::Tile tile;
         typename RA::Ids id = x.ids(t), ahead = x.ids(t + 1);
+        x.begin(a.q, Hq);
         x.load_k(tile, t, id);
         x.load_v(tile, t, id);
         for (; t < e; ++t) {
@@ -490,90 +466,103 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
             mine[D + 1] = x.l;
           }
         }
-        if (lane == 0) seg[wave][s] = Seg{b, unit, t1 == tiles};
+        if (lane == 0) seg[wave][s] = Seg{b, unit, tiles, t1 == tiles, at};
       }
     }
   }
   __syncthreads();
-  // Chains of pieces of one unit: the one that the workgroup begins in, and
-  // those that begin in a wave.  Thread (row, 4 columns).
+  // Chains of pieces of one unit: the one that the workgroup begins in (v = -1),
+  // and those that begin in a wave.  Thread (row, 4 columns).
   const int row = tid / (D / 4), d4 = 4 * (tid % (D / 4));
+  auto store = [&](const RowSet& r, int g, const Merge& acc) {
+    const int tok = r.row / a.rep;
+    store_row(a.out + ((int64_t)(r.s0 + tok) * Hq + g * a.rep + r.row % a.rep) * D + d4, acc.o,
+              acc.den, r.first + tok, r.cap);
+  };
+  Seg out[2];  // chains that another workgroup has parts of: not begun, not ended here
+  out[0].unit = out[1].unit = -1;
   for (int v = -1; v < kPaWaves; ++v) {  // uniform
     const int v0 = max(v, 0), s0 = v < 0 ? 0 : 1;
     const Seg head = seg[v0][s0];
     if (head.unit < 0) continue;
-    const bool began = v >= 0;
     bool ended = head.ended;
     int v1 = v0 + 1;
     while (!ended && v1 < kPaWaves && seg[v1][0].unit >= 0) ended = seg[v1++][0].ended;
     RowSet r;
     const int qt = head.unit / c.Hk, g = head.unit - qt * c.Hk;
     set_rows(r, c, head.b, qt, a.rep, a.window, row & 15);
-    const bool mine = row < kPaRows && r.live;
+    if (row >= a.rows) r.live = false;
     Merge acc;
-    if (mine) {
+    if (r.live) {
       for (int w = v0; w < v1; ++w) {
         const float* p = parts + ((w * 2 + (w == v0 ? s0 : 0)) * a.rows + row) * PS;
         acc.add(p[D], p[D + 1], *(const f32x4*)(p + d4));
       }
     }
-    if (!(began && ended)) {
-      // to memory; the last workgroup of the unit merges its parts in order
-      float* my = a.part + ((int64_t)(blockIdx.x * 2 + began) * kPaRows + row) * PS;
-      if (mine) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) handoff_put(my + d4 + e, acc.o[e]);
-        if (d4 == 0) {
-          handoff_put(my + D, acc.M);
-          handoff_put(my + D + 1, acc.den);
-        }
-      }
-      int tiles, units;
-      weigh(head.b, tiles, units);
-      // the unit's place on the line, from a piece of this workgroup's
-      const long long base = wg0 + v0 * quota - at_off[v0];  // (at_seq[v0] begins here)
-      long long u0;
-      if (at_seq[v0] == head.b) {
-        u0 = base + (long long)head.unit * tiles;
-      } else {  // the sequence begins inside wave v0's piece
-        u0 = base;
-        for (int b = at_seq[v0]; b < head.b; ++b) {
-          int t, u;
-          weigh(b, t, u);
-          u0 += (long long)t * u;
-        }
-        u0 += (long long)head.unit * tiles;
-      }
-      const int w0 = (int)(u0 / wg_quota), w1 = (int)((u0 + tiles - 1) / wg_quota);
-      const int slot = c.starts ? (int)((int64_t)r.s0 * a.rep / kPaRows) + head.b
-                                : head.b * a.tiles_each;
-      unsigned* cnt = a.count + (int64_t)(slot + qt) * c.Hk + g;
-      if (!handoff_arrive(cnt, (unsigned)(w1 - w0 + 1), &flag)) continue;
-      acc = Merge();
-      const float* p0 = a.part + (int64_t)(row & 15) * PS;
-      for (int w = w0; w <= w1; w += 8) {
-        float m[8], l[8];
-        f32x4 o[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int ww = min(w + j, w1);
-          const float* p = p0 + (int64_t)(ww * 2 + (ww == w0)) * (kPaRows * PS);
-          m[j] = handoff_get(p + D);
-          l[j] = handoff_get(p + D + 1);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[j][e] = handoff_get(p + d4 + e);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (w + j <= w1) acc.add(m[j], l[j], o[j]);
-      }
-      if (tid == 0) handoff_reset(cnt);
+    if (v >= 0 && ended) {
+      if (r.live) store(r, g, acc);
+      continue;
     }
-    if (mine) {
-      const int tok = r.row / a.rep;
-      store_row(a.out + ((int64_t)(r.s0 + tok) * Hq + g * a.rep + r.row % a.rep) * D + d4, acc.o,
-                acc.den, r.first + tok, r.cap);
+    out[s0] = head;
+    if (r.live) {
+      float* my = a.part + ((int64_t)(blockIdx.x * 2 + s0) * kPaRows + row) * PS;
+      handoff_put((uint64_t*)(my + d4), __builtin_bit_cast(uint64_t, float2{acc.o[0], acc.o[1]}));
+      handoff_put((uint64_t*)(my + d4) + 1,
+                  __builtin_bit_cast(uint64_t, float2{acc.o[2], acc.o[3]}));
+      if (d4 == 0)
+        handoff_put((uint64_t*)(my + D), __builtin_bit_cast(uint64_t, float2{acc.M, acc.den}));
     }
+  }
+  // The last workgroup of a unit to arrive merges its parts: thread (group,
+  // row, 4 columns), the groups taking the parts in turn, 8 in flight.
+#pragma unroll
+  for (int s0 = 0; s0 < 2; ++s0) {
+    const Seg head = out[s0];
+    if (head.unit < 0) continue;  // uniform
+    const int w0 = head.line / wg_quota, w1 = (head.line + head.tiles - 1) / wg_quota;
+    const int qt = head.unit / c.Hk, g = head.unit - qt * c.Hk;
+    const int slot = c.starts ? (int)((int64_t)c.start(head.b) * a.rep / kPaRows) + head.b
+                              : head.b * a.tiles_each;
+    unsigned* cnt = a.count + (int64_t)(slot + qt) * c.Hk + g;
+    if (!handoff_arrive(cnt, (unsigned)(w1 - w0 + 1), &flag)) continue;
+    const int groups = kPaThreads / (a.rows * (D / 4)), grp = row / a.rows, rw = row - grp * a.rows;
+    Merge acc;
+    const float* p0 = a.part + (int64_t)rw * PS;
+    for (int w = w0 + grp; w <= w1; w += 8 * groups) {
+      float2 ml[8], o[8][2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int ww = min(w + j * groups, w1);
+        const float* p = p0 + (int64_t)(ww * 2 + (ww == w0)) * (kPaRows * PS);
+        ml[j] = __builtin_bit_cast(float2, handoff_get((const uint64_t*)(p + D)));
+        o[j][0] = __builtin_bit_cast(float2, handoff_get((const uint64_t*)(p + d4)));
+        o[j][1] = __builtin_bit_cast(float2, handoff_get((const uint64_t*)(p + d4) + 1));
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (w + j * groups <= w1)
+          acc.add(ml[j].x, ml[j].y, f32x4{o[j][0].x, o[j][0].y, o[j][1].x, o[j][1].y});
+    }
+    if (groups > 1) {  // through LDS, whose pieces have been merged
+      float* mine = parts + (grp * a.rows + rw) * PS;
+      *(f32x4*)(mine + d4) = acc.o;
+      if (d4 == 0) {
+        mine[D] = acc.M;
+        mine[D + 1] = acc.den;
+      }
+      __syncthreads();
+      if (grp == 0) {
+        for (int k = 1; k < groups; ++k) {
+          const float* p = parts + (k * a.rows + rw) * PS;
+          acc.add(p[D], p[D + 1], *(const f32x4*)(p + d4));
+        }
+      }
+      __syncthreads();
+    }
+    RowSet r;
+    set_rows(r, c, head.b, qt, a.rep, a.window, rw);
+    if (grp == 0 && r.live) store(r, g, acc);
+    if (tid == 0) handoff_reset(cnt);
   }
 }
 
@@ -627,6 +616,9 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
   const int64_t rows_each = (int64_t)a.c.each * a.rep;
   a.tiles_each = (int)((rows_each + kPaRows - 1) / kPaRows);
   a.rows = !starts && rows_each <= 8 ? 8 : kPaRows;
+  const int64_t most = (cache->max_pages * cache->page_size + 31) / 32 + 1;
+  GLQ_CHECK((tokens * a.rep / kPaRows + cache->seqs) * Hk <= (1ll << 31) / most - 1,
+            "a batch of too many rows for its page table's length");
   a.part = (float*)p->workspace;
   a.count = (unsigned*)((char*)p->workspace + glq_paged_attention_scratch_bytes());
   const size_t lds = (size_t)kPaWaves * 2 * a.rows * (D + 4) * 4;
