@@ -93,7 +93,8 @@ class PagedAttentionParams(ctypes.Structure):
     """glq_paged_attention_params (include/glorcq_hip.h), field for field."""
     _fields_ = [
         ("cache", PagedCache), ("starts", _vp), ("tokens", _i64), ("q", _vp), ("out", _vp),
-        ("q_heads", _i64), ("window", _i64), ("workspace", _vp), ("workspace_bytes", _i64),
+        ("q_heads", _i64), ("window", _i64), ("counters", _vp), ("scratch", _vp),
+        ("counter_bytes", _i64), ("scratch_bytes", _i64),
         ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
     ]
 
@@ -258,8 +259,8 @@ SIGNATURES = {
     ]),
     # (params as c_void_p: a pointer to one of the structures above, or its bytes)
     "glq_paged_append": (_c_int, [_vp, _vp]),            # params, stream
-    "glq_paged_attention_scratch_bytes": (_i64, []),
-    "glq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "glq_paged_attention_counter_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "glq_paged_attention_scratch_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "glq_paged_attention": (_c_int, [_vp, _vp]),         # params, stream
 }
 

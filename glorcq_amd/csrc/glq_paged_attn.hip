@@ -3,38 +3,14 @@
 
 #include <algorithm>
 
-#include "glq_handoff.h"
-#include "glq_paged.h"
+#include "glq_paged_attn.h"
 
 namespace glq {
 namespace {
 
 constexpr int kPaThreads = 512;
 constexpr int kPaWaves = kPaThreads / 64;
-constexpr int kPaRows = 16;  // query rows (tokens x the KV head's q heads) of a unit
 constexpr int kPaGrid = 256;
-
-struct PagedAttnArgs {
-  PagedView c;
-  const __half* q;  // (T, Hq, D)
-  __half* out;      // (T, Hq D)
-  float* part;      // [workgroup][2][kPaRows][D + 4]: o, m, l
-  unsigned* count;  // [unit], zero between calls
-  int rep, window, tiles_each, rows;
-  float scale2;     // scale log2(e)
-};
-
-// The 16 query rows of a unit, column li of the matrix products on the lanes
-// (li, kb), and the positions they see.
-struct RowSet {
-  int first;         // position of the sequence's first new token
-  int s0, n;         // its rows of q
-  int row;           // this lane's row: token row / rep, head row % rep
-  bool live;
-  int lo, hi;        // positions this lane's row sees: [lo, hi)
-  int lo_all, hi_all, lo_any, hi_any;  // seen by all rows, by any
-  int cap;           // positions of the page table
-};
 
 template <int D, bool FP8>
 struct RowAttention {
@@ -236,27 +212,6 @@ struct RowAttention {
   }
 };
 
-// Sets r for rows [16 qt, 16 qt + 16) of sequence b's n new tokens.
-__device__ __forceinline__ void set_rows(RowSet& r, const PagedView& c, int b, int qt, int rep,
-                                         int window, int li) {
-  r.s0 = c.start(b);
-  r.n = max((c.starts ? c.start(b + 1) : r.s0 + c.each) - r.s0, 0);
-  r.first = c.length(b) - r.n;
-  r.cap = c.max_pages << c.page_shift;
-  const int rows = r.n * rep, r0 = qt * kPaRows, r1 = min(r0 + kPaRows, rows) - 1;
-  r.live = r0 + li < rows;
-  r.row = min(r0 + li, rows - 1);
-  auto lo = [&](int pos) { return window > 0 ? max(pos - window + 1, 0) : 0; };
-  auto hi = [&](int pos) { return min(max(pos + 1, 0), r.cap); };
-  const int pos = r.first + r.row / rep;
-  r.lo = lo(pos);
-  r.hi = hi(pos);
-  r.lo_any = lo(r.first + r0 / rep);
-  r.hi_all = hi(r.first + r0 / rep);
-  r.lo_all = lo(r.first + r1 / rep);
-  r.hi_any = hi(r.first + r1 / rep);
-}
-
 // Tiles of each of a sequence's units, 0 for a sequence without new tokens (the
 // rows of others are written even where they see nothing: at least 1).
 template <int TP>
@@ -265,30 +220,6 @@ __device__ __forceinline__ int sequence_tiles(const RowSet& r, int window) {
   const int lo = window > 0 ? max(r.first - window + 1, 0) : 0;
   const int hi = min(max(r.first + r.n, 0), r.cap);
   return max((hi + TP - 1) / TP - lo / TP, 1);
-}
-
-// Merges pieces (m, l, o) of a row's attention, 4 columns a thread.
-struct Merge {
-  float M = -__builtin_inff(), den = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  __device__ void add(float m, float l, f32x4 v) {
-    const float Mn = fmaxf(M, m), Mf = Mn == -__builtin_inff() ? 0.f : Mn;
-    const float fo = __builtin_amdgcn_exp2f(M - Mf), fn = __builtin_amdgcn_exp2f(m - Mf);
-    den = den * fo + l * fn;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * fo + v[e] * fn;
-    M = Mn;
-  }
-};
-
-// 4 columns of a row's result to memory.
-__device__ __forceinline__ void store_row(__half* dst, f32x4 v, float den, int pos, int cap) {
-  const float inv = 1.f / den;
-  f16x2 y[2];
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    y[e >> 1][e & 1] = (_Float16)(pos < 0 ? 0.f : pos >= cap ? __builtin_nanf("") : v[e] * inv);
-  *(uint2*)dst = uint2{__builtin_bit_cast(uint32_t, y[0]), __builtin_bit_cast(uint32_t, y[1])};
 }
 
 // The batch's work is a line of tiles: sequence by sequence, unit by unit (KV
@@ -318,7 +249,8 @@ struct Line {
     r.first = c.length(b) - r.n;
     r.cap = c.max_pages << c.page_shift;
     tiles = sequence_tiles<TP>(r, a.window);
-    units = (r.n * a.rep + kPaRows - 1) / kPaRows * c.Hk;
+    // (a sequence of more rows is the second form's)
+    units = c.starts && r.n * a.rep > kPaMostRows ? 0 : (r.n * a.rep + kPaRows - 1) / kPaRows * c.Hk;
   }
   __device__ int rounded(int tiles) const { return (tiles + align - 1) / align * align; }
 
@@ -422,7 +354,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
       const int qt = unit / c.Hk;
       x.b = b;
       x.g = unit - qt * c.Hk;
-      set_rows(x.r, c, b, qt, a.rep, a.window, x.li);
+      set_rows<kPaRows>(x.r, c, b, qt * kPaRows, a.rep, a.window, x.li);
       const int first = (a.window > 0 ? max(x.r.first - a.window + 1, 0) : 0) / TP;
       // k and v of the next tile are fetched as soon as the present one's have
       // been used, page ids a tile before them
@@ -490,7 +422,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
     while (!ended && v1 < kPaWaves && seg[v1][0].unit >= 0) ended = seg[v1++][0].ended;
     RowSet r;
     const int qt = head.unit / c.Hk, g = head.unit - qt * c.Hk;
-    set_rows(r, c, head.b, qt, a.rep, a.window, row & 15);
+    set_rows<kPaRows>(r, c, head.b, qt * kPaRows, a.rep, a.window, row & 15);
     if (row >= a.rows) r.live = false;
     Merge acc;
     if (r.live) {
@@ -522,7 +454,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
     const int w0 = head.line / wg_quota, w1 = (head.line + head.tiles - 1) / wg_quota;
     const int qt = head.unit / c.Hk, g = head.unit - qt * c.Hk;
     const int slot = c.starts ? (int)((int64_t)c.start(head.b) * a.rep / kPaRows) + head.b
-                              : head.b * a.tiles_each;
+                              : head.b * a.slots_each;
     unsigned* cnt = a.count + (int64_t)(slot + qt) * c.Hk + g;
     if (!handoff_arrive(cnt, (unsigned)(w1 - w0 + 1), &flag)) continue;
     const int groups = kPaThreads / (a.rows * (D / 4)), grp = row / a.rows, rw = row - grp * a.rows;
@@ -560,7 +492,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
       __syncthreads();
     }
     RowSet r;
-    set_rows(r, c, head.b, qt, a.rep, a.window, rw);
+    set_rows<kPaRows>(r, c, head.b, qt * kPaRows, a.rep, a.window, rw);
     if (grp == 0 && r.live) store(r, g, acc);
     if (tid == 0) handoff_reset(cnt);
   }
@@ -569,19 +501,22 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
 }  // namespace
 }  // namespace glq
 
-extern "C" int64_t glq_paged_attention_scratch_bytes(void) {
-  using namespace glq;
-  return (int64_t)kPaGrid * 2 * kPaRows * (128 + 4) * 4;
-}
-
-extern "C" int64_t glq_paged_attention_workspace_bytes(int64_t seqs, int64_t tokens,
-                                                       int64_t q_heads, int64_t kv_heads) {
+extern "C" int64_t glq_paged_attention_counter_bytes(int64_t seqs, int64_t tokens,
+                                                     int64_t q_heads, int64_t kv_heads) {
   using namespace glq;
   if (seqs < 0 || tokens < 0 || q_heads <= 0 || kv_heads <= 0) return -1;
-  // a counter a unit: at most rows / 16 + 1 units a sequence and KV head
+  // a counter a unit of the first form: at most rows / 16 + 1 a sequence and KV head
   const int64_t rep = (q_heads + kv_heads - 1) / kv_heads;
-  const int64_t units = (tokens * rep / kPaRows + seqs) * kv_heads;
-  return glq_paged_attention_scratch_bytes() + align_up(4 * units, 256);
+  return align_up(4 * (tokens * rep / kPaRows + seqs) * kv_heads, 256);
+}
+
+extern "C" int64_t glq_paged_attention_scratch_bytes(int64_t seqs, int64_t tokens, int64_t q_heads,
+                                                     int64_t kv_heads) {
+  using namespace glq;
+  if (seqs < 0 || tokens < 0 || q_heads <= 0 || kv_heads <= 0) return -1;
+  return align_up(std::max((int64_t)kPaGrid * 2 * kPaRows * (128 + 4) * 4,
+                           paged_prompt_scratch_bytes(seqs, tokens, q_heads, kv_heads)),
+                  256);
 }
 
 extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* stream) {
@@ -602,25 +537,35 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
   if (tokens == 0 || cache->seqs == 0) return GLQ_OK;
   GLQ_CHECK(q && out && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0,
             "q and out must be non-null and 16-byte aligned");
-  const int64_t need =
-      glq_paged_attention_workspace_bytes(cache->seqs, tokens, q_heads, Hk);
-  GLQ_CHECK(p->workspace && p->workspace_bytes >= need && ((uintptr_t)p->workspace & 255) == 0,
-            "a 256-byte aligned workspace of %lld bytes needed (got %lld)", (long long)need,
-            (long long)p->workspace_bytes);
+  const int64_t cnt = glq_paged_attention_counter_bytes(cache->seqs, tokens, q_heads, Hk);
+  const int64_t scr = glq_paged_attention_scratch_bytes(cache->seqs, tokens, q_heads, Hk);
+  GLQ_CHECK(p->counters && p->counter_bytes >= cnt && p->scratch && p->scratch_bytes >= scr &&
+                ((uintptr_t)p->counters & 3) == 0 && ((uintptr_t)p->scratch & 255) == 0,
+            "workspace of %lld (counters) and %lld bytes (scratch, 256-byte aligned) needed "
+            "(got %lld, %lld)", (long long)cnt, (long long)scr, (long long)p->counter_bytes,
+            (long long)p->scratch_bytes);
   a.q = (const __half*)q;
   a.out = (__half*)out;
   a.rep = (int)(q_heads / Hk);
   a.window = window >= cache->max_pages * cache->page_size ? 0 : (int)window;
   a.scale2 = p->scale * 1.44269504088896f;
-  GLQ_CHECK(tokens * a.rep < (1ll << 30), "batch of too many (token, head) rows");
+  a.part = (float*)p->scratch;
+  a.count = (unsigned*)p->counters;
   const int64_t rows_each = (int64_t)a.c.each * a.rep;
-  a.tiles_each = (int)((rows_each + kPaRows - 1) / kPaRows);
-  a.rows = !starts && rows_each <= 8 ? 8 : kPaRows;
+  GLQ_CHECK(tokens * a.rep < (1ll << 30), "batch of too many (token, head) rows");
+  // Many rows take the second form, a sequence at a time; where lengths are the
+  // device's, both are launched, each passing over the other's sequences.
+  if (starts ? tokens * a.rep > kPaMostRows : rows_each > kPaMostRows) {
+    if (int rc = paged_prompt_launch(a, (int)D, (hipStream_t)stream)) return rc;
+    if (!starts) return GLQ_OK;
+  }
   const int64_t most = (cache->max_pages * cache->page_size + 31) / 32 + 1;
-  GLQ_CHECK((tokens * a.rep / kPaRows + cache->seqs) * Hk <= (1ll << 31) / most - 1,
+  GLQ_CHECK(std::min(tokens * a.rep / kPaRows + cache->seqs,
+                     cache->seqs * ((kPaMostRows + kPaRows - 1) / kPaRows)) * Hk <=
+                (1ll << 31) / most - 1,
             "a batch of too many rows for its page table's length");
-  a.part = (float*)p->workspace;
-  a.count = (unsigned*)((char*)p->workspace + glq_paged_attention_scratch_bytes());
+  a.slots_each = (int)((rows_each + kPaRows - 1) / kPaRows);
+  a.rows = !starts && rows_each <= 8 ? 8 : kPaRows;
   const size_t lds = (size_t)kPaWaves * 2 * a.rows * (D + 4) * 4;
   auto kern = D == 128 ? (a.c.ks ? paged_rows_kernel<128, true> : paged_rows_kernel<128, false>)
                        : (a.c.ks ? paged_rows_kernel<64, true> : paged_rows_kernel<64, false>);

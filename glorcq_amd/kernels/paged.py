@@ -27,7 +27,7 @@ import struct
 import torch
 
 from .. import _lib
-from . import _require, _zeroed_buffer
+from . import _require, _zeroed_buffer, workspace as _stream_scratch
 
 BLOCK = 16  # tokens of a scale block
 
@@ -37,12 +37,12 @@ _FP8, _FP16, _E8M0 = torch.float8_e4m3fn, torch.float16, torch.float8_e8m0fnu
 # about 4 us of host time a call, this 1): glq_paged_cache, then the call's own.
 _CACHE = "6P7q"
 _append_params = struct.Struct(_CACHE + "Pq3P5q4PqPfi").pack
-_attention_params = struct.Struct(_CACHE + "Pq2P2qPqfi").pack
+_attention_params = struct.Struct(_CACHE + "Pq2P2q2P2qfi").pack
 assert struct.calcsize(_CACHE + "Pq3P5q4PqPfi") == ctypes.sizeof(_lib.PagedAppendParams)
-assert struct.calcsize(_CACHE + "Pq2P2qPqfi") == ctypes.sizeof(_lib.PagedAttentionParams)
+assert struct.calcsize(_CACHE + "Pq2P2q2P2qfi") == ctypes.sizeof(_lib.PagedAttentionParams)
 
-# attention workspaces: (device index, stream handle) -> zero-filled uint8 tensor
-_workspaces: dict = {}
+# attention counters: (device index, stream handle) -> zero-filled uint8 tensor
+_counters: dict = {}
 _ws_bytes: dict = {}
 
 
@@ -242,32 +242,31 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     return q_out
 
 
-def _workspace_bytes(B, T, Hq, Hk) -> int:
-    """glq_paged_attention_workspace_bytes, memoized (a function of its sizes)."""
+def _workspace_bytes(B, T, Hq, Hk) -> tuple[int, int]:
+    """Bytes of the counters and of the scratch, memoized (functions of the sizes)."""
     n = _ws_bytes.get((B, T, Hq, Hk))
     if n is None:
-        n = _lib.load().glq_paged_attention_workspace_bytes(B, T, Hq, Hk)
-        if n < 0:
+        lib = _lib.load()
+        n = (lib.glq_paged_attention_counter_bytes(B, T, Hq, Hk),
+             lib.glq_paged_attention_scratch_bytes(B, T, Hq, Hk))
+        if min(n) < 0:
             raise RuntimeError("invalid paged attention shapes")
-        n = _ws_bytes[(B, T, Hq, Hk)] = max(int(n), 256)
+        _ws_bytes[(B, T, Hq, Hk)] = n
     return n
 
 
-def _new_workspace(n: int, dev: int) -> torch.Tensor:
-    """A workspace whose counters, the part behind its scratch, are zero."""
-    ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", dev))
-    ws[_lib.load().glq_paged_attention_scratch_bytes():].zero_()
-    return ws
+def _new_workspace(n, device) -> tuple[torch.Tensor, torch.Tensor]:
+    return (torch.zeros(max(n[0], 256), dtype=torch.uint8, device=device),
+            torch.empty(n[1], dtype=torch.uint8, device=device))
 
 
-def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor,
-                              page_table: torch.Tensor) -> torch.Tensor:
-    """A workspace for paged_attention at these shapes (keep it for the calls
-    that follow: every call leaves its counters zero, and calls that share it
-    must not overlap)."""
+def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor):
+    """A workspace (counters, zero between calls; scratch) for paged_attention
+    at these sizes and smaller ones (keep it for the calls that follow; calls
+    that share it must not overlap)."""
     return _new_workspace(_workspace_bytes(page_table.shape[0], q.shape[0],
                                            q.shape[1:].numel() // k_pages.shape[3],
-                                           k_pages.shape[1]), k_pages.get_device())
+                                           k_pages.shape[1]), k_pages.device)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -275,7 +274,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     starts: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
                     v_scales: torch.Tensor | None = None, window: int = 0,
                     out: torch.Tensor | None = None,
-                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+                    workspace: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
     """Causal attention of the new tokens' q (T, Hq, D) fp16 (paged_append's
     result) over their sequences' pages -> (T, Hq*D) fp16 (glq_paged_attention).
     The token at position p attends to (p - window, p], or [0, p] with window
@@ -307,12 +306,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if workspace is None:
         n = _workspace_bytes(cache[6], T, Hq, Hk)
         if torch.cuda.is_current_stream_capturing():
-            workspace = _new_workspace(n, dev)
+            counters, scratch = _new_workspace(n, q.device)
         else:
-            workspace = _zeroed_buffer(_workspaces, torch.device("cuda", dev), n)
+            counters = _zeroed_buffer(_counters, q.device, n[0])
+            scratch = _stream_scratch(q.device, n[1])
     else:
-        _check(workspace, "workspace", dev, torch.uint8)
+        counters, scratch = workspace
+        _check(counters, "workspace's counters", dev, torch.uint8)
+        _check(scratch, "workspace's scratch", dev, torch.uint8)
     _launch(lib.glq_paged_attention, "glq_paged_attention", _attention_params(
-        *cache, _ptr(starts), T, q.data_ptr(), out.data_ptr(), Hq, window, workspace.data_ptr(),
-        workspace.numel(), scale, 0), dev)
+        *cache, _ptr(starts), T, q.data_ptr(), out.data_ptr(), Hq, window, counters.data_ptr(),
+        scratch.data_ptr(), counters.numel(), scratch.numel(), scale, 0), dev)
     return out

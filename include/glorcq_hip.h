@@ -810,11 +810,11 @@ int glq_paged_append(const glq_paged_append_params* p, void* stream);
  *   out[t][h*D + d] = fp16(sum_p softmax_p(scale * q.k_p) v_p[d]),
  * KV head h / (q_heads / kv_heads), fp32 scores, softmax and sums.  A row
  * without positions (p < 0) is 0; one past the page table NaN.  q (tokens,
- * q_heads, head_dim) fp16, out (tokens, q_heads * head_dim).  workspace: of
- * glq_paged_attention_workspace_bytes (negative: invalid sizes), 256-byte
- * aligned; what lies behind its first glq_paged_attention_scratch_bytes are
- * counters, zero before its first use and left zero by each call.  Calls that
- * share it must not overlap.
+ * q_heads, head_dim) fp16, out (tokens, q_heads * head_dim).  workspace: the
+ * counters (glq_paged_attention_counter_bytes) are zero before their first use
+ * and left zero by each call; the scratch (.._scratch_bytes, 256-byte aligned)
+ * needs no initialisation (both negative for invalid sizes).  Calls that share
+ * either must not overlap.
  */
 typedef struct glq_paged_attention_params {
   glq_paged_cache cache;
@@ -824,15 +824,16 @@ typedef struct glq_paged_attention_params {
   void* out;
   int64_t q_heads;
   int64_t window;
-  void* workspace;
-  int64_t workspace_bytes;
+  void *counters, *scratch;
+  int64_t counter_bytes, scratch_bytes;
   float scale;
   int32_t reserved;
 } glq_paged_attention_params;
 
-int64_t glq_paged_attention_scratch_bytes(void);
-int64_t glq_paged_attention_workspace_bytes(int64_t seqs, int64_t tokens, int64_t q_heads,
-                                            int64_t kv_heads);
+int64_t glq_paged_attention_counter_bytes(int64_t seqs, int64_t tokens, int64_t q_heads,
+                                          int64_t kv_heads);
+int64_t glq_paged_attention_scratch_bytes(int64_t seqs, int64_t tokens, int64_t q_heads,
+                                          int64_t kv_heads);
 int glq_paged_attention(const glq_paged_attention_params* p, void* stream);
 
 #ifdef __cplusplus

@@ -439,7 +439,8 @@ def _append(lib, cache={}, **kw):
 
 
 def _attend(lib, cache={}, **kw):
-    a = dict(tokens=2, q=P, out=P, q_heads=8, scale=1.0, workspace=P, workspace_bytes=1 << 30)
+    a = dict(tokens=2, q=P, out=P, q_heads=8, scale=1.0, counters=P, scratch=P,
+             counter_bytes=1 << 30, scratch_bytes=1 << 30)
     p = _lib.PagedAttentionParams(cache=_paged_cache(**cache), **{**a, **kw})
     return lib.glq_paged_attention(ctypes.byref(p), None), lib.glq_last_error()
 
@@ -477,8 +478,9 @@ def test_paged_append_checks(lib, kw, what):
 
 @pytest.mark.parametrize("kw,what", [
     (dict(q_heads=7), b"q_heads"), (dict(window=-1), b"window"), (dict(out=None), b"null"),
-    (dict(q=P + 2), b"aligned"), (dict(workspace=None), b"workspace"),
-    (dict(workspace_bytes=100), b"workspace"), (dict(workspace=P + 64), b"workspace"),
+    (dict(q=P + 2), b"aligned"), (dict(counters=None), b"workspace"),
+    (dict(counter_bytes=10), b"workspace"), (dict(scratch_bytes=10), b"workspace"),
+    (dict(scratch=P + 64), b"workspace"),
 ])
 def test_paged_attention_checks(lib, kw, what):
     rc, msg = _attend(lib, **kw)
@@ -490,5 +492,6 @@ def test_paged_no_tokens(lib):
     assert lib.glq_paged_append(None, None) == 1 and lib.glq_paged_attention(None, None) == 1
     c = dict(k_pages=None, pages=0)
     assert _append(lib, c, tokens=0, k=None)[0] == 0
-    assert _attend(lib, c, tokens=0, q=None, workspace=None)[0] == 0
-    assert lib.glq_paged_attention_workspace_bytes(-1, 1, 1, 1) == -1
+    assert _attend(lib, c, tokens=0, q=None, counters=None)[0] == 0
+    assert lib.glq_paged_attention_counter_bytes(-1, 1, 1, 1) == -1
+    assert lib.glq_paged_attention_scratch_bytes(1, 1, 1, 0) == -1

@@ -591,7 +591,7 @@ def test_refusals(gpu):
         ("window", lambda: attend(window=-1)),
         ("multiple of the KV", lambda: attend(q=q[:, :3].contiguous())),
         ("out must", lambda: attend(out=torch.zeros(2, 128, dtype=FP16, device=gpu))),
-        ("workspace", lambda: attend(workspace=torch.zeros(8, dtype=torch.uint8, device=gpu))),
+        ("workspace", lambda: attend(workspace=[torch.zeros(8, dtype=torch.uint8, device=gpu)] * 2)),
         ("q must be", lambda: attend(q=q[..., :32].contiguous())),
         ("GPU", lambda: attend(q=q.cpu())),
         ("pages' GPU", lambda: append(v=k.cpu())),
