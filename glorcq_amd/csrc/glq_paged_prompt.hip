@@ -44,55 +44,58 @@ struct PromptStage {
   static constexpr int kBytes = 2 * kPpTile * D * 2;          // K and V of a step in LDS
 
   u32x4 k[KP], v[VC][S];
-  int ks, vs;  // scale bytes of block tid & 3
+  int ks, vs;  // scale bytes of the wave's block
   bool bad;
+  int wave;    // uniform
 
-  __device__ static int k_block(int j) { return (KR * j + threadIdx.x / KC) >> 4; }
-  __device__ static int v_block(int j) { return (kPpThreads * j + (int)threadIdx.x) / D; }
+  // A wave's pieces of a pass lie in one block, so that addresses are scalars
+  // but for a lane's constant part.
+  __device__ int k_block(int j) const { return KR * j / 16 + wave * 64 / KC / 16; }
+  __device__ int v_block(int j) const { return (kPpThreads * j + 64 * wave) / D; }
+  static_assert(KR % 16 == 0, "a pass's rows");
 
+  // Page ids of the blocks that the wave fetches, and of the one whose scales
+  // it does (block `wave`).
   struct Ids {
-    int id[4];
+    int k[KP], v[VC], own;
   };
-  __device__ static Ids ids(const PagedView& c, int b, int tile) {
+  __device__ Ids ids(const PagedView& c, int b, int tile) const {
     const int* row = c.table + b * c.table_stride;
+    auto id = [&](int blk) {
+      return __builtin_amdgcn_readfirstlane(
+          row[min((4 * tile + blk) >> (c.page_shift - 4), c.max_pages - 1)]);
+    };
     Ids r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r.id[i] = row[min((4 * tile + i) >> (c.page_shift - 4), c.max_pages - 1)];
+    for (int j = 0; j < KP; ++j) r.k[j] = id(k_block(j));
+#pragma unroll
+    for (int j = 0; j < VC; ++j) r.v[j] = id(v_block(j));
+    r.own = id(wave);
     return r;
-  }
-  __device__ static int64_t place(const PagedView& c, int g, int p, int blk) {
-    const int bpp = 1 << (c.page_shift - 4);
-    return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g) * bpp + (blk & (bpp - 1));
-  }
-  __device__ static int pick(const Ids& r, int i) {
-    return i & 2 ? (i & 1 ? r.id[3] : r.id[2]) : (i & 1 ? r.id[1] : r.id[0]);
   }
 
   __device__ void load(const PagedView& c, int g, int tile, const Ids& r) {
-    const int t = threadIdx.x;
-    {
-      const int p = pick(r, t & 3);
-      bad = (unsigned)p >= (unsigned)c.pages;
-      if constexpr (FP8) {
-        const int64_t at = place(c, g, p, 4 * tile + (t & 3));
-        ks = c.ks[at];
-        vs = c.vs[at];
-      }
+    const int t = threadIdx.x, bpp = 1 << (c.page_shift - 4);
+    auto place = [&](int p, int blk) {  // ids out of range read page 0
+      return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g) * bpp +
+             ((4 * tile + blk) & (bpp - 1));
+    };
+    bad = (unsigned)r.own >= (unsigned)c.pages;
+    if constexpr (FP8) {
+      const int64_t at = place(r.own, wave);
+      ks = c.ks[at];
+      vs = c.vs[at];
     }
+    const unsigned k_lane = (t / KC & 15) * (D * S) + 16 * (t % KC), v_lane = t % D * (16 * S);
 #pragma unroll
-    for (int j = 0; j < KP; ++j) {
-      const int row = KR * j + t / KC, blk = k_block(j);
-      const char* p = (const char*)c.k + place(c, g, pick(r, blk), 4 * tile + blk) * (16 * D * S);
-      k[j] = *(const u32x4*)(p + (row & 15) * (D * S) + 16 * (t % KC));
-    }
+    for (int j = 0; j < KP; ++j)
+      k[j] = *(const u32x4*)((const char*)c.k + place(r.k[j], k_block(j)) * (16 * D * S) + k_lane);
 #pragma unroll
-    for (int j = 0; j < VC; ++j) {
-      const int blk = v_block(j), d = (kPpThreads * j + t) % D;
-      const char* p = (const char*)c.v + place(c, g, pick(r, blk), 4 * tile + blk) * (16 * D * S);
+    for (int j = 0; j < VC; ++j)
 #pragma unroll
-      for (int i = 0; i < S; ++i) v[j][i] = *(const u32x4*)(p + d * 16 * S + 16 * i);
-    }
+      for (int i = 0; i < S; ++i)
+        v[j][i] = *(const u32x4*)((const char*)c.v + place(r.v[j], v_block(j)) * (16 * D * S) +
+                                  v_lane + 16 * i);
   }
 
   // K: piece (8 d8 .. + 8 of a position) at (d8, position, its low bits mixed
@@ -136,9 +139,9 @@ struct PromptStage {
           any |= FP8 ? (v[j][i][e] & 0x7F7F7F7Fu) + 0x01010101u
                      : (v[j][i][e] & 0x7FFF7FFFu) + 0x04000400u;
     }
-    if (t < 4) {
-      scales[t] = bad ? __builtin_nanf("") : FP8 ? e8m0_value(ks) * scale2 : scale2;
-      scales[4 + t] = FP8 ? e8m0_exponent(vs) : 0.f;
+    if ((t & 63) == 0) {
+      scales[wave] = bad ? __builtin_nanf("") : FP8 ? e8m0_value(ks) * scale2 : scale2;
+      scales[4 + wave] = FP8 ? e8m0_exponent(vs) : 0.f;
     }
     return (any & (FP8 ? 0x80808080u : 0x80008000u)) != 0;
   }
@@ -184,6 +187,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnAr
     t0 += split * per;
     t1 = min(t1, t0 + per);
   }
+  const int unit_lo = r.lo_all, unit_hi = r.hi_all;  // what all of its rows see
   const int r0 = slot * kPpRows + 32 * wave;
   const bool any = r0 < rows;  // the wave has rows
   set_rows<32>(r, c, b, min(r0, rows - 1), a.rep, a.window, col);
@@ -207,9 +211,10 @@ __global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnAr
   for (int i = 0; i < NG; ++i) o[i] = f32x16{};
 
   Stage st;
-  typename Stage::Ids ids = Stage::ids(c, b, t0);
+  st.wave = wave;
+  typename Stage::Ids ids = st.ids(c, b, t0);
   st.load(c, g, t0, ids);
-  ids = Stage::ids(c, b, t0 + 1);
+  ids = st.ids(c, b, t0 + 1);
   auto stage = [&](int buf) {
     const bool odd = st.store(bufs + buf * (Stage::kBytes / 2), scales[buf], scale2);
     if (lane == 0) odds[buf][wave] = 0;
@@ -218,18 +223,20 @@ __global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnAr
   stage(0);
   if (t0 + 1 < t1) {
     const typename Stage::Ids now = ids;
-    ids = Stage::ids(c, b, t0 + 2);
+    ids = st.ids(c, b, t0 + 2);
     st.load(c, g, t0 + 1, now);
   }
   __syncthreads();
-  for (int t = t0; t < t1; ++t) {
+  // A step.  OddV: V holds an infinity or a NaN in a step that some row does not
+  // see all of (rare; a loop of its own, which keeps the other free of copies).
+  auto step = [&](int t, auto odd_v) {
     const int cur = (t - t0) & 1;
     const _Float16* kb = bufs + cur * (Stage::kBytes / 2);
     if (t + 1 < t1) {
       stage(cur ^ 1);
       if (t + 2 < t1) {
         const typename Stage::Ids now = ids;
-        ids = Stage::ids(c, b, t + 3);
+        ids = st.ids(c, b, t + 3);
         st.load(c, g, t + 2, now);
       }
     }
@@ -237,15 +244,14 @@ __global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnAr
     if (any && p0 < r.hi_any && p0 + kPpTile > r.lo_any) {  // (uniform in the wave)
       const bool edge = p0 < r.lo_all || p0 + kPpTile > r.hi_all;
       f32x16 s[2];
+      s[0] = s[1] = f32x16{};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[i] = f32x16{};
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
+        for (int i = 0; i < 2; ++i) {
           const f16x8 ka = *(const f16x8*)(kb + Stage::k_at(2 * k + half, 32 * i + col));
           s[i] = mfma_32x32x16(ka, q[k], s[i]);
         }
-      }
       if (edge) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -305,12 +311,11 @@ __global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnAr
         weights(std::true_type());
       else
         weights(std::false_type());
-      const int* od = odds[cur];
-      if (!edge || !__builtin_amdgcn_readfirstlane(od[0] | od[1] | od[2] | od[3])) {
+      if constexpr (!odd_v.value) {
 #pragma unroll
-        for (int i = 0; i < NG; ++i)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int i = 0; i < NG; ++i) {
             const f16x8 va = *(const f16x8*)(kb + Stage::v_at(k, half, 32 * i + col));
             o[i] = mfma_32x32x16(va, w[k], o[i]);
           }
@@ -345,7 +350,16 @@ __global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnAr
       }
     }
     __syncthreads();
+  };
+  int t = t0;
+  for (; t < t1; ++t) {
+    const int* od = odds[(t - t0) & 1];
+    if (__builtin_amdgcn_readfirstlane(od[0] | od[1] | od[2] | od[3]) &&
+        (t * kPpTile < unit_lo || (t + 1) * kPpTile > unit_hi))
+      break;  // uniform in the workgroup
+    step(t, std::false_type());
   }
+  for (; t < t1; ++t) step(t, std::true_type());
   l += __shfl_xor(l, 32);
   if (!r.live) return;
   if (parts == 1) {
