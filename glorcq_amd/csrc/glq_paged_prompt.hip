@@ -41,7 +41,6 @@ struct PromptStage {
   static constexpr int KC = D * S / 16;                       // pieces of a K row
   static constexpr int KR = kPpThreads / KC;                  // rows a pass
   static constexpr int VC = 4 * D / kPpThreads;               // V columns (of a block) a thread
-  static constexpr int kBytes = 2 * kPpTile * D * 2;          // K and V of a step in LDS
 
   u32x4 k[KP], v[VC][S];
   int ks, vs;  // scale bytes of the wave's block
@@ -74,41 +73,52 @@ struct PromptStage {
     return r;
   }
 
-  __device__ void load(const PagedView& c, int g, int tile, const Ids& r) {
-    const int t = threadIdx.x, bpp = 1 << (c.page_shift - 4);
-    auto place = [&](int p, int blk) {  // ids out of range read page 0
-      return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g) * bpp +
-             ((4 * tile + blk) & (bpp - 1));
-    };
+  // (ids out of range read page 0)
+  __device__ static int64_t place(const PagedView& c, int g, int p, int tile, int blk) {
+    const int bpp = 1 << (c.page_shift - 4);
+    return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g) * bpp +
+           ((4 * tile + blk) & (bpp - 1));
+  }
+  __device__ void load_k(const PagedView& c, int g, int tile, const Ids& r) {
+    const int t = threadIdx.x;
     bad = (unsigned)r.own >= (unsigned)c.pages;
     if constexpr (FP8) {
-      const int64_t at = place(r.own, wave);
+      const int64_t at = place(c, g, r.own, tile, wave);
       ks = c.ks[at];
       vs = c.vs[at];
     }
-    const unsigned k_lane = (t / KC & 15) * (D * S) + 16 * (t % KC), v_lane = t % D * (16 * S);
+    const unsigned lane = (t / KC & 15) * (D * S) + 16 * (t % KC);
 #pragma unroll
     for (int j = 0; j < KP; ++j)
-      k[j] = *(const u32x4*)((const char*)c.k + place(r.k[j], k_block(j)) * (16 * D * S) + k_lane);
+      k[j] = *(const u32x4*)((const char*)c.k +
+                             place(c, g, r.k[j], tile, k_block(j)) * (16 * D * S) + lane);
+  }
+  __device__ void load_v(const PagedView& c, int g, int tile, const Ids& r) {
+    const unsigned lane = threadIdx.x % D * (16 * S);
 #pragma unroll
     for (int j = 0; j < VC; ++j)
 #pragma unroll
       for (int i = 0; i < S; ++i)
-        v[j][i] = *(const u32x4*)((const char*)c.v + place(r.v[j], v_block(j)) * (16 * D * S) +
-                                  v_lane + 16 * i);
+        v[j][i] = *(const u32x4*)((const char*)c.v +
+                                  place(c, g, r.v[j], tile, v_block(j)) * (16 * D * S) + lane +
+                                  16 * i);
   }
 
-  // K: piece (8 d8 .. + 8 of a position) at (d8, position, its low bits mixed
-  // with d8's so that a row's pieces go to different banks); V: piece (block,
-  // half, column), half 0 the block's positions 0-3 and 8-11, as lane halves
-  // hold them.
-  __device__ static int k_at(int d8, int pos) { return (d8 * kPpTile + (pos ^ (d8 & 14))) * 8; }
+  // LDS places in halves.  K: piece (8 d8 .. + 8 of a position) at (d8,
+  // position), 32 bytes between pairs of d8 so that a row's pieces go to
+  // different banks as they are stored (between single d8, the two lane halves
+  // of a read collide: half of the LDS cycles); V: piece (block, half, column),
+  // half 0 the block's positions 0-3 and 8-11, as the lane halves hold them.
+  static constexpr int kKPair = 2 * kPpTile * 8 + 16;
+  __device__ static int k_at(int d8, int pos) {
+    return (d8 >> 1) * kKPair + (d8 & 1) * (kPpTile * 8) + pos * 8;
+  }
   __device__ static int v_at(int blk, int half, int d) {
-    return kPpTile * D + ((blk * 2 + half) * D + d) * 8;
+    return D / 16 * kKPair + ((blk * 2 + half) * D + d) * 8;
   }
+  static constexpr int kBytes = 2 * (D / 16 * kKPair + kPpTile * D);  // of a step
 
-  // Returns whether the thread's part of V holds an infinity or a NaN.
-  __device__ bool store(_Float16* buf, float* scales, float scale2) const {
+  __device__ void store_k(_Float16* buf, float* scales, float scale2) const {
     const int t = threadIdx.x;
 #pragma unroll
     for (int j = 0; j < KP; ++j) {
@@ -120,40 +130,120 @@ struct PromptStage {
         *(u32x4*)(buf + k_at(piece, row)) = k[j];
       }
     }
-    uint32_t any = 0;
-#pragma unroll
-    for (int j = 0; j < VC; ++j) {
-      const int blk = v_block(j), d = (kPpThreads * j + t) % D;
-      if constexpr (FP8) {
-        *(f16x8*)(buf + v_at(blk, 0, d)) = fp8x8_to_f16(v[j][0][0], v[j][0][2]);
-        *(f16x8*)(buf + v_at(blk, 1, d)) = fp8x8_to_f16(v[j][0][1], v[j][0][3]);
-      } else {
-        *(u32x4*)(buf + v_at(blk, 0, d)) = u32x4{v[j][0][0], v[j][0][1], v[j][1][0], v[j][1][1]};
-        *(u32x4*)(buf + v_at(blk, 1, d)) = u32x4{v[j][0][2], v[j][0][3], v[j][1][2], v[j][1][3]};
-      }
-      // (the largest exponent field carries into the sign's place)
-#pragma unroll
-      for (int i = 0; i < S; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          any |= FP8 ? (v[j][i][e] & 0x7F7F7F7Fu) + 0x01010101u
-                     : (v[j][i][e] & 0x7FFF7FFFu) + 0x04000400u;
-    }
     if ((t & 63) == 0) {
       scales[wave] = bad ? __builtin_nanf("") : FP8 ? e8m0_value(ks) * scale2 : scale2;
       scales[4 + wave] = FP8 ? e8m0_exponent(vs) : 0.f;
     }
-    return (any & (FP8 ? 0x80808080u : 0x80008000u)) != 0;
+  }
+  // Infinities and NaN go into LDS as zeros (weight 0 times one that a row does
+  // not see is not 0); returns whether the wave's part of V holds any, for
+  // them to be added afterwards.
+  __device__ bool store_v(_Float16* buf) const {
+    const int t = threadIdx.x;
+    uint32_t any = 0;
+#pragma unroll
+    for (int j = 0; j < VC; ++j)
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= odd_values(v[j][i][e]);
+    const bool found = __builtin_amdgcn_ballot_w64((any & kOdd) != 0) != 0;
+    u32x4 u[VC][S];
+#pragma unroll
+    for (int j = 0; j < VC; ++j)
+#pragma unroll
+      for (int i = 0; i < S; ++i) u[j][i] = v[j][i];
+    if (found) {
+#pragma unroll
+      for (int j = 0; j < VC; ++j)
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = (odd_values(v[j][i][e]) & kOdd) >> (FP8 ? 7 : 15);
+            u[j][i][e] &= ~(x * (FP8 ? 0xFFu : 0xFFFFu));
+          }
+    }
+#pragma unroll
+    for (int j = 0; j < VC; ++j) {
+      const int blk = v_block(j), d = (kPpThreads * j + t) % D;
+      if constexpr (FP8) {
+        *(f16x8*)(buf + v_at(blk, 0, d)) = fp8x8_to_f16(u[j][0][0], u[j][0][2]);
+        *(f16x8*)(buf + v_at(blk, 1, d)) = fp8x8_to_f16(u[j][0][1], u[j][0][3]);
+      } else {
+        *(u32x4*)(buf + v_at(blk, 0, d)) = u32x4{u[j][0][0], u[j][0][1], u[j][1][0], u[j][1][1]};
+        *(u32x4*)(buf + v_at(blk, 1, d)) = u32x4{u[j][0][2], u[j][0][3], u[j][1][2], u[j][1][3]};
+      }
+    }
+    return found;
+  }
+  // Of a word of values, the top bit of each infinity or NaN (with kOdd).
+  static constexpr uint32_t kOdd = FP8 ? 0x80808080u : 0x80008000u;
+  __device__ static uint32_t odd_values(uint32_t w) {
+    // (the largest exponent field carries into the sign's place)
+    return FP8 ? (w & 0x7F7F7F7Fu) + 0x01010101u : (w & 0x7FFF7FFFu) + 0x04000400u;
   }
 };
 
+// Adds the infinities and NaN of V that the row of a lane sees, at positions of
+// steps [t0, t1), to its sums: rare, and so a plain walk over the blocks.
 template <int D, bool FP8>
-__global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnArgs a) {
+__device__ void add_odd_values(f32x16 (&o)[D / 32], const PagedView& c, int b, int g, int t0,
+                               int t1, const RowSet& r) {
+  using Stage = PromptStage<D, FP8>;
+  constexpr int S = FP8 ? 1 : 2, NG = D / 32;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  for (int blk = 4 * t0; blk < 4 * t1; ++blk) {
+    const int p = c.page_of(b, blk >> (c.page_shift - 4));
+    if (p < 0) continue;  // (the scores are NaN there)
+    const char* base = (const char*)c.v + Stage::place(c, g, p, 0, blk) * (16 * D * S);
+    uint32_t here = 0;  // positions of the block with one
+    for (int d = lane; d < D; d += 64)
+#pragma unroll
+      for (int i = 0; i < 4 * S; ++i) {
+        const uint32_t x = Stage::odd_values(((const uint32_t*)(base + d * 16 * S))[i]) & Stage::kOdd;
+        if constexpr (FP8)
+          here |= (x >> 7 & 1 | x >> 14 & 2 | x >> 21 & 4 | x >> 28 & 8) << (4 * i);
+        else
+          here |= (x >> 15 & 1 | x >> 30 & 2) << (2 * i);
+      }
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) here |= __shfl_xor((int)here, k);
+    here = __builtin_amdgcn_readfirstlane(here);
+    bool all_nan = true;
+    while (here) {
+      const int j = __builtin_ctz(here), pos = 16 * blk + j;
+      here &= here - 1;
+      const bool sees = pos >= r.lo && pos < r.hi;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int d = 32 * n + 8 * (e >> 2) + 4 * half + (e & 3);
+          float x;
+          if constexpr (FP8)
+            x = (((const uint8_t*)base)[d * 16 + j] & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
+          else
+            x = (float)((const _Float16*)base)[d * 16 + j];
+          if (sees && !(fabsf(x) < __builtin_inff())) o[n][e] += x;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) all_nan &= o[n][e] != o[n][e];
+    if (__builtin_amdgcn_ballot_w64(!all_nan && r.live) == 0) return;
+  }
+}
+
+template <int D, bool FP8>
+__global__ __launch_bounds__(kPpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_prompt_kernel(PagedAttnArgs a) {
   using Stage = PromptStage<D, FP8>;
   constexpr int NG = D / 32, KS = D / 16, PS = D + 4;
   extern __shared__ __align__(16) unsigned char smem[];
   _Float16* bufs = (_Float16*)smem;  // 2 x Stage::kBytes
-  __shared__ float scales[2][8];
+  __shared__ float scales[4][8];  // (a step's are read into the next one's first half)
   __shared__ int odds[2][kPpThreads / 64];
   const PagedView& c = a.c;
   // the last rows of a sequence, which see most, first
@@ -187,7 +277,6 @@ __global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnAr
     t0 += split * per;
     t1 = min(t1, t0 + per);
   }
-  const int unit_lo = r.lo_all, unit_hi = r.hi_all;  // what all of its rows see
   const int r0 = slot * kPpRows + 32 * wave;
   const bool any = r0 < rows;  // the wave has rows
   set_rows<32>(r, c, b, min(r0, rows - 1), a.rep, a.window, col);
@@ -206,160 +295,182 @@ __global__ __launch_bounds__(kPpThreads, 2) void paged_prompt_kernel(PagedAttnAr
   }
   const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
   float m = -__builtin_inff(), l = 0.f;
-  f32x16 o[NG];
+  f32x16 o[NG], sa = {}, sb = {};
+  f16x8 w[2] = {f16x8{}, f16x8{}};
 #pragma unroll
   for (int i = 0; i < NG; ++i) o[i] = f32x16{};
 
   Stage st;
   st.wave = wave;
-  typename Stage::Ids ids = st.ids(c, b, t0);
-  st.load(c, g, t0, ids);
-  ids = st.ids(c, b, t0 + 1);
-  auto stage = [&](int buf) {
-    const bool odd = st.store(bufs + buf * (Stage::kBytes / 2), scales[buf], scale2);
-    if (lane == 0) odds[buf][wave] = 0;
-    if (__builtin_amdgcn_ballot_w64(odd) && lane == 0) odds[buf][wave] = 1;
+  auto buf = [&](int t) { return bufs + ((t - t0) & 1) * (Stage::kBytes / 2); };
+  // 32 scores a row: positions 32 i .. + 32 of step t
+  auto scores = [&](f32x16& s, int t, int i) {
+    const _Float16* kb = buf(t);
+    s = f32x16{};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const f16x8 ka = *(const f16x8*)(kb + Stage::k_at(2 * k + half, 32 * i + col));
+      s = mfma_32x32x16(ka, q[k], s);
+    }
   };
-  stage(0);
-  if (t0 + 1 < t1) {
-    const typename Stage::Ids now = ids;
-    ids = st.ids(c, b, t0 + 2);
-    st.load(c, g, t0 + 1, now);
-  }
-  __syncthreads();
-  // A step.  OddV: V holds an infinity or a NaN in a step that some row does not
-  // see all of (rare; a loop of its own, which keeps the other free of copies).
-  auto step = [&](int t, auto odd_v) {
-    const int cur = (t - t0) & 1;
-    const _Float16* kb = bufs + cur * (Stage::kBytes / 2);
-    if (t + 1 < t1) {
-      stage(cur ^ 1);
-      if (t + 2 < t1) {
-        const typename Stage::Ids now = ids;
-        ids = st.ids(c, b, t + 3);
-        st.load(c, g, t + 2, now);
+  // O += the weights of positions 32 i .. of step t times their V
+  auto weigh_v = [&](int t, int i) {
+    const _Float16* kb = buf(t);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const f16x8 va = *(const f16x8*)(kb + Stage::v_at(2 * i + k, half, 32 * n + col));
+        o[n] = mfma_32x32x16(va, w[k], o[n]);
+      }
+  };
+  // Half a step, on positions 32 i .. of step t, whose scores are in s: the
+  // matrix instructions of the half before (its weighted V) and of the half
+  // after (its scores, to `next`) run beside this one's exponentials.
+  auto half_step = [&](int t, auto i_, f32x16& s, f32x16& next) {
+    constexpr int i = i_.value;
+    const int p0 = t * kPpTile + 32 * i;
+    // the operands of the matrix instructions below, kAhead of them in flight:
+    // in turn K's of the scores and V's
+    constexpr int kOps = KS + 2 * NG, kAhead = 4;
+    static_assert(KS == 2 * NG, "as many of each");
+    const _Float16 *kbuf = buf(t + i), *vbuf = buf(t + i - 1);
+    auto operand = [&](int n) {
+      return n & 1 ? *(const f16x8*)(vbuf + Stage::v_at(2 * (1 - i) + n / 2 / NG, half,
+                                                        32 * (n / 2 % NG) + col))
+                   : *(const f16x8*)(kbuf + Stage::k_at(n + half, 32 * (1 - i) + col));
+    };
+    f16x8 op[kAhead];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) op[n] = operand(n);
+    __builtin_amdgcn_sched_barrier(0);
+    // block 2 i + k of the step: its scales
+    const float* sc = scales[(t - t0) & 3] + 2 * i;
+    float ks[2] = {sc[0], sc[1]}, ev[2] = {sc[4], sc[5]};
+    if (p0 < r.lo_all || p0 + 32 > r.hi_all) {
+      // a position that a row does not see has no weight, whatever its block's
+      // scale is: a NaN goes from the scale to the scores
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const bool bad = ks[k] != ks[k] || ev[k] != ev[k];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int p = p0 + 16 * k + 8 * (e >> 2) + 4 * half + (e & 3);
+          if (bad) s[8 * k + e] = __builtin_nanf("");
+          if (p < r.lo || p >= r.hi) s[8 * k + e] = -__builtin_inff();
+        }
+        if (bad) {
+          ks[k] = 1.f;
+          ev[k] = 0.f;
+        }
       }
     }
-    const int p0 = t * kPpTile;
-    if (any && p0 < r.hi_any && p0 + kPpTile > r.lo_any) {  // (uniform in the wave)
-      const bool edge = p0 < r.lo_all || p0 + kPpTile > r.hi_all;
-      f32x16 s[2];
-      s[0] = s[1] = f32x16{};
+    float mx = -__builtin_inff();
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
+    for (int k = 0; k < 2; ++k) {
+      float bm = s[8 * k];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f16x8 ka = *(const f16x8*)(kb + Stage::k_at(2 * k + half, 32 * i + col));
-          s[i] = mfma_32x32x16(ka, q[k], s[i]);
-        }
-      if (edge) {
+      for (int e = 1; e < 8; ++e) bm = fmaxf(bm, s[8 * k + e]);
+      mx = fmaxf(mx, fmaf(bm, ks[k], ev[k]));
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__builtin_amdgcn_ballot_w64(mx > m + kPpLag)) {  // (-inf + lag: any score passes)
+      // a whole number, so that the factor of the weights in w is a power of two
+      const float mn = fmaxf(m, ceilf(mx)), mf = mn == -__builtin_inff() ? 0.f : mn;
+      const float f = __builtin_amdgcn_exp2f(m - mf);
+      const _Float16 fh = (_Float16)f;
+      m = mn;
+      l *= f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int k = 0; k < 2; ++k) w[k] *= fh;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int p = p0 + 32 * i + 8 * (e >> 2) + 4 * half + (e & 3);
-            if (p < r.lo || p >= r.hi) s[i][e] = -__builtin_inff();
-          }
-      }
-      // block 2 i + (e >> 3) of the step: its scales
-      const float* sc = scales[cur];
-      float mx = -__builtin_inff();
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float bm = s[k >> 1][8 * (k & 1)];
+        for (int e = 0; e < 16; ++e) o[n][e] *= f;
+    }
+    const float mf = m == -__builtin_inff() ? 0.f : m;
+    const float off[2] = {ev[0] - mf, ev[1] - mf};
+    f16x8 wn[2];
+    float sum[2] = {0.f, 0.f};
+    next = f32x16{};
 #pragma unroll
-        for (int e = 1; e < 8; ++e) bm = fmaxf(bm, s[k >> 1][8 * (k & 1) + e]);
-        mx = fmaxf(mx, fmaf(bm, sc[k], sc[4 + k]));
-      }
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (__builtin_amdgcn_ballot_w64(mx > m + kPpLag)) {  // (-inf + lag: any score passes)
-        const float mn = fmaxf(m, mx), mf = mn == -__builtin_inff() ? 0.f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - mf);
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < NG; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[i][e] *= f;
-      }
-      const float mf = m == -__builtin_inff() ? 0.f : m;
-      f16x8 w[4];
-      // (a position that a row does not see has no weight, whatever its block's
-      // scale is)
-      auto weights = [&](auto masked) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float ks = sc[k], ev = sc[4 + k], off = ev - mf;
-          float sum = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = s[k >> 1][8 * (k & 1) + e];
-            float x = __builtin_amdgcn_exp2f(fmaf(v, ks, off));
-            if (masked.value) x = v == -__builtin_inff() ? 0.f : x;
-            sum += x;
-            w[k][e] = (_Float16)x;
-          }
-          if constexpr (!FP8)
-            l += sum;
-          else if (masked.value)
-            l = sum == 0.f ? l : fmaf(sum, __builtin_amdgcn_exp2f(-ev), l);
-          else
-            l = fmaf(sum, __builtin_amdgcn_exp2f(-ev), l);
-        }
-      };
-      if (edge)
-        weights(std::true_type());
+    for (int n = 0; n < kOps; ++n) {
+      if (n & 1)
+        o[n / 2 % NG] = mfma_32x32x16(op[n % kAhead], w[n / 2 / NG], o[n / 2 % NG]);
       else
-        weights(std::false_type());
-      if constexpr (!odd_v.value) {
+        next = mfma_32x32x16(op[n % kAhead], q[n / 2], next);
+      if (n + kAhead < kOps) op[n % kAhead] = operand(n + kAhead);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            const f16x8 va = *(const f16x8*)(kb + Stage::v_at(k, half, 32 * i + col));
-            o[i] = mfma_32x32x16(va, w[k], o[i]);
-          }
-      } else {
-        // weight 0 times an inf or a NaN that a row does not see is not 0: a
-        // token's rows at a time, with zeros for the positions behind its own
-        const int last = __builtin_amdgcn_readlane(tok, 31);
-#pragma nounroll
-        for (int n = __builtin_amdgcn_readfirstlane(tok); n <= last; ++n) {
-          const int pos = r.first + n, hi = pos + 1, lo = a.window > 0 ? pos - a.window + 1 : 0;
-#pragma nounroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t keep[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {  // values 2 e, 2 e + 1 of a piece
-              const int p = p0 + 16 * k + 8 * (e >> 1) + 4 * half + 2 * (e & 1);
-              keep[e] = (p >= lo && p < hi ? 0xFFFFu : 0u) |
-                        (p + 1 >= lo && p + 1 < hi ? 0xFFFF0000u : 0u);
-            }
-            const f16x8 wk = k & 2 ? (k & 1 ? w[3] : w[2]) : (k & 1 ? w[1] : w[0]);
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-              u32x4 va = *(const u32x4*)(kb + Stage::v_at(k, half, 32 * i + col));
-#pragma unroll
-              for (int e = 0; e < 4; ++e) va[e] &= keep[e];
-              const f32x16 on = mfma_32x32x16(__builtin_bit_cast(f16x8, va), wk, o[i]);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[i][e] = tok == n ? on[e] : o[i][e];
-            }
-          }
-        }
+      for (int e = 16 / kOps * n; e < 16 / kOps * (n + 1); ++e) {
+        const int k = e >> 3;
+        float x = __builtin_amdgcn_exp2f(fmaf(s[e], ks[k], off[k]));
+        asm volatile("" : "+v"(x));  // (in this place)
+        sum[k] += x;
+        wn[k][e & 7] = (_Float16)x;
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      l = FP8 ? fmaf(sum[k], __builtin_amdgcn_exp2f(-ev[k]), l) : l + sum[k];
+    w[0] = wn[0];
+    w[1] = wn[1];
+  };
+
+  // Before the loop: K and V of step t0 in LDS, the next step's in registers,
+  // zeros where the first half step looks for the V of the one before it.
+  typename Stage::Ids ids = st.ids(c, b, t0);
+  st.load_k(c, g, t0, ids);
+  st.load_v(c, g, t0, ids);
+  ids = st.ids(c, b, t0 + 1);
+  for (int i = tid; i < 4 * D; i += kPpThreads)
+    *(u32x4*)(buf(t0 - 1) + Stage::v_at(2, 0, 0) + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+  st.store_k(buf(t0), scales[0], scale2);
+  // steps whose V holds infinities or NaN: the wave's first, one past its last
+  int odd0 = st.store_v(buf(t0)) ? t0 : 0x7FFFFFFF, odd1 = t0 + 1;
+  if (t0 + 1 < t1) {
+    st.load_k(c, g, t0 + 1, ids);
+    st.load_v(c, g, t0 + 1, ids);
+  }
+  ids = st.ids(c, b, t0 + 2);
+  __syncthreads();
+  if (any) scores(sa, t0, 0);
+  // A step.  K of the next one is stored in its first half and V in its second,
+  // so that the one barrier between the halves parts writers and readers: K of
+  // t + 1 is first read after it and K of t - 1 last before the barrier of
+  // t - 1; V of t is first read after it, V of t - 2 last before t - 1's.
+  using H0 = std::integral_constant<int, 0>;
+  using H1 = std::integral_constant<int, 1>;
+  for (int t = t0; t < t1; ++t) {
+    if (any) half_step(t, H0(), sa, sb);
+    if (t + 1 < t1) {
+      st.store_k(buf(t + 1), scales[(t + 1 - t0) & 3], scale2);
+      if (t + 2 < t1) st.load_k(c, g, t + 2, ids);
     }
     __syncthreads();
-  };
-  int t = t0;
-  for (; t < t1; ++t) {
-    const int* od = odds[(t - t0) & 1];
-    if (__builtin_amdgcn_readfirstlane(od[0] | od[1] | od[2] | od[3]) &&
-        (t * kPpTile < unit_lo || (t + 1) * kPpTile > unit_hi))
-      break;  // uniform in the workgroup
-    step(t, std::false_type());
+    if (any) half_step(t, H1(), sb, sa);
+    if (t + 1 < t1) {
+      if (st.store_v(buf(t + 1))) {
+        odd0 = min(odd0, t + 1);
+        odd1 = t + 2;
+      }
+      if (t + 2 < t1) {
+        st.load_v(c, g, t + 2, ids);
+        ids = st.ids(c, b, t + 3);
+      }
+    }
   }
-  for (; t < t1; ++t) step(t, std::true_type());
+  if (any && t1 > t0) weigh_v(t1 - 1, 1);
+  if (lane == 0) {
+    odds[0][wave] = odd0;
+    odds[1][wave] = odd1;
+  }
+  __syncthreads();
+  odd0 = min(min(odds[0][0], odds[0][1]), min(odds[0][2], odds[0][3]));
+  odd1 = max(max(odds[1][0], odds[1][1]), max(odds[1][2], odds[1][3]));
+  if (any && odd0 < odd1 && t1 > t0)
+    add_odd_values<D, FP8>(o, c, b, g, __builtin_amdgcn_readfirstlane(odd0),
+                           __builtin_amdgcn_readfirstlane(min(odd1, t1)), r);
   l += __shfl_xor(l, 32);
   if (!r.live) return;
   if (parts == 1) {
