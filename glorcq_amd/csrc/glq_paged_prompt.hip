@@ -15,20 +15,31 @@ __device__ __forceinline__ f32x16 mfma_32x32x16(f16x8 a, f16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+// The larger of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float halves_max(float x) {
+  const auto r =
+      __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 constexpr int kPpThreads = 256;
-constexpr int kPpTile = 64;    // positions of a step
+constexpr int kPpStep = 32;    // positions of a step: two blocks
 constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running maximum
 
 // One workgroup takes 128 query rows (tokens x the KV head's q heads) of one KV
-// head, 32 a wave, over the positions they see (or a split of them), 64 a step:
+// head, 32 a wave, over the positions they see (or a split of them), 32 a step:
 //   S^T = K Q^T   v_mfma_f32_32x32x16_f16, A = 32 positions of K, B = the rows
 //   O^T += V^T P^T                         A = 32 columns of V,   B = the weights
-// so that a row of the softmax is a column of both products: its 64 scores of
+// so that a row of the softmax is a column of both products: its 32 scores of
 // a step lie on two lanes, and the weights are the second product's operand as
-// they stand.  The step's K and V go through LDS as fp16, decoded once for the
-// four waves, in the order of the operands (16-byte pieces, conflict-free both
-// ways), double buffered, one barrier a step.  The next step's bytes are in
-// flight meanwhile, page ids one step before them.
+// they stand.  K and V go through LDS as fp16, decoded once for the four waves,
+// in the order of the operands (16-byte pieces, conflict-free both ways).
+//
+// Three steps are worked on at once, so that matrix and vector instructions of
+// a wave have nothing to wait for from each other: step u's exponentials beside
+// the scores of u + 2 and the weighted V of u - 1, a vector instruction or four
+// between two matrix ones; and the maximum of u + 1 with them.  The bytes of
+// u + 4 are in flight meanwhile.
 //
 // Softmax: the running maximum m of t + e (e the exponent of V's block, as in
 // the first form) follows the scores only when one passes it by more than
@@ -36,72 +47,71 @@ constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running max
 // the 64 sums of O a lane are rarely scaled.
 template <int D, bool FP8>
 struct PromptStage {
-  static constexpr int S = FP8 ? 1 : 2;                       // bytes of a value
-  static constexpr int KP = kPpTile * D * S / 16 / kPpThreads;  // 16-byte pieces of K a thread
-  static constexpr int KC = D * S / 16;                       // pieces of a K row
-  static constexpr int KR = kPpThreads / KC;                  // rows a pass
-  static constexpr int VC = 4 * D / kPpThreads;               // V columns (of a block) a thread
+  static constexpr int S = FP8 ? 1 : 2;     // bytes of a value
+  static constexpr int KC = D * S / 16;     // 16-byte pieces of a K row
+  static constexpr int NP = kPpStep * KC;   // of a step's K, and of its V
+  // With too few for all threads, waves 0 and 1 take K and the others V.
+  static constexpr bool kShared = NP < kPpThreads;
+  static constexpr int KP = kShared ? 1 : NP / kPpThreads;  // pieces of each a thread
+  static constexpr int NB = KP;             // blocks that a wave's pieces lie in
 
-  u32x4 k[KP], v[VC][S];
-  int ks, vs;  // scale bytes of the wave's block
-  bool bad;
-  int wave;    // uniform
+  u32x4 k[KP], v[KP];  // (kShared: one of them)
+  int ks, vs;          // scale bytes of the wave's block
+  bool bad[NB];
+  int wave;            // uniform
 
-  // A wave's pieces of a pass lie in one block, so that addresses are scalars
-  // but for a lane's constant part.
-  __device__ int k_block(int j) const { return KR * j / 16 + wave * 64 / KC / 16; }
-  __device__ int v_block(int j) const { return (kPpThreads * j + 64 * wave) / D; }
-  static_assert(KR % 16 == 0, "a pass's rows");
+  // A wave's pieces of a pass lie in one block, K's and V's in the same, so
+  // that addresses are scalars but for a lane's constant part.
+  __device__ int block(int j) const { return KP == 2 ? j : kShared ? wave & 1 : wave >> 1; }
+  // The wave that hands on a block's scales.
+  __device__ bool scales_mine() const {
+    return KP == 2 ? wave == 0 : kShared ? wave < 2 : !(wave & 1);
+  }
+  __device__ static int piece(int j) {
+    return kPpThreads * j + (kShared ? threadIdx.x & 127 : threadIdx.x);
+  }
+  __device__ bool has_k() const { return !kShared || wave < 2; }
+  __device__ bool has_v() const { return !kShared || wave >= 2; }
 
-  // Page ids of the blocks that the wave fetches, and of the one whose scales
-  // it does (block `wave`).
   struct Ids {
-    int k[KP], v[VC], own;
+    int id[NB];
   };
-  __device__ Ids ids(const PagedView& c, int b, int tile) const {
+  __device__ Ids ids(const PagedView& c, int b, int step) const {
     const int* row = c.table + b * c.table_stride;
-    auto id = [&](int blk) {
-      return __builtin_amdgcn_readfirstlane(
-          row[min((4 * tile + blk) >> (c.page_shift - 4), c.max_pages - 1)]);
-    };
     Ids r;
 #pragma unroll
-    for (int j = 0; j < KP; ++j) r.k[j] = id(k_block(j));
-#pragma unroll
-    for (int j = 0; j < VC; ++j) r.v[j] = id(v_block(j));
-    r.own = id(wave);
+    for (int j = 0; j < NB; ++j)
+      r.id[j] = __builtin_amdgcn_readfirstlane(
+          row[min((2 * step + block(j)) >> (c.page_shift - 4), c.max_pages - 1)]);
     return r;
   }
-
   // (ids out of range read page 0)
-  __device__ static int64_t place(const PagedView& c, int g, int p, int tile, int blk) {
-    const int bpp = 1 << (c.page_shift - 4);
-    return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g) * bpp +
-           ((4 * tile + blk) & (bpp - 1));
+  __device__ static int64_t place(const PagedView& c, int g, int p, int blk) {
+    const int s = c.page_shift - 4;
+    return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g << s) +
+           (blk & ((1 << s) - 1));
   }
-  __device__ void load_k(const PagedView& c, int g, int tile, const Ids& r) {
-    const int t = threadIdx.x;
-    bad = (unsigned)r.own >= (unsigned)c.pages;
-    if constexpr (FP8) {
-      const int64_t at = place(c, g, r.own, tile, wave);
-      ks = c.ks[at];
-      vs = c.vs[at];
+  __device__ void load_k(const PagedView& c, int g, int step, const Ids& r) {
+#pragma unroll
+    for (int j = 0; j < KP; ++j) {
+      const int64_t at = place(c, g, r.id[j], 2 * step + block(j));
+      bad[j] = (unsigned)r.id[j] >= (unsigned)c.pages;
+      if constexpr (FP8) {
+        ks = c.ks[at];
+        vs = c.vs[at];
+      }
+      // (a pass's rows are a block's, or start at a block)
+      const unsigned lane = (piece(0) / KC & 15) * (D * S) + 16 * (piece(0) % KC);
+      if (has_k()) k[j] = *(const u32x4*)((const char*)c.k + at * (16 * D * S) + lane);
     }
-    const unsigned lane = (t / KC & 15) * (D * S) + 16 * (t % KC);
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-      k[j] = *(const u32x4*)((const char*)c.k +
-                             place(c, g, r.k[j], tile, k_block(j)) * (16 * D * S) + lane);
   }
-  __device__ void load_v(const PagedView& c, int g, int tile, const Ids& r) {
-    const unsigned lane = threadIdx.x % D * (16 * S);
+  __device__ void load_v(const PagedView& c, int g, int step, const Ids& r) {
 #pragma unroll
-    for (int j = 0; j < VC; ++j)
-#pragma unroll
-      for (int i = 0; i < S; ++i)
-        v[j][i] = *(const u32x4*)((const char*)c.v +
-                                  place(c, g, r.v[j], tile, v_block(j)) * (16 * D * S) + lane +
-                                  16 * i);
+    for (int j = 0; j < KP; ++j) {
+      const int64_t at = place(c, g, r.id[j], 2 * step + block(j));
+      const unsigned lane = piece(0) % (D * S) * 16;
+      if (has_v()) v[j] = *(const u32x4*)((const char*)c.v + at * (16 * D * S) + lane);
+    }
   }
 
   // LDS places in halves.  K: piece (8 d8 .. + 8 of a position) at (d8,
@@ -109,70 +119,64 @@ struct PromptStage {
   // different banks as they are stored (between single d8, the two lane halves
   // of a read collide: half of the LDS cycles); V: piece (block, half, column),
   // half 0 the block's positions 0-3 and 8-11, as the lane halves hold them.
-  static constexpr int kKPair = 2 * kPpTile * 8 + 16;
+  static constexpr int kKPair = 2 * kPpStep * 8 + 16;
   __device__ static int k_at(int d8, int pos) {
-    return (d8 >> 1) * kKPair + (d8 & 1) * (kPpTile * 8) + pos * 8;
+    return (d8 >> 1) * kKPair + (d8 & 1) * (kPpStep * 8) + pos * 8;
   }
-  __device__ static int v_at(int blk, int half, int d) {
-    return D / 16 * kKPair + ((blk * 2 + half) * D + d) * 8;
-  }
-  static constexpr int kBytes = 2 * (D / 16 * kKPair + kPpTile * D);  // of a step
+  static constexpr int kV = D / 16 * kKPair;  // where V begins
+  __device__ static int v_at(int blk, int half, int d) { return kV + ((blk * 2 + half) * D + d) * 8; }
+  static constexpr int kBytes = 2 * (kV + kPpStep * D);  // of a step
 
   __device__ void store_k(_Float16* buf, float* scales, float scale2) const {
-    const int t = threadIdx.x;
 #pragma unroll
     for (int j = 0; j < KP; ++j) {
-      const int row = KR * j + t / KC, piece = t % KC;
-      if constexpr (FP8) {
-        *(f16x8*)(buf + k_at(2 * piece, row)) = fp8x8_to_f16(k[j][0], k[j][1]);
-        *(f16x8*)(buf + k_at(2 * piece + 1, row)) = fp8x8_to_f16(k[j][2], k[j][3]);
-      } else {
-        *(u32x4*)(buf + k_at(piece, row)) = k[j];
+      const int row = piece(j) / KC, n = piece(j) % KC;
+      if (has_k()) {
+        if constexpr (FP8) {
+          *(f16x8*)(buf + k_at(2 * n, row)) = fp8x8_to_f16(k[j][0], k[j][1]);
+          *(f16x8*)(buf + k_at(2 * n + 1, row)) = fp8x8_to_f16(k[j][2], k[j][3]);
+        } else {
+          *(u32x4*)(buf + k_at(n, row)) = k[j];
+        }
       }
-    }
-    if ((t & 63) == 0) {
-      scales[wave] = bad ? __builtin_nanf("") : FP8 ? e8m0_value(ks) * scale2 : scale2;
-      scales[4 + wave] = FP8 ? e8m0_exponent(vs) : 0.f;
+      if (scales_mine() && (threadIdx.x & 63) == 0) {
+        scales[block(j)] = bad[j] ? __builtin_nanf("") : FP8 ? e8m0_value(ks) * scale2 : scale2;
+        scales[2 + block(j)] = FP8 ? e8m0_exponent(vs) : 0.f;
+      }
     }
   }
   // Infinities and NaN go into LDS as zeros (weight 0 times one that a row does
   // not see is not 0); returns whether the wave's part of V holds any, for
   // them to be added afterwards.
   __device__ bool store_v(_Float16* buf) const {
-    const int t = threadIdx.x;
+    if (!has_v()) return false;
     uint32_t any = 0;
 #pragma unroll
-    for (int j = 0; j < VC; ++j)
+    for (int j = 0; j < KP; ++j)
 #pragma unroll
-      for (int i = 0; i < S; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) any |= odd_values(v[j][i][e]);
+      for (int e = 0; e < 4; ++e) any |= odd_values(v[j][e]);
     const bool found = __builtin_amdgcn_ballot_w64((any & kOdd) != 0) != 0;
-    u32x4 u[VC][S];
+    u32x4 u[KP];
 #pragma unroll
-    for (int j = 0; j < VC; ++j)
-#pragma unroll
-      for (int i = 0; i < S; ++i) u[j][i] = v[j][i];
+    for (int j = 0; j < KP; ++j) u[j] = v[j];
     if (found) {
 #pragma unroll
-      for (int j = 0; j < VC; ++j)
+      for (int j = 0; j < KP; ++j)
 #pragma unroll
-        for (int i = 0; i < S; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t x = (odd_values(v[j][i][e]) & kOdd) >> (FP8 ? 7 : 15);
-            u[j][i][e] &= ~(x * (FP8 ? 0xFFu : 0xFFFFu));
-          }
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x = (odd_values(v[j][e]) & kOdd) >> (FP8 ? 7 : 15);
+          u[j][e] &= ~(x * (FP8 ? 0xFFu : 0xFFFFu));
+        }
     }
 #pragma unroll
-    for (int j = 0; j < VC; ++j) {
-      const int blk = v_block(j), d = (kPpThreads * j + t) % D;
+    for (int j = 0; j < KP; ++j) {
+      const int blk = piece(j) / (D * S), n = piece(j) % (D * S);
       if constexpr (FP8) {
-        *(f16x8*)(buf + v_at(blk, 0, d)) = fp8x8_to_f16(u[j][0][0], u[j][0][2]);
-        *(f16x8*)(buf + v_at(blk, 1, d)) = fp8x8_to_f16(u[j][0][1], u[j][0][3]);
-      } else {
-        *(u32x4*)(buf + v_at(blk, 0, d)) = u32x4{u[j][0][0], u[j][0][1], u[j][1][0], u[j][1][1]};
-        *(u32x4*)(buf + v_at(blk, 1, d)) = u32x4{u[j][0][2], u[j][0][3], u[j][1][2], u[j][1][3]};
+        *(f16x8*)(buf + v_at(blk, 0, n)) = fp8x8_to_f16(u[j][0], u[j][2]);
+        *(f16x8*)(buf + v_at(blk, 1, n)) = fp8x8_to_f16(u[j][1], u[j][3]);
+      } else {  // positions 8 (n & 1) .. + 8 of column n / 2
+        *(u32x2*)(buf + v_at(blk, 0, n >> 1) + 4 * (n & 1)) = u32x2{u[j][0], u[j][1]};
+        *(u32x2*)(buf + v_at(blk, 1, n >> 1) + 4 * (n & 1)) = u32x2{u[j][2], u[j][3]};
       }
     }
     return found;
@@ -186,17 +190,17 @@ struct PromptStage {
 };
 
 // Adds the infinities and NaN of V that the row of a lane sees, at positions of
-// steps [t0, t1), to its sums: rare, and so a plain walk over the blocks.
+// steps [u0, u1), to its sums: rare, and so a plain walk over the blocks.
 template <int D, bool FP8>
-__device__ void add_odd_values(f32x16 (&o)[D / 32], const PagedView& c, int b, int g, int t0,
-                               int t1, const RowSet& r) {
+__device__ void add_odd_values(f32x16 (&o)[D / 32], const PagedView& c, int b, int g, int u0,
+                               int u1, const RowSet& r) {
   using Stage = PromptStage<D, FP8>;
   constexpr int S = FP8 ? 1 : 2, NG = D / 32;
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  for (int blk = 4 * t0; blk < 4 * t1; ++blk) {
+  for (int blk = 2 * u0; blk < 2 * u1; ++blk) {
     const int p = c.page_of(b, blk >> (c.page_shift - 4));
     if (p < 0) continue;  // (the scores are NaN there)
-    const char* base = (const char*)c.v + Stage::place(c, g, p, 0, blk) * (16 * D * S);
+    const char* base = (const char*)c.v + Stage::place(c, g, p, blk) * (16 * D * S);
     uint32_t here = 0;  // positions of the block with one
     for (int d = lane; d < D; d += 64)
 #pragma unroll
@@ -236,6 +240,11 @@ __device__ void add_odd_values(f32x16 (&o)[D / 32], const PagedView& c, int b, i
   }
 }
 
+// Parts of a unit of so many steps.
+__device__ __forceinline__ int split_parts(const PagedAttnArgs& a, int steps) {
+  return min(max(steps / a.split_steps, 1), a.splits);
+}
+
 template <int D, bool FP8>
 __global__ __launch_bounds__(kPpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_prompt_kernel(PagedAttnArgs a) {
@@ -243,7 +252,7 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   constexpr int NG = D / 32, KS = D / 16, PS = D + 4;
   extern __shared__ __align__(16) unsigned char smem[];
   _Float16* bufs = (_Float16*)smem;  // 2 x Stage::kBytes
-  __shared__ float scales[4][8];  // (a step's are read into the next one's first half)
+  __shared__ float scales[4][4];  // of a step: k's of its two blocks, v's exponents
   __shared__ int odds[2][kPpThreads / 64];
   const PagedView& c = a.c;
   // the last rows of a sequence, which see most, first
@@ -267,15 +276,14 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   set_rows<kPpRows>(r, c, b, slot * kPpRows, a.rep, a.window, 0);
   const int rows = r.n * a.rep;
   if (slot < 0 || slot * kPpRows >= rows || (c.starts && rows <= kPaMostRows)) return;  // uniform
-  // the unit's tiles, and this split's of them
-  int t0 = r.lo_any / kPpTile, t1 = (r.hi_any + kPpTile - 1) / kPpTile;
-  int per = max(t1 - t0, 1), parts = 1;
-  if (a.splits > 1) {
-    per = max((per + a.splits - 1) / a.splits, a.split_tiles);
-    parts = (max(t1 - t0, 1) + per - 1) / per;
-    if (split >= parts) return;  // uniform
-    t0 += split * per;
-    t1 = min(t1, t0 + per);
+  // the unit's steps, and this split's of them
+  int u0 = r.lo_any / kPpStep, u1 = (r.hi_any + kPpStep - 1) / kPpStep;
+  const int parts = split_parts(a, u1 - u0);
+  if (split >= parts) return;  // uniform
+  if (parts > 1) {
+    const int per = (u1 - u0 + parts - 1) / parts;
+    u0 += split * per;
+    u1 = min(u1, u0 + per);
   }
   const int r0 = slot * kPpRows + 32 * wave;
   const bool any = r0 < rows;  // the wave has rows
@@ -295,61 +303,34 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   }
   const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
   float m = -__builtin_inff(), l = 0.f;
-  f32x16 o[NG], sa = {}, sb = {};
+  f32x16 o[NG], sa, sb, sc;
   f16x8 w[2] = {f16x8{}, f16x8{}};
+  float ks[2], ev[2];  // the scales of the step whose exponentials are next
 #pragma unroll
   for (int i = 0; i < NG; ++i) o[i] = f32x16{};
 
   Stage st;
   st.wave = wave;
-  auto buf = [&](int t) { return bufs + ((t - t0) & 1) * (Stage::kBytes / 2); };
-  // 32 scores a row: positions 32 i .. + 32 of step t
-  auto scores = [&](f32x16& s, int t, int i) {
-    const _Float16* kb = buf(t);
+  auto buf = [&](int j) { return bufs + (j & 1) * (Stage::kBytes / 2); };
+  // the scores of a step, 16 of a row on a lane: positions 8 (e / 4) + 4 half + e % 4
+  auto scores = [&](f32x16& s, int j) {
     s = f32x16{};
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const f16x8 ka = *(const f16x8*)(kb + Stage::k_at(2 * k + half, 32 * i + col));
-      s = mfma_32x32x16(ka, q[k], s);
+    for (int k = 0; k < KS; ++k)
+      s = mfma_32x32x16(*(const f16x8*)(buf(j) + Stage::k_at(2 * k + half, col)), q[k], s);
+  };
+  // A step's scales, and its scores' masks where some row does not see all of
+  // it: a position that a row does not see has no weight, whatever its block's
+  // scale is, so a NaN goes from the scale to the scores.
+  auto mask = [&](int j, f32x16& s, float (&ks)[2], float (&ev)[2]) {
+    const float* x = scales[j & 3];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      ks[k] = x[k];
+      ev[k] = x[2 + k];
     }
-  };
-  // O += the weights of positions 32 i .. of step t times their V
-  auto weigh_v = [&](int t, int i) {
-    const _Float16* kb = buf(t);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        const f16x8 va = *(const f16x8*)(kb + Stage::v_at(2 * i + k, half, 32 * n + col));
-        o[n] = mfma_32x32x16(va, w[k], o[n]);
-      }
-  };
-  // Half a step, on positions 32 i .. of step t, whose scores are in s: the
-  // matrix instructions of the half before (its weighted V) and of the half
-  // after (its scores, to `next`) run beside this one's exponentials.
-  auto half_step = [&](int t, auto i_, f32x16& s, f32x16& next) {
-    constexpr int i = i_.value;
-    const int p0 = t * kPpTile + 32 * i;
-    // the operands of the matrix instructions below, kAhead of them in flight:
-    // in turn K's of the scores and V's
-    constexpr int kOps = KS + 2 * NG, kAhead = 4;
-    static_assert(KS == 2 * NG, "as many of each");
-    const _Float16 *kbuf = buf(t + i), *vbuf = buf(t + i - 1);
-    auto operand = [&](int n) {
-      return n & 1 ? *(const f16x8*)(vbuf + Stage::v_at(2 * (1 - i) + n / 2 / NG, half,
-                                                        32 * (n / 2 % NG) + col))
-                   : *(const f16x8*)(kbuf + Stage::k_at(n + half, 32 * (1 - i) + col));
-    };
-    f16x8 op[kAhead];
-#pragma unroll
-    for (int n = 0; n < kAhead; ++n) op[n] = operand(n);
-    __builtin_amdgcn_sched_barrier(0);
-    // block 2 i + k of the step: its scales
-    const float* sc = scales[(t - t0) & 3] + 2 * i;
-    float ks[2] = {sc[0], sc[1]}, ev[2] = {sc[4], sc[5]};
-    if (p0 < r.lo_all || p0 + 32 > r.hi_all) {
-      // a position that a row does not see has no weight, whatever its block's
-      // scale is: a NaN goes from the scale to the scores
+    const int p0 = (u0 + j) * kPpStep;
+    if (p0 < r.lo_all || p0 + kPpStep > r.hi_all) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const bool bad = ks[k] != ks[k] || ev[k] != ev[k];
@@ -365,17 +346,11 @@ void paged_prompt_kernel(PagedAttnArgs a) {
         }
       }
     }
-    float mx = -__builtin_inff();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float bm = s[8 * k];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) bm = fmaxf(bm, s[8 * k + e]);
-      mx = fmaxf(mx, fmaf(bm, ks[k], ev[k]));
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+  };
+  // m follows where a score has passed it by 2^kPpLag, in whole powers of two,
+  // by which the weights in w can be scaled exactly
+  auto follow = [&](float mx) {
     if (__builtin_amdgcn_ballot_w64(mx > m + kPpLag)) {  // (-inf + lag: any score passes)
-      // a whole number, so that the factor of the weights in w is a power of two
       const float mn = fmaxf(m, ceilf(mx)), mf = mn == -__builtin_inff() ? 0.f : mn;
       const float f = __builtin_amdgcn_exp2f(m - mf);
       const _Float16 fh = (_Float16)f;
@@ -388,79 +363,132 @@ void paged_prompt_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[n][e] *= f;
     }
+  };
+  const int n = u1 - u0;
+  // Step j: s0 its scores, s1 those of j + 1, s2 gets those of j + 2.
+  auto step = [&](int j, f32x16& s0, f32x16& s1, f32x16& s2) {
+    // the operands of the matrix instructions below, kAhead of them in flight:
+    // in turn K's of the scores and V's
+    constexpr int kOps = KS + 2 * NG, kAhead = 4, kEach = 16 / kOps;
+    static_assert(KS == 2 * NG && kOps * kEach == 16, "as many of each");
+    const _Float16 *kbuf = buf(j), *vbuf = buf(j - 1);
+    auto operand = [&](int n) {
+      return n & 1
+                 ? *(const f16x8*)(vbuf + Stage::v_at(n / 2 / NG, half, 32 * (n / 2 % NG) + col))
+                 : *(const f16x8*)(kbuf + Stage::k_at(n + half, col));
+    };
+    f16x8 op[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) op[i] = operand(i);
+    __builtin_amdgcn_sched_barrier(0);
+    float ks1[2], ev1[2];
+    mask(j + 1, s1, ks1, ev1);
     const float mf = m == -__builtin_inff() ? 0.f : m;
     const float off[2] = {ev[0] - mf, ev[1] - mf};
     f16x8 wn[2];
-    float sum[2] = {0.f, 0.f};
-    next = f32x16{};
+    float sum[2] = {0.f, 0.f}, big[2] = {s1[0], s1[8]};
+    s2 = f32x16{};
 #pragma unroll
-    for (int n = 0; n < kOps; ++n) {
-      if (n & 1)
-        o[n / 2 % NG] = mfma_32x32x16(op[n % kAhead], w[n / 2 / NG], o[n / 2 % NG]);
+    for (int i = 0; i < kOps; ++i) {
+      if (i & 1)
+        o[i / 2 % NG] = mfma_32x32x16(op[i % kAhead], w[i / 2 / NG], o[i / 2 % NG]);
       else
-        next = mfma_32x32x16(op[n % kAhead], q[n / 2], next);
-      if (n + kAhead < kOps) op[n % kAhead] = operand(n + kAhead);
+        s2 = mfma_32x32x16(op[i % kAhead], q[i / 2], s2);
+      if (i + kAhead < kOps) op[i % kAhead] = operand(i + kAhead);
 #pragma unroll
-      for (int e = 16 / kOps * n; e < 16 / kOps * (n + 1); ++e) {
+      for (int e = kEach * i; e < kEach * (i + 1); ++e) {
         const int k = e >> 3;
-        float x = __builtin_amdgcn_exp2f(fmaf(s[e], ks[k], off[k]));
+        float x = __builtin_amdgcn_exp2f(fmaf(s0[e], ks[k], off[k]));
         asm volatile("" : "+v"(x));  // (in this place)
         sum[k] += x;
         wn[k][e & 7] = (_Float16)x;
+        if (e & 1) {
+          big[k] = fmaxf(fmaxf(big[k], s1[e - 1]), s1[e]);
+          asm volatile("" : "+v"(big[k]));
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k) {
       l = FP8 ? fmaf(sum[k], __builtin_amdgcn_exp2f(-ev[k]), l) : l + sum[k];
-    w[0] = wn[0];
-    w[1] = wn[1];
+      w[k] = wn[k];
+      ks[k] = ks1[k];
+      ev[k] = ev1[k];
+    }
+    // (of the step past the last, its scores are of anything)
+    if (j + 1 < n)
+      follow(halves_max(fmaxf(fmaf(big[0], ks[0], ev[0]), fmaf(big[1], ks[1], ev[1]))));
   };
 
-  // Before the loop: K and V of step t0 in LDS, the next step's in registers,
-  // zeros where the first half step looks for the V of the one before it.
-  typename Stage::Ids ids = st.ids(c, b, t0);
-  st.load_k(c, g, t0, ids);
-  st.load_v(c, g, t0, ids);
-  ids = st.ids(c, b, t0 + 1);
+  // Before the loop: the scores of the first two steps, K of the third in LDS,
+  // K of the fourth and V of the first in registers; zeros where the first step
+  // looks for the V of the one before it.  Steps past the last are not fetched:
+  // their scores, of what LDS held before, are not used.
+  auto ids = [&](int j) { return st.ids(c, b, u0 + j); };
+  {
+    const typename Stage::Ids i0 = ids(0), i1 = ids(1);
+    st.load_k(c, g, u0, i0);
+    Stage s2 = st;
+    s2.load_k(c, g, u0 + 1, i1);
+    st.store_k(buf(0), scales[0], scale2);
+    s2.store_k(buf(1), scales[1], scale2);
+    st.load_v(c, g, u0, i0);
+  }
   for (int i = tid; i < 4 * D; i += kPpThreads)
-    *(u32x4*)(buf(t0 - 1) + Stage::v_at(2, 0, 0) + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-  st.store_k(buf(t0), scales[0], scale2);
-  // steps whose V holds infinities or NaN: the wave's first, one past its last
-  int odd0 = st.store_v(buf(t0)) ? t0 : 0x7FFFFFFF, odd1 = t0 + 1;
-  if (t0 + 1 < t1) {
-    st.load_k(c, g, t0 + 1, ids);
-    st.load_v(c, g, t0 + 1, ids);
-  }
-  ids = st.ids(c, b, t0 + 2);
+    *(u32x4*)(buf(1) + Stage::kV + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+  st.load_k(c, g, u0 + 2, ids(2));
   __syncthreads();
-  if (any) scores(sa, t0, 0);
-  // A step.  K of the next one is stored in its first half and V in its second,
-  // so that the one barrier between the halves parts writers and readers: K of
-  // t + 1 is first read after it and K of t - 1 last before the barrier of
-  // t - 1; V of t is first read after it, V of t - 2 last before t - 1's.
-  using H0 = std::integral_constant<int, 0>;
-  using H1 = std::integral_constant<int, 1>;
-  for (int t = t0; t < t1; ++t) {
-    if (any) half_step(t, H0(), sa, sb);
-    if (t + 1 < t1) {
-      st.store_k(buf(t + 1), scales[(t + 1 - t0) & 3], scale2);
-      if (t + 2 < t1) st.load_k(c, g, t + 2, ids);
-    }
-    __syncthreads();
-    if (any) half_step(t, H1(), sb, sa);
-    if (t + 1 < t1) {
-      if (st.store_v(buf(t + 1))) {
-        odd0 = min(odd0, t + 1);
-        odd1 = t + 2;
-      }
-      if (t + 2 < t1) {
-        st.load_v(c, g, t + 2, ids);
-        ids = st.ids(c, b, t + 3);
-      }
-    }
+  if (any) {
+    scores(sa, 0);
+    scores(sb, 1);
+    mask(0, sa, ks, ev);
+    float big[2] = {sa[0], sa[8]};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 1; e < 8; ++e) big[k] = fmaxf(big[k], sa[8 * k + e]);
+    follow(halves_max(fmaxf(fmaf(big[0], ks[0], ev[0]), fmaf(big[1], ks[1], ev[1]))));
   }
-  if (any && t1 > t0) weigh_v(t1 - 1, 1);
+  __syncthreads();
+  st.store_k(buf(0), scales[2], scale2);
+  st.load_k(c, g, u0 + 3, ids(3));
+  typename Stage::Ids next_v = ids(1), next_k = ids(4);
+  // steps whose V holds infinities or NaN: the wave's first, one past its last
+  int odd0 = 0x7FFFFFFF, odd1 = 0;
+  // A step of the workgroup.  One barrier parts the writers and the readers of
+  // K (read of j + 2, written of j + 3) and V (read of j - 1, written of j).
+  auto round = [&](int j, f32x16& s0, f32x16& s1, f32x16& s2) {
+    __syncthreads();
+    if (any) step(j, s0, s1, s2);
+    st.store_k(buf(j + 1), scales[(j + 3) & 3], scale2);
+    if (st.store_v(buf(j))) {
+      odd0 = min(odd0, u0 + j);
+      odd1 = u0 + j + 1;
+    }
+    if (j + 1 < n) {
+      st.load_v(c, g, u0 + j + 1, next_v);
+      next_v = ids(j + 2);
+      if (j + 4 < n) {
+        st.load_k(c, g, u0 + j + 4, next_k);
+        next_k = ids(j + 5);
+      }
+    }
+  };
+  for (int j = 0; j < n; j += 3) {
+    round(j, sa, sb, sc);
+    if (j + 1 < n) round(j + 1, sb, sc, sa);
+    if (j + 2 < n) round(j + 2, sc, sa, sb);
+  }
+  __syncthreads();
+  if (any && n > 0) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+        o[i] = mfma_32x32x16(*(const f16x8*)(buf(n - 1) + Stage::v_at(k, half, 32 * i + col)),
+                             w[k], o[i]);
+  }
   if (lane == 0) {
     odds[0][wave] = odd0;
     odds[1][wave] = odd1;
@@ -468,9 +496,9 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   __syncthreads();
   odd0 = min(min(odds[0][0], odds[0][1]), min(odds[0][2], odds[0][3]));
   odd1 = max(max(odds[1][0], odds[1][1]), max(odds[1][2], odds[1][3]));
-  if (any && odd0 < odd1 && t1 > t0)
+  if (any && odd0 < odd1)
     add_odd_values<D, FP8>(o, c, b, g, __builtin_amdgcn_readfirstlane(odd0),
-                           __builtin_amdgcn_readfirstlane(min(odd1, t1)), r);
+                           __builtin_amdgcn_readfirstlane(odd1), r);
   l += __shfl_xor(l, 32);
   if (!r.live) return;
   if (parts == 1) {
@@ -517,10 +545,8 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   set_rows<kPpRows>(r, c, b, slot * kPpRows, a.rep, a.window, rw);
   const int rows = r.n * a.rep;
   if (slot < 0 || slot * kPpRows >= rows || (c.starts && rows <= kPaMostRows) || !r.live) return;
-  const int tiles =
-      max((r.hi_any + kPpTile - 1) / kPpTile - r.lo_any / kPpTile, 1);
-  const int per = max((tiles + a.splits - 1) / a.splits, a.split_tiles);
-  const int parts = (tiles + per - 1) / per;
+  const int parts = split_parts(
+      a, (r.hi_any + kPpStep - 1) / kPpStep - r.lo_any / kPpStep);
   if (parts == 1) return;
   const int d4 = 4 * (threadIdx.x % (D / 4));
   const float* p = a.part + (((int64_t)slot0 * c.Hk + g) * a.splits * kPpRows + rw) * PS;
@@ -533,11 +559,11 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
 
 struct PromptShape {
   int64_t slots;
-  int splits, split_tiles;
+  int splits, split_steps;
 };
 
 // Units of 128 rows, and the splits of the positions that fill the 512
-// workgroups the card holds of them: with few units, down to 8 steps a split;
+// workgroups the card holds of them: with few units, down to 16 steps a split;
 // with more, only to even out contexts of very different lengths.
 PromptShape prompt_shape(bool ragged, int64_t seqs, int64_t tokens, int64_t rep, int64_t kv_heads) {
   PromptShape s;
@@ -545,7 +571,7 @@ PromptShape prompt_shape(bool ragged, int64_t seqs, int64_t tokens, int64_t rep,
                    : seqs * ((tokens / std::max<int64_t>(seqs, 1) * rep + kPpRows - 1) / kPpRows);
   const int64_t units = std::max<int64_t>(s.slots * kv_heads, 1);
   s.splits = (int)std::min<int64_t>(16, std::max<int64_t>(1, (units < 512 ? 1024 : 2048) / units));
-  s.split_tiles = units < 512 ? 8 : 64;
+  s.split_steps = units < 512 ? 16 : 128;
   return s;
 }
 
@@ -569,10 +595,10 @@ int paged_prompt_launch(PagedAttnArgs a, int head_dim, hipStream_t stream) {
   a.slots = (int)s.slots;
   a.slots_each = a.c.starts ? 0 : (int)(s.slots / a.c.B);
   a.splits = s.splits;
-  a.split_tiles = s.split_tiles;
+  a.split_steps = s.split_steps;
   // no context that needs splitting
-  const int64_t tiles = (((int64_t)a.c.max_pages << a.c.page_shift) + kPpTile - 1) / kPpTile;
-  if (tiles <= s.split_tiles) a.splits = 1;
+  const int64_t steps = (((int64_t)a.c.max_pages << a.c.page_shift) + kPpStep - 1) / kPpStep;
+  if (steps < 2 * s.split_steps) a.splits = 1;
   const int64_t grid = s.slots * a.c.Hk * a.splits;
   GLQ_CHECK(s.slots * 16 < (1ll << 24) && grid < (1ll << 24), "batch of too many query rows");
   const bool fp8 = a.c.ks != nullptr, wide = head_dim == 128;
