@@ -14,18 +14,20 @@ constexpr int kPaGrid = 256;
 
 template <int D, bool FP8>
 struct RowAttention {
-  // A tile is TP positions; lane group kb has P consecutive ones of them, as
-  // rows 4 kb + j of the NT products of 16 positions and as the P values of a
-  // V column, so the weights go from one product to the next in registers.
-  static constexpr int TP = FP8 ? 64 : 32, P = TP / 4, NT = TP / 16, NM = P / 8;
+  // A tile is TP positions, in NS parts of TS; of each part, lane group kb has P
+  // consecutive ones, as rows 4 kb + j of the NT products of 16 positions and as
+  // the P values of a V column, so the weights go from one product to the next
+  // in registers.  64 positions of 128 columns or 128 of 64: 16 KB of codes.
+  static constexpr int TS = FP8 ? 64 : 32, NS = 128 / D, TP = NS * TS;
+  static constexpr int P = TS / 4, NT = TS / 16, NM = P / 8;
   static constexpr int KL = FP8 ? D / 64 : D / 32;  // 16-byte pieces of a K row and lane
   static constexpr int NC = D / 16;
   static constexpr int S = FP8 ? 1 : 2;             // bytes of a value
 
   struct Tile {
-    u32x4 k[NT][KL], v[NC];
-    int ks, vs;
-    bool bad;
+    u32x4 k[NS][NT][KL], v[NS][NC];
+    int ks[NS], vs[NS];
+    bool bad[NS];
   };
 
   const PagedView& c;
@@ -46,7 +48,7 @@ struct RowAttention {
     const f16x8* src = (const f16x8*)(qp + ((int64_t)t * Hq + h) * D);
 #pragma unroll
     for (int s = 0; s < D / 32; ++s)  // (e4m3: the two halves of a 16-code piece)
-      q[s] = r.live ? src[FP8 ? 8 * (s >> 1) + 2 * kb + (s & 1) : 4 * s + kb] : f16x8{};
+      q[s] = src[FP8 ? 8 * (s >> 1) + 2 * kb + (s & 1) : 4 * s + kb];
     m = -__builtin_inff();
     l = 0.f;
 #pragma unroll
@@ -56,50 +58,64 @@ struct RowAttention {
   // Page ids of a tile's blocks as a lane needs them, for k's rows and for v
   // (and the scales, which are the blocks' of v's lanes).
   struct Ids {
-    int k, v;
+    int k[NS], v[NS];
   };
+  __device__ static int k_block(int tile, int u, int li) {
+    return (tile * NS + u) * (TS / 16) + (FP8 ? li >> 2 : li >> 3);
+  }
+  __device__ static int v_block(int tile, int u, int kb) {
+    return (tile * NS + u) * (TS / 16) + (FP8 ? kb : kb >> 1);
+  }
   __device__ Ids ids(int tile) const {
-    const int bps = c.page_shift - 4, b0 = tile * (TP / 16);
+    const int bps = c.page_shift - 4;
     const int* row = c.table + b * c.table_stride;
-    return {row[min((b0 + (FP8 ? li >> 2 : li >> 3)) >> bps, c.max_pages - 1)],
-            row[min((b0 + (FP8 ? kb : kb >> 1)) >> bps, c.max_pages - 1)]};
+    Ids r;
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      r.k[u] = row[min(k_block(tile, u, li) >> bps, c.max_pages - 1)];
+      r.v[u] = row[min(v_block(tile, u, kb) >> bps, c.max_pages - 1)];
+    }
+    return r;
   }
 
   // A block's place in the pool; ids out of range read page 0.
   __device__ int64_t place(int p, int blk) const {
-    const int bpp = 1 << (c.page_shift - 4);
-    return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g) * bpp + (blk & (bpp - 1));
+    const int bps = c.page_shift - 4;
+    return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g << bps) +
+           (blk & ((1 << bps) - 1));
   }
   __device__ void load_k(Tile& x, int tile, Ids id) const {
-    const int b0 = tile * (TP / 16);
-    if constexpr (FP8) {
-      const int64_t vblk = place(id.v, b0 + kb);
-      x.ks = c.ks[vblk];
-      x.vs = c.vs[vblk];
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      if constexpr (FP8) {
+        const int64_t vblk = place(id.v[u], v_block(tile, u, kb));
+        x.ks[u] = c.ks[vblk];
+        x.vs[u] = c.vs[vblk];
+      }
+      x.bad[u] = (unsigned)id.v[u] >= (unsigned)c.pages;
+      const char* p = (const char*)c.k + place(id.k[u], k_block(tile, u, li)) * (16 * D * S) +
+                      ((FP8 ? 0 : 8 * ((li >> 2) & 1)) + (li & 3)) * D * S + 16 * kb;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int t = 0; t < KL; ++t) x.k[u][i][t] = *(const u32x4*)(p + 4 * i * D * S + 64 * t);
     }
-    x.bad = (unsigned)id.v >= (unsigned)c.pages;
-    const char* p = (const char*)c.k + place(id.k, b0 + (FP8 ? li >> 2 : li >> 3)) * (16 * D * S) +
-                    ((FP8 ? 0 : 8 * ((li >> 2) & 1)) + (li & 3)) * D * S + 16 * kb;
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int t = 0; t < KL; ++t) x.k[i][t] = *(const u32x4*)(p + 4 * i * D * S + 64 * t);
   }
   __device__ void load_v(Tile& x, int tile, Ids id) const {
-    const char* p = (const char*)c.v +
-                    place(id.v, tile * (TP / 16) + (FP8 ? kb : kb >> 1)) * (16 * D * S) +
-                    li * 16 * S + (FP8 ? 0 : 16 * (kb & 1));
 #pragma unroll
-    for (int i = 0; i < NC; ++i) x.v[i] = *(const u32x4*)(p + 16 * i * 16 * S);
+    for (int u = 0; u < NS; ++u) {
+      const char* p = (const char*)c.v + place(id.v[u], v_block(tile, u, kb)) * (16 * D * S) +
+                      li * 16 * S + (FP8 ? 0 : 16 * (kb & 1));
+#pragma unroll
+      for (int i = 0; i < NC; ++i) x.v[u][i] = *(const u32x4*)(p + 16 * i * 16 * S);
+    }
   }
 
-  __device__ static f16x8 k_frag(const Tile& x, int i, int s) {
-    if constexpr (FP8) {
-      const u32x4 w = x.k[i][s >> 1];
-      return fp8x8_to_f16(w[2 * (s & 1)], w[2 * (s & 1) + 1]);
-    } else {
-      return __builtin_bit_cast(f16x8, x.k[i][s]);
-    }
+  __device__ static f16x8 k_frag(const u32x4 (&k)[KL], int s) {
+    if constexpr (FP8)
+      return fp8x8_to_f16(k[s >> 1][2 * (s & 1)], k[s >> 1][2 * (s & 1) + 1]);
+    else
+      return __builtin_bit_cast(f16x8, k[s]);
   }
   __device__ static f16x8 v_frag(u32x4 v, int mm) {
     if constexpr (FP8)
@@ -117,26 +133,30 @@ struct RowAttention {
   __device__ void step(Tile& x, int tile, Next next_k) {
     const int p0 = tile * TP + P * kb;
     const bool edge = tile * TP < r.lo_all || (tile + 1) * TP > r.hi_all;
-    float t[NT][4];
-    const float ks = FP8 ? e8m0_value(x.ks) * scale2 : scale2;
-    const float ev = FP8 ? e8m0_exponent(x.vs) : 0.f;
+    float t[NS][NT][4], ev[NS];
     float mx = m;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < NS; ++u) {
+      const float ks = FP8 ? e8m0_value(x.ks[u]) * scale2 : scale2;
+      ev[u] = FP8 ? e8m0_exponent(x.vs[u]) : 0.f;
 #pragma unroll
-      for (int s = 0; s < D / 32; ++s) acc = mfma_16x16x32(k_frag(x, i, s), q[s], acc);
+      for (int i = 0; i < NT; ++i) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) t[i][j] = x.bad ? __builtin_nanf("") : fmaf(acc[j], ks, ev);
-      if (edge) {
+        for (int s = 0; s < D / 32; ++s) acc = mfma_16x16x32(k_frag(x.k[u][i], s), q[s], acc);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int p = p0 + 4 * i + j;
-          if (p < r.lo || p >= r.hi) t[i][j] = -__builtin_inff();
+        for (int j = 0; j < 4; ++j)
+          t[u][i][j] = x.bad[u] ? __builtin_nanf("") : fmaf(acc[j], ks, ev[u]);
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int p = p0 + u * TS + 4 * i + j;
+            if (p < r.lo || p >= r.hi) t[u][i][j] = -__builtin_inff();
+          }
         }
-      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, t[i][j]);
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, t[u][i][j]);
+      }
     }
     next_k();
     mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -149,24 +169,30 @@ struct RowAttention {
     for (int i = 0; i < NC; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] *= f;
-    f16x8 w[NM];
-    float ls = 0.f;
+    f16x8 w[NS][NM];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int u = 0; u < NS; ++u) {
+      float ls = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = __builtin_amdgcn_exp2f(t[i][j] - mf);
-        ls += e;
-        w[i >> 1][4 * (i & 1) + j] = (_Float16)e;
-      }
-    // (a block that the row does not see may hold any scale)
-    l = ls == 0.f ? l : fmaf(ls, __builtin_amdgcn_exp2f(-ev), l);
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e = __builtin_amdgcn_exp2f(t[u][i][j] - mf);
+          ls += e;
+          w[u][i >> 1][4 * (i & 1) + j] = (_Float16)e;
+        }
+      // (a block that the row does not see may hold any scale)
+      l = ls == 0.f ? l : fmaf(ls, __builtin_amdgcn_exp2f(-ev[u]), l);
+    }
     // weight 0 times an inf or a NaN behind a row's positions is not 0
     if (!edge || __builtin_amdgcn_ballot_w64(odd(x)) == 0) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
+      for (int u = 0; u < NS; ++u)
 #pragma unroll
-        for (int mm = 0; mm < NM; ++mm) o[i] = mfma_16x16x32(v_frag(x.v[i], mm), w[mm], o[i]);
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+          for (int mm = 0; mm < NM; ++mm)
+            o[i] = mfma_16x16x32(v_frag(x.v[u][i], mm), w[u][mm], o[i]);
     } else {
       // a token's rows at a time, with zeros for the positions that it does
       // not see
@@ -174,22 +200,26 @@ struct RowAttention {
 #pragma nounroll
       for (int k = __builtin_amdgcn_readfirstlane(tok); k <= last; ++k) {
         const int pos = r.first + k, hi = pos + 1, lo = window > 0 ? pos - window + 1 : 0;
-        const int n0 = min(max(lo - p0, 0), P), n1 = min(max(hi - p0, 0), P);
-        constexpr int E = FP8 ? 4 : 2;  // values of a word
-        auto below = [](int n) {        // the bits of its first n values
-          return n <= 0 ? 0u : n >= E ? ~0u : (1u << (32 / E * n)) - 1u;
-        };
-        u32x4 keep;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) keep[e] = below(n1 - E * e) & ~below(n0 - E * e);
+        for (int u = 0; u < NS; ++u) {
+          const int pu = p0 + u * TS;
+          const int n0 = min(max(lo - pu, 0), P), n1 = min(max(hi - pu, 0), P);
+          constexpr int E = FP8 ? 4 : 2;  // values of a word
+          auto below = [](int n) {        // the bits of its first n values
+            return n <= 0 ? 0u : n >= E ? ~0u : (1u << (32 / E * n)) - 1u;
+          };
+          u32x4 keep;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const u32x4 v = x.v[i] & keep;
-          f32x4 on = o[i];
+          for (int e = 0; e < 4; ++e) keep[e] = below(n1 - E * e) & ~below(n0 - E * e);
 #pragma unroll
-          for (int mm = 0; mm < NM; ++mm) on = mfma_16x16x32(v_frag(v, mm), w[mm], on);
+          for (int i = 0; i < NC; ++i) {
+            const u32x4 v = x.v[u][i] & keep;
+            f32x4 on = o[i];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[i][j] = tok == k ? on[j] : o[i][j];
+            for (int mm = 0; mm < NM; ++mm) on = mfma_16x16x32(v_frag(v, mm), w[u][mm], on);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = tok == k ? on[j] : o[i][j];
+          }
         }
       }
     }
@@ -199,15 +229,17 @@ struct RowAttention {
   __device__ static bool odd(const Tile& x) {
     uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
+    for (int u = 0; u < NS; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // the largest exponent field carries into the sign's place
-        if constexpr (FP8)
-          any |= (x.v[i][e] & 0x7F7F7F7Fu) + 0x01010101u;
-        else
-          any |= (x.v[i][e] & 0x7FFF7FFFu) + 0x04000400u;
-      }
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // the largest exponent field carries into the sign's place
+          if constexpr (FP8)
+            any |= (x.v[u][i][e] & 0x7F7F7F7Fu) + 0x01010101u;
+          else
+            any |= (x.v[u][i][e] & 0x7FFF7FFFu) + 0x04000400u;
+        }
     return (any & (FP8 ? 0x80808080u : 0x80008000u)) != 0;
   }
 };
@@ -284,8 +316,9 @@ struct Line {
     }
   }
 
-  // Sequence of the line's tile p, and p's place from its first one; -1 past the end.
-  __device__ int find(const PagedAttnArgs& a, int p, int& off) const {
+  // Sequence of the line's tile p, and p's place from its first one, and what
+  // weigh says of the sequence; -1 past the end.
+  __device__ int find(const PagedAttnArgs& a, int p, int& off, int& tiles, int& units) const {
     const int lane = threadIdx.x & 63;
     for (int base = 0, before = 0; base < a.c.B; base += 64) {
       int t = 0, u = 0;
@@ -302,6 +335,8 @@ struct Line {
       if (hit) {
         const int l = __builtin_ctzll(hit);
         off = __builtin_amdgcn_readlane(at, l);
+        tiles = __builtin_amdgcn_readlane(t, l);
+        units = __builtin_amdgcn_readlane(u, l);
         return base + l;
       }
       before += __builtin_amdgcn_readlane(upto, 63);
@@ -334,14 +369,13 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
   x.window = a.window;
   {
     int off = 0, left = line.quota, pos = wg0 + wave * line.quota;
-    int b = line.find(a, pos, off);
-    while (b >= 0 && b < c.B && left > 0) {  // (b grows, or off to its end)
-      int tiles, units;
-      line.weigh(a, b, tiles, units);
+    int tiles = 0, units = 0, b = line.find(a, pos, off, tiles, units);
+    while (b >= 0 && left > 0) {  // (b grows, or off to its end)
       const int size = line.rounded(tiles);
       if (off >= size * units) {
-        ++b;
+        if (++b >= c.B) break;
         off = 0;
+        line.weigh(a, b, tiles, units);
         continue;
       }
       const int unit = off / size, t0 = off - unit * size;
@@ -403,8 +437,9 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
     }
   }
   __syncthreads();
-  // Chains of pieces of one unit: the one that the workgroup begins in (v = -1),
-  // and those that begin in a wave.  Thread (row, 4 columns).
+  // Chains of pieces of one unit: the one that the workgroup begins in (slot 0 of
+  // its first wave), and those that begin in a wave (slot 1 of it).  Thread (row,
+  // 4 columns).
   const int row = tid / (D / 4), d4 = 4 * (tid % (D / 4));
   auto store = [&](const RowSet& r, int g, const Merge& acc) {
     const int tok = r.row / a.rep;
@@ -413,13 +448,18 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
   };
   Seg out[2];  // chains that another workgroup has parts of: not begun, not ended here
   out[0].unit = out[1].unit = -1;
-  for (int v = -1; v < kPaWaves; ++v) {  // uniform
-    const int v0 = max(v, 0), s0 = v < 0 ? 0 : 1;
-    const Seg head = seg[v0][s0];
-    if (head.unit < 0) continue;
-    bool ended = head.ended;
+  // a bit a (wave, slot)
+  const Seg* all = &seg[0][0];
+  const uint64_t there =
+      __builtin_amdgcn_ballot_w64(lane < 2 * kPaWaves && all[lane % (2 * kPaWaves)].unit >= 0);
+  const uint64_t last =
+      __builtin_amdgcn_ballot_w64(lane < 2 * kPaWaves && all[lane % (2 * kPaWaves)].ended);
+  for (uint64_t heads = there & (0xAAAAAAAAAAAAAAAAull | 1); heads; heads &= heads - 1) {  // uniform
+    const int h = __builtin_ctzll(heads), v0 = h >> 1, s0 = h & 1;
+    const Seg head = all[h];
+    bool ended = last >> h & 1;
     int v1 = v0 + 1;
-    while (!ended && v1 < kPaWaves && seg[v1][0].unit >= 0) ended = seg[v1++][0].ended;
+    while (!ended && v1 < kPaWaves && (there >> 2 * v1 & 1)) ended = last >> 2 * v1++ & 1;
     RowSet r;
     const int qt = head.unit / c.Hk, g = head.unit - qt * c.Hk;
     set_rows<kPaRows>(r, c, head.b, qt * kPaRows, a.rep, a.window, row & 15);
@@ -431,7 +471,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
         acc.add(p[D], p[D + 1], *(const f32x4*)(p + d4));
       }
     }
-    if (v >= 0 && ended) {
+    if (s0 && ended) {
       if (r.live) store(r, g, acc);
       continue;
     }

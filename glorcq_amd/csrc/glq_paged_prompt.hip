@@ -299,7 +299,9 @@ void paged_prompt_kernel(PagedAttnArgs a) {
     // its largest score; a scale of 0 too
     const _Float16 sign = (_Float16)(a.scale2 < 0.f ? -1.f : a.scale2 == 0.f ? 0.f : 1.f);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) q[s] = r.live ? src[2 * s + half] * sign : f16x8{};
+    for (int s = 0; s < KS; ++s) q[s] = src[2 * s + half];  // (a row that is none: the last one's)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] *= r.live ? sign : (_Float16)0.f;
   }
   const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
   float m = -__builtin_inff(), l = 0.f;
