@@ -14,6 +14,9 @@ with one launch each, keeping the framework's fp16 rounding points:
   attention (glq_decode_attention), GLoRCQLinear o projection.  Prefill (more
   than one token) and a cache that is not static or not yet allocated take
   the wrapped module's own forward;
+  With a paged cache (paged_cache.PagedStep) prompts and decode tokens alike,
+  of sequences of lengths of their own, run on paged_append and
+  paged_attention;
 * `GLoRCQQwen3DecoderLayer` -- Qwen3MoeDecoderLayer with the residual add
   after attention fused into the post-attention RMSNorm.
 
@@ -30,6 +33,7 @@ import torch.nn as nn
 
 from . import kernels
 from .moe_block import GraphCompatibleMoeBlock
+from .paged_cache import PagedStep
 
 
 class FusedRMSNorm(nn.Module):
@@ -68,6 +72,7 @@ class GLoRCQQwen3Attention(nn.Module):
         self.layer_idx = attn.layer_idx
         self.head_dim = attn.head_dim
         self.scaling = attn.scaling
+        self.window = getattr(attn, "sliding_window", None) or 0
         if attn.q_norm.variance_epsilon != attn.k_norm.variance_epsilon:
             raise RuntimeError("q_norm and k_norm must share eps")
         # q/k/v share their input: their U factors side by side, so one
@@ -139,19 +144,11 @@ class GLoRCQQwen3Attention(nn.Module):
             return self._U_qkv
         return None
 
-    def forward(self, hidden_states, position_embeddings, attention_mask, past_key_values=None,
-                qkv_xu=None, **kwargs):
-        """qkv_xu: x U partials of the q/k/v stack (3, S, B, rpad) for this
-        step's normalized hidden states, formed by their RMSNorm launch
-        (qkv_u, rmsnorm_xu)."""
-        B, S, H = hidden_states.shape
-        lay = _static_layer(past_key_values, self.layer_idx, B) if S == 1 else None
-        if lay is None or self.head_dim != 128:
-            return self.inner(hidden_states, position_embeddings, attention_mask,
-                              past_key_values=past_key_values, **kwargs)
+    def _project(self, x, qkv_xu=None):
+        """q, k and v of the normalized rows x: q item-major (n, rows, R) where
+        one batched launch forms all three."""
         inner = self.inner
-        x = hidden_states.reshape(B, H)
-        if self._qkv is not None and B <= kernels.GEMV_MAX_M:
+        if self._qkv is not None and x.shape[0] <= kernels.GEMV_MAX_M:
             c = self._qkv
             if qkv_xu is not None:  # partials per U, item i summing qkv_xu[u_index[i]]
                 y = kernels.packed_dequant_matmul_parts(
@@ -163,16 +160,45 @@ class GLoRCQQwen3Attention(nn.Module):
                     inner.q_proj.gptq_groupsize, U=c["U"], SV=c["SV"],
                     u_index=c["u_index"])  # (items, B, kv rows)
             n = y.shape[0] - 2
-            q, k, v = y[:n], y[n], y[n + 1]  # q item-major: the norm/rotary kernel reads it so
-        elif self._U_qkv is not None and B <= kernels.GEMV_MAX_M:
+            return y[:n], y[n], y[n + 1]  # q item-major: the norm/rotary kernel reads it so
+        if self._U_qkv is not None and x.shape[0] <= kernels.GEMV_MAX_M:
             xu = kernels.lowrank_xu(x.contiguous(), self._U_qkv)  # (3, B, r)
-            q = inner.q_proj(x, precomputed_xU=xu[0])
-            k = inner.k_proj(x, precomputed_xU=xu[1])
-            v = inner.v_proj(x, precomputed_xU=xu[2])
-        else:
-            q = inner.q_proj(x)
-            k = inner.k_proj(x)
-            v = inner.v_proj(x)
+            return (inner.q_proj(x, precomputed_xU=xu[0]), inner.k_proj(x, precomputed_xU=xu[1]),
+                    inner.v_proj(x, precomputed_xU=xu[2]))
+        return inner.q_proj(x), inner.k_proj(x), inner.v_proj(x)
+
+    def _forward_paged(self, hidden_states, position_embeddings, step, qkv_xu):
+        """The new tokens of a paged batch (any number a sequence): projections,
+        append with norm and rotation, attention over the pages."""
+        B, S, H = hidden_states.shape
+        inner, T, hd = self.inner, B * S, self.head_dim
+        q, k, v = self._project(hidden_states.reshape(T, H), qkv_xu)
+        cos, sin = (t.reshape(-1, hd).contiguous() for t in position_embeddings)
+        kp, vp, ks, vs = step.cache.layers[self.layer_idx]
+        at = dict(page_table=step.page_table, lengths=step.lengths, starts=step.starts,
+                  k_scales=ks, v_scales=vs)
+        qr = kernels.paged_append(k, v, kp, vp, cos=cos, sin=sin, q=q,
+                                  q_norm_w=inner.q_norm.weight, k_norm_w=inner.k_norm.weight,
+                                  eps=inner.q_norm.variance_epsilon, **at)
+        a = kernels.paged_attention(qr, kp, vp, scale=self.scaling, window=self.window,
+                                    workspace=step.workspace(qr), **at)
+        return inner.o_proj(a).reshape(B, S, -1), None
+
+    def forward(self, hidden_states, position_embeddings, attention_mask, past_key_values=None,
+                qkv_xu=None, **kwargs):
+        """qkv_xu: x U partials of the q/k/v stack (3, S, B, rpad) for this
+        step's normalized hidden states, formed by their RMSNorm launch
+        (qkv_u, rmsnorm_xu)."""
+        if isinstance(past_key_values, PagedStep):
+            return self._forward_paged(hidden_states, position_embeddings, past_key_values, qkv_xu)
+        B, S, H = hidden_states.shape
+        lay = _static_layer(past_key_values, self.layer_idx, B) if S == 1 else None
+        if lay is None or self.head_dim != 128:
+            return self.inner(hidden_states, position_embeddings, attention_mask,
+                              past_key_values=past_key_values, **kwargs)
+        inner = self.inner
+        x = hidden_states.reshape(B, H)
+        q, k, v = self._project(x, qkv_xu)
         cos, sin = position_embeddings
         if self._len is None or self._len.device != x.device:
             self._len = torch.zeros(1, dtype=torch.int32, device=x.device)

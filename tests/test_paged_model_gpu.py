@@ -1,0 +1,126 @@
+"""The Qwen3-MoE-shaped model (2 layers at full width, glorcq_amd.synthetic_model)
+over a paged cache: prompts of different lengths in one forward, decode steps
+under a captured graph.
+
+Checks: an fp16 paged cache gives the logits of the same model over the static
+cache, each prompt alone, within 2 % of their range (the bar of the model tests:
+the attention's sums and roundings differ), prompt and teacher-forced decode
+steps both; graph replays give the bits of eager steps, fp16 and 8 bits; pages
+are given back and used again."""
+
+import pytest
+import torch
+
+from glorcq_amd.graph_wrapper import _static_cache
+from glorcq_amd.paged_cache import GLoRCQPagedWrapper, PagedStep, paged_forward
+from glorcq_amd.synthetic_model import build_qwen3_moe, qwen3_moe_config
+
+pytestmark = pytest.mark.gpu
+
+VOCAB = 1024
+_CACHE = {}
+
+
+def _model(dev):
+    if "m" not in _CACHE:
+        cfg = qwen3_moe_config(num_hidden_layers=2, vocab_size=VOCAB, max_position_embeddings=512)
+        _CACHE["m"] = build_qwen3_moe(cfg, dev, seed=0)[0]
+    return _CACHE["m"]
+
+
+def _prompts(lens, dev, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, VOCAB, (n,), generator=g).to(dev) for n in lens]
+
+
+@torch.no_grad()
+def _static_logits(model, prompt, cont, dev):
+    """Logits after the prompt and after each forced token, static cache."""
+    cache = _static_cache(model, 1, 256, dev, torch.float16)
+    out = [model(input_ids=prompt[None], cache_position=torch.arange(len(prompt), device=dev),
+                 past_key_values=cache, use_cache=True, return_dict=False)[0][0, -1]]
+    for i, t in enumerate(cont):
+        pos = torch.tensor([len(prompt) + i], device=dev)
+        out.append(model(input_ids=t.view(1, 1), cache_position=pos, past_key_values=cache,
+                         use_cache=True, return_dict=False)[0][0, -1])
+    return torch.stack(out).float()
+
+
+@pytest.mark.parametrize("lens", [(5, 33, 70), (1,), (130, 2)])
+@torch.no_grad()
+def test_fp16_pages_match_static_cache(gpu, lens):
+    model = _model(gpu)
+    prompts = _prompts(lens, gpu)
+    g = torch.Generator().manual_seed(8)
+    cont = torch.randint(0, VOCAB, (4, len(lens)), generator=g).to(gpu)
+    w = GLoRCQPagedWrapper(model, max_batch_size=len(lens), max_seq_len=160, page_size=32,
+                           cache_dtype=torch.float16)
+    w.capture_graph()
+    got = [w.prefill(prompts).clone()]
+    for t in cont:
+        got.append(w.replay(t).clone())
+    torch.cuda.synchronize()
+    got = torch.stack(got).float()  # (steps, batch, vocab)
+    for b, p in enumerate(prompts):
+        ref = _static_logits(model, p, cont[:, b], gpu)
+        err = float((got[:, b] - ref).abs().max())
+        assert err <= 0.02 * float(ref.abs().max()), (b, err)
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float16])
+@torch.no_grad()
+def test_replays_match_eager_steps(gpu, dtype):
+    model = _model(gpu)
+    prompts = _prompts((40, 7, 64), gpu)
+    w = GLoRCQPagedWrapper(model, max_batch_size=3, max_seq_len=80, page_size=16,
+                           cache_dtype=dtype)
+    out, secs = w.generate(prompts, max_new_tokens=12)
+    assert secs > 0 and [len(o) for o in out] == [52, 19, 76]
+    token = torch.argmax(w.prefill(prompts), -1)
+    toks = [token]
+    for _ in range(11):
+        pos = torch.tensor([w.cache.length(b) for b in range(3)], device=gpu)
+        w.cache.extend(1)
+        logits = paged_forward(model, token, pos, PagedStep(w.cache))
+        assert bool(torch.isfinite(logits).all())
+        token = torch.argmax(logits, -1)
+        toks.append(token)
+    torch.cuda.synchronize()
+    for b, p in enumerate(prompts):
+        assert torch.equal(out[b][:len(p)], p)
+        assert torch.equal(out[b][len(p):], torch.stack(toks, 1)[b])
+
+
+@torch.no_grad()
+def test_continued_prompts_and_room(gpu):
+    """A prompt in two parts beside a decode token in one step; a wrapper stops
+    where its longest sequence is full; a released sequence's pages serve
+    another."""
+    model = _model(gpu)
+    a, b = _prompts((90, 20), gpu)
+    w = GLoRCQPagedWrapper(model, max_batch_size=2, max_seq_len=96, page_size=32,
+                           cache_dtype=torch.float16)
+    cache = w.cache
+
+    def step(parts):
+        lens = [len(p) for p in parts]
+        past = [cache.length(i) for i in range(2)]
+        cache.extend(lens)
+        st = torch.tensor([0] + lens).cumsum(0)
+        pos = torch.cat([torch.arange(p, p + n) for p, n in zip(past, lens)])
+        return paged_forward(model, torch.cat(parts), pos.to(gpu),
+                             PagedStep(cache, st.to(torch.int32).to(gpu)),
+                             last=(st[1:] - 1).to(gpu))
+
+    step([a[:50], b[:19]])
+    got = step([a[50:], b[19:]]).float()  # 40 tokens and 1
+    for i, p in enumerate((a, b)):
+        ref = _static_logits(model, p, [], gpu)[0]
+        assert float((got[i] - ref).abs().max()) <= 0.02 * float(ref.abs().max())
+    cache.release(0)
+    again = step([b, b[:0]]).float()
+    assert float((again[0] - got[1]).abs().max()) <= 0.02 * float(got[1].abs().max())
+    out, _ = w.generate([a, b], max_new_tokens=100)
+    assert [len(o) for o in out] == [97, 27]
+    with pytest.raises(RuntimeError, match="max_seq_len"):
+        w.replay(torch.zeros(2, dtype=torch.long, device=gpu))
