@@ -47,78 +47,70 @@ constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running max
 // the 64 sums of O a lane are rarely scaled.
 template <int D, bool FP8>
 struct PromptStage {
-  static constexpr int S = FP8 ? 1 : 2;     // bytes of a value
-  static constexpr int KC = D * S / 16;     // 16-byte pieces of a K row
-  static constexpr int NP = kPpStep * KC;   // of a step's K, and of its V
-  // With too few for all threads, waves 0 and 1 take K and the others V.
-  static constexpr bool kShared = NP < kPpThreads;
-  static constexpr int KP = kShared ? 1 : NP / kPpThreads;  // pieces of each a thread
-  static constexpr int NB = KP;             // blocks that a wave's pieces lie in
+  static constexpr int S = FP8 ? 1 : 2;             // bytes of a value
+  static constexpr int PB = FP8 && D == 64 ? 8 : 16;  // bytes of a piece
+  static constexpr int KC = D * S / PB;             // pieces of a K row
+  static constexpr int VC = 16 * D * S / PB;        // pieces of a V block
+  static constexpr int KP = kPpStep * KC / kPpThreads;  // pieces of K, and of V, a thread
+  static constexpr int kParts = FP8 && D == 128 ? 2 : KP;  // in which they go to LDS
 
-  u32x4 k[KP], v[KP];  // (kShared: one of them)
-  int ks, vs;          // scale bytes of the wave's block
-  bool bad[NB];
-  int wave;            // uniform
+  using Piece = std::conditional_t<PB == 8, u32x2, u32x4>;
+  Piece k[KP], v[KP];
+  int wave;  // uniform
 
   // A wave's pieces of a pass lie in one block, K's and V's in the same, so
   // that addresses are scalars but for a lane's constant part.
-  __device__ int block(int j) const { return KP == 2 ? j : kShared ? wave & 1 : wave >> 1; }
-  // The wave that hands on a block's scales.
-  __device__ bool scales_mine() const {
-    return KP == 2 ? wave == 0 : kShared ? wave < 2 : !(wave & 1);
-  }
-  __device__ static int piece(int j) {
-    return kPpThreads * j + (kShared ? threadIdx.x & 127 : threadIdx.x);
-  }
-  __device__ bool has_k() const { return !kShared || wave < 2; }
-  __device__ bool has_v() const { return !kShared || wave >= 2; }
+  __device__ int block(int j) const { return KP == 2 ? j : wave >> 1; }
 
-  struct Ids {
-    int id[NB];
-  };
-  __device__ Ids ids(const PagedView& c, int b, int step) const {
-    const int* row = c.table + b * c.table_stride;
-    Ids r;
+  // Pages and scales of the two blocks of 64 steps, a step a lane: a step finds
+  // its own in registers and waits for none.
+  int base;
+  int page[2], ks[2], vs[2];
+  __device__ void look_up(const PagedView& c, int b, int g, int step) {
+    const int s = c.page_shift - 4;
+    base = step;
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-      r.id[j] = __builtin_amdgcn_readfirstlane(
-          row[min((2 * step + block(j)) >> (c.page_shift - 4), c.max_pages - 1)]);
-    return r;
+    for (int k = 0; k < 2; ++k) {
+      const int blk = 2 * (step + (int)(threadIdx.x & 63)) + k;
+      const int p = c.table[b * c.table_stride + min(blk >> s, c.max_pages - 1)];
+      const bool bad = (unsigned)p >= (unsigned)c.pages;  // page 0 is read, its scores are NaN
+      page[k] = bad ? 0 : p;
+      ks[k] = vs[k] = 127;
+      if constexpr (FP8) {
+        const int64_t at = place(c, g, page[k], blk);
+        ks[k] = c.ks[at];
+        vs[k] = c.vs[at];
+      }
+      if (bad) ks[k] = 255;
+    }
   }
-  // (ids out of range read page 0)
   __device__ static int64_t place(const PagedView& c, int g, int p, int blk) {
     const int s = c.page_shift - 4;
-    return ((int64_t)((unsigned)p < (unsigned)c.pages ? p : 0) * c.Hk + g << s) +
-           (blk & ((1 << s) - 1));
+    return ((int64_t)p * c.Hk + g << s) + (blk & ((1 << s) - 1));
   }
-  __device__ void load_k(const PagedView& c, int g, int step, const Ids& r) {
-#pragma unroll
-    for (int j = 0; j < KP; ++j) {
-      const int64_t at = place(c, g, r.id[j], 2 * step + block(j));
-      bad[j] = (unsigned)r.id[j] >= (unsigned)c.pages;
-      if constexpr (FP8) {
-        ks = c.ks[at];
-        vs = c.vs[at];
-      }
-      // (a pass's rows are a block's, or start at a block)
-      const unsigned lane = (piece(0) / KC & 15) * (D * S) + 16 * (piece(0) % KC);
-      if (has_k()) k[j] = *(const u32x4*)((const char*)c.k + at * (16 * D * S) + lane);
-    }
+  __device__ int64_t place_of(const PagedView& c, int g, int step, int j) const {
+    const int k = block(j);
+    return place(c, g, __builtin_amdgcn_readlane(k ? page[1] : page[0], step - base), 2 * step + k);
   }
-  __device__ void load_v(const PagedView& c, int g, int step, const Ids& r) {
+  __device__ void load_k(const PagedView& c, int g, int step) {
+    // (a pass's rows are a block's, or start at a block)
+    const unsigned lane = (threadIdx.x / KC & 15) * (D * S) + PB * (threadIdx.x % KC);
 #pragma unroll
-    for (int j = 0; j < KP; ++j) {
-      const int64_t at = place(c, g, r.id[j], 2 * step + block(j));
-      const unsigned lane = piece(0) % (D * S) * 16;
-      if (has_v()) v[j] = *(const u32x4*)((const char*)c.v + at * (16 * D * S) + lane);
-    }
+    for (int j = 0; j < KP; ++j)
+      k[j] = *(const Piece*)((const char*)c.k + place_of(c, g, step, j) * (16 * D * S) + lane);
+  }
+  __device__ void load_v(const PagedView& c, int g, int step) {
+    const unsigned lane = threadIdx.x % VC * PB;
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+      v[j] = *(const Piece*)((const char*)c.v + place_of(c, g, step, j) * (16 * D * S) + lane);
   }
 
-  // LDS places in halves.  K: piece (8 d8 .. + 8 of a position) at (d8,
+  // LDS places in halves.  K: values 8 d8 .. + 8 of a position at (d8,
   // position), 32 bytes between pairs of d8 so that a row's pieces go to
   // different banks as they are stored (between single d8, the two lane halves
-  // of a read collide: half of the LDS cycles); V: piece (block, half, column),
-  // half 0 the block's positions 0-3 and 8-11, as the lane halves hold them.
+  // of a read collide: half of the LDS cycles); V: 8 values at (block, half,
+  // column), half 0 the block's positions 0-3 and 8-11, as lane halves hold them.
   static constexpr int kKPair = 2 * kPpStep * 8 + 16;
   __device__ static int k_at(int d8, int pos) {
     return (d8 >> 1) * kKPair + (d8 & 1) * (kPpStep * 8) + pos * 8;
@@ -127,65 +119,54 @@ struct PromptStage {
   __device__ static int v_at(int blk, int half, int d) { return kV + ((blk * 2 + half) * D + d) * 8; }
   static constexpr int kBytes = 2 * (kV + kPpStep * D);  // of a step
 
-  __device__ void store_k(_Float16* buf, float* scales, float scale2) const {
-#pragma unroll
-    for (int j = 0; j < KP; ++j) {
-      const int row = piece(j) / KC, n = piece(j) % KC;
-      if (has_k()) {
-        if constexpr (FP8) {
-          *(f16x8*)(buf + k_at(2 * n, row)) = fp8x8_to_f16(k[j][0], k[j][1]);
-          *(f16x8*)(buf + k_at(2 * n + 1, row)) = fp8x8_to_f16(k[j][2], k[j][3]);
-        } else {
-          *(u32x4*)(buf + k_at(n, row)) = k[j];
-        }
-      }
-      if (scales_mine() && (threadIdx.x & 63) == 0) {
-        scales[block(j)] = bad[j] ? __builtin_nanf("") : FP8 ? e8m0_value(ks) * scale2 : scale2;
-        scales[2 + block(j)] = FP8 ? e8m0_exponent(vs) : 0.f;
-      }
-    }
+  __device__ void store_k(_Float16* buf, int part) const {
+    const int j = KP == 2 ? part : 0, p = kPpThreads * j + threadIdx.x, row = p / KC, n = p % KC;
+    if constexpr (!FP8)
+      *(Piece*)(buf + k_at(n, row)) = k[j];
+    else if constexpr (PB == 8)
+      *(f16x8*)(buf + k_at(n, row)) = fp8x8_to_f16(k[0][0], k[0][1]);
+    else
+      *(f16x8*)(buf + k_at(2 * n + part, row)) = fp8x8_to_f16(k[0][2 * part], k[0][2 * part + 1]);
   }
-  // Infinities and NaN go into LDS as zeros (weight 0 times one that a row does
-  // not see is not 0); returns whether the wave's part of V holds any, for
-  // them to be added afterwards.
-  __device__ bool store_v(_Float16* buf) const {
-    if (!has_v()) return false;
-    uint32_t any = 0;
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) any |= odd_values(v[j][e]);
-    const bool found = __builtin_amdgcn_ballot_w64((any & kOdd) != 0) != 0;
-    u32x4 u[KP];
-#pragma unroll
-    for (int j = 0; j < KP; ++j) u[j] = v[j];
-    if (found) {
-#pragma unroll
-      for (int j = 0; j < KP; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t x = (odd_values(v[j][e]) & kOdd) >> (FP8 ? 7 : 15);
-          u[j][e] &= ~(x * (FP8 ? 0xFFu : 0xFFFFu));
-        }
+  __device__ static void store_v(_Float16* buf, const Piece (&v)[KP], int part) {
+    const int j = KP == 2 ? part : 0, p = kPpThreads * j + threadIdx.x, blk = p / VC, n = p % VC;
+    if constexpr (FP8 && PB == 16) {  // a column of the block
+      *(f16x8*)(buf + v_at(blk, part, n)) = fp8x8_to_f16(v[0][part], v[0][part + 2]);
+    } else {  // positions 8 (n & 1) .. + 8 of column n / 2
+      u32x4 x;
+      if constexpr (FP8)
+        x = __builtin_bit_cast(u32x4, fp8x8_to_f16(v[0][0], v[0][1]));
+      else
+        x = v[j];
+      *(u32x2*)(buf + v_at(blk, 0, n >> 1) + 4 * (n & 1)) = u32x2{x[0], x[1]};
+      *(u32x2*)(buf + v_at(blk, 1, n >> 1) + 4 * (n & 1)) = u32x2{x[2], x[3]};
     }
-#pragma unroll
-    for (int j = 0; j < KP; ++j) {
-      const int blk = piece(j) / (D * S), n = piece(j) % (D * S);
-      if constexpr (FP8) {
-        *(f16x8*)(buf + v_at(blk, 0, n)) = fp8x8_to_f16(u[j][0], u[j][2]);
-        *(f16x8*)(buf + v_at(blk, 1, n)) = fp8x8_to_f16(u[j][1], u[j][3]);
-      } else {  // positions 8 (n & 1) .. + 8 of column n / 2
-        *(u32x2*)(buf + v_at(blk, 0, n >> 1) + 4 * (n & 1)) = u32x2{u[j][0], u[j][1]};
-        *(u32x2*)(buf + v_at(blk, 1, n >> 1) + 4 * (n & 1)) = u32x2{u[j][2], u[j][3]};
-      }
-    }
-    return found;
   }
   // Of a word of values, the top bit of each infinity or NaN (with kOdd).
   static constexpr uint32_t kOdd = FP8 ? 0x80808080u : 0x80008000u;
   __device__ static uint32_t odd_values(uint32_t w) {
     // (the largest exponent field carries into the sign's place)
     return FP8 ? (w & 0x7F7F7F7Fu) + 0x01010101u : (w & 0x7FFF7FFFu) + 0x04000400u;
+  }
+  __device__ uint32_t odd_in_v(int j) const {
+    uint32_t any = 0;
+#pragma unroll
+    for (int e = 0; e < PB / 4; ++e) any |= odd_values(v[j][e]);
+    return any;
+  }
+  // Infinities and NaN go into LDS as zeros (weight 0 times one that a row does
+  // not see is not 0; they are added afterwards): V again, where it has any.
+  __device__ void store_v_finite(_Float16* buf) const {
+    Piece u[KP];
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+#pragma unroll
+      for (int e = 0; e < PB / 4; ++e) {
+        const uint32_t x = (odd_values(v[j][e]) & kOdd) >> (FP8 ? 7 : 15);
+        u[j][e] = v[j][e] & ~(x * (FP8 ? 0xFFu : 0xFFFFu));
+      }
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) store_v(buf, u, i);
   }
 };
 
@@ -249,10 +230,9 @@ template <int D, bool FP8>
 __global__ __launch_bounds__(kPpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_prompt_kernel(PagedAttnArgs a) {
   using Stage = PromptStage<D, FP8>;
-  constexpr int NG = D / 32, KS = D / 16, PS = D + 4;
+  constexpr int NG = D / 32, KS = D / 16, PS = D + 4, kOps = KS + 2 * NG;
   extern __shared__ __align__(16) unsigned char smem[];
   _Float16* bufs = (_Float16*)smem;  // 2 x Stage::kBytes
-  __shared__ float scales[4][4];  // of a step: k's of its two blocks, v's exponents
   __shared__ int odds[2][kPpThreads / 64];
   const PagedView& c = a.c;
   // the last rows of a sequence, which see most, first
@@ -325,11 +305,10 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   // it: a position that a row does not see has no weight, whatever its block's
   // scale is, so a NaN goes from the scale to the scores.
   auto mask = [&](int j, f32x16& s, float (&ks)[2], float (&ev)[2]) {
-    const float* x = scales[j & 3];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      ks[k] = x[k];
-      ev[k] = x[2 + k];
+      ks[k] = e8m0_value(__builtin_amdgcn_readlane(st.ks[k], u0 + j - st.base)) * scale2;
+      ev[k] = e8m0_exponent(__builtin_amdgcn_readlane(st.vs[k], u0 + j - st.base));
     }
     const int p0 = (u0 + j) * kPpStep;
     if (p0 < r.lo_all || p0 + kPpStep > r.hi_all) {
@@ -367,11 +346,12 @@ void paged_prompt_kernel(PagedAttnArgs a) {
     }
   };
   const int n = u1 - u0;
-  // Step j: s0 its scores, s1 those of j + 1, s2 gets those of j + 2.
-  auto step = [&](int j, f32x16& s0, f32x16& s1, f32x16& s2) {
+  // Step j: s0 its scores, s1 those of j + 1, s2 gets those of j + 2.  other(i):
+  // what else the wave has to do, in kOps parts.
+  auto step = [&](int j, f32x16& s0, f32x16& s1, f32x16& s2, auto other) {
     // the operands of the matrix instructions below, kAhead of them in flight:
     // in turn K's of the scores and V's
-    constexpr int kOps = KS + 2 * NG, kAhead = 4, kEach = 16 / kOps;
+    constexpr int kAhead = 4, kEach = 16 / kOps;
     static_assert(KS == 2 * NG && kOps * kEach == 16, "as many of each");
     const _Float16 *kbuf = buf(j), *vbuf = buf(j - 1);
     auto operand = [&](int n) {
@@ -397,6 +377,7 @@ void paged_prompt_kernel(PagedAttnArgs a) {
       else
         s2 = mfma_32x32x16(op[i % kAhead], q[i / 2], s2);
       if (i + kAhead < kOps) op[i % kAhead] = operand(i + kAhead);
+      other(i);
 #pragma unroll
       for (int e = kEach * i; e < kEach * (i + 1); ++e) {
         const int k = e >> 3;
@@ -427,19 +408,21 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   // K of the fourth and V of the first in registers; zeros where the first step
   // looks for the V of the one before it.  Steps past the last are not fetched:
   // their scores, of what LDS held before, are not used.
-  auto ids = [&](int j) { return st.ids(c, b, u0 + j); };
+  st.look_up(c, b, g, u0);
   {
-    const typename Stage::Ids i0 = ids(0), i1 = ids(1);
-    st.load_k(c, g, u0, i0);
     Stage s2 = st;
-    s2.load_k(c, g, u0 + 1, i1);
-    st.store_k(buf(0), scales[0], scale2);
-    s2.store_k(buf(1), scales[1], scale2);
-    st.load_v(c, g, u0, i0);
+    st.load_k(c, g, u0);
+    s2.load_k(c, g, u0 + 1);
+    st.load_v(c, g, u0);
+#pragma unroll
+    for (int i = 0; i < Stage::kParts; ++i) {
+      st.store_k(buf(0), i);
+      s2.store_k(buf(1), i);
+    }
   }
   for (int i = tid; i < 4 * D; i += kPpThreads)
     *(u32x4*)(buf(1) + Stage::kV + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-  st.load_k(c, g, u0 + 2, ids(2));
+  st.load_k(c, g, u0 + 2);
   __syncthreads();
   if (any) {
     scores(sa, 0);
@@ -453,29 +436,45 @@ void paged_prompt_kernel(PagedAttnArgs a) {
     follow(halves_max(fmaxf(fmaf(big[0], ks[0], ev[0]), fmaf(big[1], ks[1], ev[1]))));
   }
   __syncthreads();
-  st.store_k(buf(0), scales[2], scale2);
-  st.load_k(c, g, u0 + 3, ids(3));
-  typename Stage::Ids next_v = ids(1), next_k = ids(4);
+#pragma unroll
+  for (int i = 0; i < Stage::kParts; ++i) st.store_k(buf(0), i);
+  st.load_k(c, g, u0 + 3);
   // steps whose V holds infinities or NaN: the wave's first, one past its last
   int odd0 = 0x7FFFFFFF, odd1 = 0;
   // A step of the workgroup.  One barrier parts the writers and the readers of
   // K (read of j + 2, written of j + 3) and V (read of j - 1, written of j).
   auto round = [&](int j, f32x16& s0, f32x16& s1, f32x16& s2) {
+    // (of steps j + 1 to j + 4 below)
+    if (u0 + j + 5 > st.base + 64) st.look_up(c, b, g, u0 + j);
     __syncthreads();
-    if (any) step(j, s0, s1, s2);
-    st.store_k(buf(j + 1), scales[(j + 3) & 3], scale2);
-    if (st.store_v(buf(j))) {
+    uint32_t found = 0;
+    // K of j + 3 and V of j to LDS, K of j + 4 and V of j + 1 on their way
+    // (steps past the last: what lies there of the last pages, not used)
+    auto other = [&](int i) {
+      constexpr int U = kOps / 8;
+#pragma unroll
+      for (int part = 0; part < Stage::kParts; ++part) {
+        if (i == U * part) st.store_k(buf(j + 1), part);
+        if (i == U * (2 + part)) Stage::store_v(buf(j), st.v, part);
+      }
+      if (i == 4 * U) {
+#pragma unroll
+        for (int p = 0; p < Stage::KP; ++p) found |= st.odd_in_v(p);
+      }
+      if (i == 5 * U) st.load_k(c, g, u0 + j + 4);
+    };
+    if (any) {
+      step(j, s0, s1, s2, other);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kOps; ++i) other(i);
+    }
+    if (__builtin_amdgcn_ballot_w64((found & Stage::kOdd) != 0)) {
+      st.store_v_finite(buf(j));
       odd0 = min(odd0, u0 + j);
       odd1 = u0 + j + 1;
     }
-    if (j + 1 < n) {
-      st.load_v(c, g, u0 + j + 1, next_v);
-      next_v = ids(j + 2);
-      if (j + 4 < n) {
-        st.load_k(c, g, u0 + j + 4, next_k);
-        next_k = ids(j + 5);
-      }
-    }
+    st.load_v(c, g, u0 + j + 1);
   };
   for (int j = 0; j < n; j += 3) {
     round(j, sa, sb, sc);
