@@ -12,6 +12,18 @@ constexpr int kPaThreads = 512;
 constexpr int kPaWaves = kPaThreads / 64;
 constexpr int kPaGrid = 256;
 
+// A wave takes 16 query rows (tokens x the KV head's q heads) of one KV head
+// over some of their positions, a tile of 16 KB at a time:
+//   S^T = K Q^T   v_mfma_f32_16x16x32_f16, A = 16 positions of K, B = the rows
+//   O^T += V^T P^T                         A = 16 columns of V,   B = the weights
+// so that a row's scores of a tile lie on the four lanes of its column, and
+// need two exchanges for their maximum and none for the second product.
+//
+// Bound by the pages' bytes, which go from memory to registers, 16 bytes a lane
+// and load, without LDS: each is used once.  8 waves of 200 registers a CU keep
+// 128 KB in flight there.  64 sequences of 3 to 8000 positions, 8-bit pages:
+// 61 us, 4.8 TB/s, what a copy reaches (a read alone 6.1); one sequence of
+// 130000: 36 us, 3.7 TB/s; of 517, 10 us, of which 5 are an empty launch's.
 template <int D, bool FP8>
 struct RowAttention {
   // A tile is TP positions, in NS parts of TS; of each part, lane group kb has P
@@ -265,7 +277,9 @@ __device__ __forceinline__ int sequence_tiles(const RowSet& r, int window) {
 // parts a workgroup, not a cache's length of them.
 //
 // Where every unit fits a workgroup with at most kPaShort tiles a wave, a unit
-// gets a workgroup of its own, and nothing goes through memory.
+// gets a workgroup of its own, and nothing goes through memory: one sequence of
+// 517 positions 10.2 us, 15.8 without the rule; with 16 tiles a wave, 4
+// sequences of 4000 fp16 positions 44 us instead of 33.
 constexpr int kPaShort = 4;
 
 // The line, as every wave works it out for itself: 64 sequences a step.
@@ -605,6 +619,8 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
                 (1ll << 31) / most - 1,
             "a batch of too many rows for its page table's length");
   a.slots_each = (int)((rows_each + kPaRows - 1) / kPaRows);
+  // (rows of the pieces' places in LDS: of 8, two threads merge a value's parts;
+  // a sequence of 60000 positions 30 us, 37 with 16; 64 of 3000 46 and 45)
   a.rows = !starts && rows_each <= 8 ? 8 : kPaRows;
   const size_t lds = (size_t)kPaWaves * 2 * a.rows * (D + 4) * 4;
   auto kern = D == 128 ? (a.c.ks ? paged_rows_kernel<128, true> : paged_rows_kernel<128, false>)

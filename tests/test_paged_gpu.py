@@ -313,6 +313,26 @@ def test_attention_split(gpu, dtype, D, page, Hq, Hk, news, past, window):
 
 
 @pytest.mark.parametrize("dtype", [FP8, FP16])
+@pytest.mark.parametrize("D,page,Hq,Hk,news,past,window", [
+    (128, 64, 8, 1, [8, 8], [70, 1000], 0),        # 64 rows a sequence
+    (128, 64, 8, 1, [9, 9], [70, 1000], 0),        # 72
+    (64, 16, 4, 2, [32, 33, 1], [40, 700, 90], 0),  # 64, 66 and 2 in a batch
+    (128, 64, 8, 1, [40], [3000], 0),              # few units over a long context
+    (128, 32, 4, 2, [130, 70], [2600, 1500], 0),
+    (64, 128, 8, 1, [33, 20], [4100, 33], 2000),
+    (64, 16, 2, 2, [100] * 3, [900, 0, 2500], 0),
+])
+def test_attention_prompt_split(gpu, dtype, D, page, Hq, Hk, news, past, window):
+    """Rows about the limit between the two forms, and prompts whose positions
+    are split over workgroups."""
+    c = Cache(gpu, len(news), Hk, D, page, dtype, max(map(sum, zip(news, past))) + page, 31)
+    c.fill([n + p for n, p in zip(news, past)])
+    q = (torch.randn(sum(news), Hq, D, generator=c.g) * 2).half().to(gpu)
+    y = check_attend(c, q, news, D ** -0.5, window=window)
+    assert torch.equal(y, check_attend(c, q, news, D ** -0.5, window=window))
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
 @pytest.mark.parametrize("window", [1, 16, 50, 200, 100000])
 def test_attention_window(gpu, dtype, window):
     news, past = [1, 40, 7, 90], [300, 0, 150, 60]
@@ -409,6 +429,59 @@ def test_rows_that_see_nothing(gpu, dtype):
     # a window that the bad page lies outside of
     y = kernels.paged_attention(q, kp, vp, c.table, c.lengths, 0.125, starts=st, window=7, **s)
     assert not y[5:7].isnan().any() and not y[9:12].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_rows_that_see_nothing(gpu, dtype, D):
+    """The same for prompts."""
+    c = Cache(gpu, 4, 1, D, 16, dtype, 800, 32)
+    c.fill([40, 700, 784, 100])
+    news = [90, 80, 75, 0]
+    st = batch(news, gpu)
+    q = torch.randn(250, 2, D, generator=c.g).half().to(gpu)
+    c.lengths[2] = c.table.shape[1] * 16 + 1  # its last position is past the table
+    c.table[1, 10] = c.pool                   # positions 160 .. 175 of sequence 1
+    out = torch.full((250, 2 * D), 7.0, dtype=torch.float16, device=gpu)
+    s, kp, vp = c.pages()
+    y = kernels.paged_attention(q, kp, vp, c.table, c.lengths, 0.125, starts=st, out=out, **s).cpu()
+    assert not y[:50].any()
+    ref, tol = R.attend(q[50:90].cpu(), c.model.k[0], c.model.v[0], c.model.ev[0], 0, 0.125, 0,
+                        c.fp8)
+    assert ((y[50:90].double().view(ref.shape) - ref).abs() <= tol).all()
+    assert y[90:170].isnan().all() and y[244].isnan().all()
+    # (positions 726 .. 783 of sequence 2; 784 .. 799 hold any bits)
+    assert not y[170:228].isnan().any() and (y[245:] == 7.0).all()
+    # a window that the bad page lies outside of
+    y = kernels.paged_attention(q, kp, vp, c.table, c.lengths, 0.125, starts=st, window=440, **s)
+    assert not y[90:170].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+def test_prompt_split_with_infinities(gpu, dtype):
+    """Infinities (NaN in 8 bits) of V inside the splits of a prompt's context,
+    seen by all rows or by some."""
+    c = Cache(gpu, 1, 1, 128, 64, dtype, 2200, 33)
+    c.fill([2100])
+    n, first = 60, 2040
+    for p, d, x in ((3, 5, "inf"), (1500, 5, "inf"), (700, 9, "-inf"), (1999, 11, "nan"),
+                    (2070, 20, "inf")):
+        c.model.v[0][p, 0, d] = float(x if dtype == FP16 else "nan")
+    c.upload()
+    q = torch.randn(n, 4, 128, generator=c.g).half().to(gpu)
+    s, kp, vp = c.pages()
+    y = kernels.paged_attention(q, kp, vp, c.table, c.lengths, 0.1, **s).cpu().double().view(n, 4, 128)
+    v = c.model.v[0]
+    ref, tol = R.attend(q.cpu(), c.model.k[0], torch.nan_to_num(v, nan=0., posinf=0., neginf=0.),
+                        c.model.ev[0], first, 0.1, 0, c.fp8)
+    odd = {5: range(n), 9: range(n), 11: range(n), 20: range(30, n)}
+    for d in range(128):
+        rows = torch.tensor([i in odd.get(d, ()) for i in range(n)])
+        assert not y[rows, :, d].isfinite().any()
+        assert ((y[~rows, :, d] - ref[~rows, :, d]).abs() <= tol[~rows, :, d]).all()
+    if dtype == FP16:
+        assert (y[:, :, 5] == float("inf")).all() and (y[:, :, 9] == float("-inf")).all()
+        assert y[:, :, 11].isnan().all() and (y[30:, :, 20] == float("inf")).all()
 
 
 @pytest.mark.parametrize("dtype", [FP8, FP16])
