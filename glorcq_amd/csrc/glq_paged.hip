@@ -9,6 +9,7 @@ namespace {
 
 constexpr int kAppThreads = 256;
 constexpr int kMinScale = 127 - 32;  // the smallest scale byte written: 2^-32
+constexpr int kQPasses = 4;          // of a wave over q
 
 struct AppendArgs {
   PagedView c;
@@ -20,7 +21,7 @@ struct AppendArgs {
   int64_t cs_stride;        // 0 when one row serves every token
   __half* q_out;            // (T, Hq, D)
   int Hq;
-  int units, slots, kv_waves, q_passes;
+  int units, slots, kv_waves;
   float eps;
 };
 
@@ -96,7 +97,18 @@ __device__ __forceinline__ int scale_byte(float amax) {
 // new ones need a larger one; then its codes are scaled down by the power of
 // two.  What lies behind the last token of an 8-bit block is zero.
 //
-// The other waves rotate q, 64 / (D / 8) heads a pass.
+// V goes through LDS, from rows of a token to columns of 16 tokens, so that
+// pages are written in 16-byte pieces of whole 16-token columns.
+//
+// The other waves rotate q, 64 / (D / 8) heads a pass, 4 passes each: 16000
+// tokens of 32 heads take 82 us with 4 and 86 with one; up to 4000 tokens
+// (19 us) it makes no difference.
+//
+// Bound by memory: each token's q, k and v are read once, q and the pages
+// written once.  8000 tokens of 32 and 4 heads of 128 into 8-bit pages: 34 us;
+// 7 ragged prompts of 7200 tokens with norms 30.5 us, 4.8 TB/s, what a copy
+// reaches (a first form that gave a workgroup a token: 43).  One token: 6.6 us,
+// the launch.
 template <int D, bool FP8>
 __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(AppendArgs a) {
   constexpr int L = D / 8;         // lanes of a head
@@ -112,8 +124,8 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(AppendArgs a)
     // rows (token, q head)
     const int Tn = c.starts ? c.start(c.B) : c.T;
     const int64_t rows = (int64_t)Tn * a.Hq;
-    int64_t r0 = (int64_t)(wave - a.kv_waves) * a.q_passes * TP;
-    for (int p = 0; p < a.q_passes; ++p, r0 += TP) {
+    int64_t r0 = (int64_t)(wave - a.kv_waves) * kQPasses * TP;
+    for (int p = 0; p < kQPasses; ++p, r0 += TP) {
       if (r0 >= rows) return;  // uniform
       const bool in = r0 + tk < rows;
       const int64_t r = in ? r0 + tk : rows - 1;
@@ -374,9 +386,8 @@ extern "C" int glq_paged_append(const glq_paged_append_params* p, void* stream) 
   const int64_t slots = starts ? tokens / kBlkTokens + 2 * cache->seqs : cache->seqs * a.units;
   const int64_t kvw = align_up(slots * 2 * Hk, kAppThreads / 64);
   const int64_t rows = q ? tokens * q_heads : 0;
-  const int per = (int)(64 / (D / 8));
-  a.q_passes = rows >= 32768 ? 4 : 1;
-  const int64_t qw = (rows + (int64_t)per * a.q_passes - 1) / (per * a.q_passes);
+  const int64_t per = 64 / (D / 8) * kQPasses;
+  const int64_t qw = (rows + per - 1) / per;
   const int64_t blocks = (kvw + qw + kAppThreads / 64 - 1) / (kAppThreads / 64);
   GLQ_CHECK(blocks < (1ll << 24), "batch of too many (token, head) rows");
   a.kv_waves = (int)kvw;
