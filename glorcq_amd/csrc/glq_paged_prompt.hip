@@ -24,6 +24,7 @@ __device__ __forceinline__ float halves_max(float x) {
 
 constexpr int kPpThreads = 256;
 constexpr int kPpStep = 32;    // positions of a step: two blocks
+constexpr int64_t kPpParts = 2048;  // of units in several, at most: 138 MB
 constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running maximum
 
 // One workgroup takes 128 query rows (tokens x the KV head's q heads) of one KV
@@ -38,8 +39,15 @@ constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running max
 // Three steps are worked on at once, so that matrix and vector instructions of
 // a wave have nothing to wait for from each other: step u's exponentials beside
 // the scores of u + 2 and the weighted V of u - 1, a vector instruction or four
-// between two matrix ones; and the maximum of u + 1 with them.  The bytes of
-// u + 4 are in flight meanwhile.
+// between two matrix ones; and the maximum of u + 1 and the way of K of u + 3
+// and V of u to LDS with them.  The bytes of two steps more are in flight.
+//
+// Bound by instructions: of a CU's 2700 cycles for two workgroups' steps, 1024
+// are matrix instructions', about as many LDS transfers' and 1300 vector ones'
+// (a step of a workgroup alone on its CU takes 1950, one wave's time to issue
+// it).  4096 tokens of 32 and 4 heads: 196 us, 700 TF/s of what the mask leaves;
+// 512 behind 30000: 314 us, 810 TF/s (a library product of 8192^3 reaches 1143,
+// these matrix instructions alone 1190).
 //
 // Softmax: the running maximum m of t + e (e the exponent of V's block, as in
 // the first form) follows the scores only when one passes it by more than
@@ -55,7 +63,10 @@ struct PromptStage {
   static constexpr int kParts = FP8 && D == 128 ? 2 : KP;  // in which they go to LDS
 
   using Piece = std::conditional_t<PB == 8, u32x2, u32x4>;
-  Piece k[KP], v[KP];
+  // Steps whose bytes are in flight, each in registers of its own (pieces of
+  // fp16 heads of 128 have none left for two).
+  static constexpr int kSets = KP * PB / 4 > 4 ? 1 : 2;
+  Piece k[kSets][KP], v[kSets][KP];
   int wave;  // uniform
 
   // A wave's pieces of a pass lie in one block, K's and V's in the same, so
@@ -83,6 +94,8 @@ struct PromptStage {
       }
       if (bad) ks[k] = 255;
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) asm volatile("" : "+v"(ks[k]), "+v"(vs[k]));  // (waits for them)
   }
   __device__ static int64_t place(const PagedView& c, int g, int p, int blk) {
     const int s = c.page_shift - 4;
@@ -92,18 +105,20 @@ struct PromptStage {
     const int k = block(j);
     return place(c, g, __builtin_amdgcn_readlane(k ? page[1] : page[0], step - base), 2 * step + k);
   }
+  template <int SET>
   __device__ void load_k(const PagedView& c, int g, int step) {
     // (a pass's rows are a block's, or start at a block)
     const unsigned lane = (threadIdx.x / KC & 15) * (D * S) + PB * (threadIdx.x % KC);
 #pragma unroll
     for (int j = 0; j < KP; ++j)
-      k[j] = *(const Piece*)((const char*)c.k + place_of(c, g, step, j) * (16 * D * S) + lane);
+      k[SET][j] = *(const Piece*)((const char*)c.k + place_of(c, g, step, j) * (16 * D * S) + lane);
   }
+  template <int SET>
   __device__ void load_v(const PagedView& c, int g, int step) {
     const unsigned lane = threadIdx.x % VC * PB;
 #pragma unroll
     for (int j = 0; j < KP; ++j)
-      v[j] = *(const Piece*)((const char*)c.v + place_of(c, g, step, j) * (16 * D * S) + lane);
+      v[SET][j] = *(const Piece*)((const char*)c.v + place_of(c, g, step, j) * (16 * D * S) + lane);
   }
 
   // LDS places in halves.  K: values 8 d8 .. + 8 of a position at (d8,
@@ -119,7 +134,7 @@ struct PromptStage {
   __device__ static int v_at(int blk, int half, int d) { return kV + ((blk * 2 + half) * D + d) * 8; }
   static constexpr int kBytes = 2 * (kV + kPpStep * D);  // of a step
 
-  __device__ void store_k(_Float16* buf, int part) const {
+  __device__ static void store_k(_Float16* buf, const Piece (&k)[KP], int part) {
     const int j = KP == 2 ? part : 0, p = kPpThreads * j + threadIdx.x, row = p / KC, n = p % KC;
     if constexpr (!FP8)
       *(Piece*)(buf + k_at(n, row)) = k[j];
@@ -148,15 +163,15 @@ struct PromptStage {
     // (the largest exponent field carries into the sign's place)
     return FP8 ? (w & 0x7F7F7F7Fu) + 0x01010101u : (w & 0x7FFF7FFFu) + 0x04000400u;
   }
-  __device__ uint32_t odd_in_v(int j) const {
+  __device__ static uint32_t odd_in(const Piece& v) {
     uint32_t any = 0;
 #pragma unroll
-    for (int e = 0; e < PB / 4; ++e) any |= odd_values(v[j][e]);
+    for (int e = 0; e < PB / 4; ++e) any |= odd_values(v[e]);
     return any;
   }
   // Infinities and NaN go into LDS as zeros (weight 0 times one that a row does
   // not see is not 0; they are added afterwards): V again, where it has any.
-  __device__ void store_v_finite(_Float16* buf) const {
+  __device__ static void store_v_finite(_Float16* buf, const Piece (&v)[KP]) {
     Piece u[KP];
 #pragma unroll
     for (int j = 0; j < KP; ++j)
@@ -235,12 +250,14 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   _Float16* bufs = (_Float16*)smem;  // 2 x Stage::kBytes
   __shared__ int odds[2][kPpThreads / 64];
   const PagedView& c = a.c;
-  // the last rows of a sequence, which see most, first
+  // KV head fastest, then the unit, the last rows of a sequence, which see most,
+  // first; the split last, so that those that a unit does not have are the
+  // grid's end (between others, they leave whole dies without work).
   int id = blockIdx.x;
-  const int split = id % a.splits;
-  id /= a.splits;
   const int g = id % c.Hk;
-  int slot = a.slots - 1 - id / c.Hk, b;
+  id /= c.Hk;
+  const int split = id / a.slots;
+  int slot = a.slots - 1 - id % a.slots, b;
   const int slot0 = slot;
   if (c.starts) {
     b = slot_sequence(c, a.rep, kPpRows, 1, slot);
@@ -266,7 +283,6 @@ void paged_prompt_kernel(PagedAttnArgs a) {
     u1 = min(u1, u0 + per);
   }
   const int r0 = slot * kPpRows + 32 * wave;
-  const bool any = r0 < rows;  // the wave has rows
   set_rows<32>(r, c, b, min(r0, rows - 1), a.rep, a.window, col);
   r.live = r0 + col < rows;
   const int Hq = c.Hk * a.rep, tok = r.row / a.rep;
@@ -408,26 +424,28 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   // K of the fourth and V of the first in registers; zeros where the first step
   // looks for the V of the one before it.  Steps past the last are not fetched:
   // their scores, of what LDS held before, are not used.
+  constexpr int kSets = Stage::kSets, kOther = kSets - 1;
   st.look_up(c, b, g, u0);
   {
     Stage s2 = st;
-    st.load_k(c, g, u0);
-    s2.load_k(c, g, u0 + 1);
-    st.load_v(c, g, u0);
+    st.template load_k<0>(c, g, u0);
+    s2.template load_k<0>(c, g, u0 + 1);
 #pragma unroll
     for (int i = 0; i < Stage::kParts; ++i) {
-      st.store_k(buf(0), i);
-      s2.store_k(buf(1), i);
+      Stage::store_k(buf(0), st.k[0], i);
+      Stage::store_k(buf(1), s2.k[0], i);
     }
   }
   for (int i = tid; i < 4 * D; i += kPpThreads)
     *(u32x4*)(buf(1) + Stage::kV + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-  st.load_k(c, g, u0 + 2);
+  st.template load_k<0>(c, g, u0 + 2);
+  if constexpr (kSets == 2) st.template load_k<kOther>(c, g, u0 + 3);
+  st.template load_v<0>(c, g, u0);
   __syncthreads();
-  if (any) {
-    scores(sa, 0);
-    scores(sb, 1);
-    mask(0, sa, ks, ev);
+  scores(sa, 0);
+  scores(sb, 1);
+  mask(0, sa, ks, ev);
+  {
     float big[2] = {sa[0], sa[8]};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -437,52 +455,64 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < Stage::kParts; ++i) st.store_k(buf(0), i);
-  st.load_k(c, g, u0 + 3);
+  for (int i = 0; i < Stage::kParts; ++i) Stage::store_k(buf(0), st.k[0], i);
+  st.template load_k<0>(c, g, u0 + 2 + kSets);
+  if constexpr (kSets == 2) st.template load_v<kOther>(c, g, u0 + 1);
   // steps whose V holds infinities or NaN: the wave's first, one past its last
   int odd0 = 0x7FFFFFFF, odd1 = 0;
   // A step of the workgroup.  One barrier parts the writers and the readers of
   // K (read of j + 2, written of j + 3) and V (read of j - 1, written of j).
-  auto round = [&](int j, f32x16& s0, f32x16& s1, f32x16& s2) {
-    // (of steps j + 1 to j + 4 below)
-    if (u0 + j + 5 > st.base + 64) st.look_up(c, b, g, u0 + j);
+  auto round = [&](auto parity, int j, f32x16& s0, f32x16& s1, f32x16& s2) {
+    // the registers of V of j, and of K of j + 3
+    constexpr int VS = decltype(parity)::value % kSets, KS3 = (decltype(parity)::value + 1) % kSets;
+    // (of steps j + 1 to j + 5 below)
+    if (u0 + j + 6 > st.base + 64) st.look_up(c, b, g, u0 + j);
     __syncthreads();
     uint32_t found = 0;
     // K of j + 3 and V of j to LDS, K of j + 4 and V of j + 1 on their way
     // (steps past the last: what lies there of the last pages, not used)
     auto other = [&](int i) {
       constexpr int U = kOps / 8;
+      // (the compiler would decode before the barrier, and wait there)
+      auto here = [](typename Stage::Piece (&x)[Stage::KP]) {
+#pragma unroll
+        for (int p = 0; p < Stage::KP; ++p) asm volatile("" : "+v"(x[p]));
+      };
 #pragma unroll
       for (int part = 0; part < Stage::kParts; ++part) {
-        if (i == U * part) st.store_k(buf(j + 1), part);
-        if (i == U * (2 + part)) Stage::store_v(buf(j), st.v, part);
+        if (i == U * part) here(st.k[KS3]);
+        if (i == U * (2 + part)) here(st.v[VS]);
+        if (i == U * part) Stage::store_k(buf(j + 1), st.k[KS3], part);
+        if (i == U * (2 + part)) Stage::store_v(buf(j), st.v[VS], part);
       }
+      if (i == U * (Stage::kParts - 1)) st.template load_k<KS3>(c, g, u0 + j + 3 + kSets);
       if (i == 4 * U) {
 #pragma unroll
-        for (int p = 0; p < Stage::KP; ++p) found |= st.odd_in_v(p);
+        for (int p = 0; p < Stage::KP; ++p) found |= Stage::odd_in(st.v[VS][p]);
+        st.template load_v<VS>(c, g, u0 + j + kSets);
       }
-      if (i == 5 * U) st.load_k(c, g, u0 + j + 4);
     };
-    if (any) {
-      step(j, s0, s1, s2, other);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kOps; ++i) other(i);
-    }
+    step(j, s0, s1, s2, other);
     if (__builtin_amdgcn_ballot_w64((found & Stage::kOdd) != 0)) {
-      st.store_v_finite(buf(j));
+      st.template load_v<VS>(c, g, u0 + j);
+      Stage::store_v_finite(buf(j), st.v[VS]);
+      st.template load_v<VS>(c, g, u0 + j + kSets);
       odd0 = min(odd0, u0 + j);
       odd1 = u0 + j + 1;
     }
-    st.load_v(c, g, u0 + j + 1);
   };
-  for (int j = 0; j < n; j += 3) {
-    round(j, sa, sb, sc);
-    if (j + 1 < n) round(j + 1, sb, sc, sa);
-    if (j + 2 < n) round(j + 2, sc, sa, sb);
+  const std::integral_constant<int, 0> even;
+  const std::integral_constant<int, 1> uneven;
+  for (int j = 0; j < n; j += 6) {
+    round(even, j, sa, sb, sc);
+    if (j + 1 < n) round(uneven, j + 1, sb, sc, sa);
+    if (j + 2 < n) round(even, j + 2, sc, sa, sb);
+    if (j + 3 < n) round(uneven, j + 3, sa, sb, sc);
+    if (j + 4 < n) round(even, j + 4, sb, sc, sa);
+    if (j + 5 < n) round(uneven, j + 5, sc, sa, sb);
   }
   __syncthreads();
-  if (any && n > 0) {
+  if (n > 0) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -497,7 +527,7 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   __syncthreads();
   odd0 = min(min(odds[0][0], odds[0][1]), min(odds[0][2], odds[0][3]));
   odd1 = max(max(odds[1][0], odds[1][1]), max(odds[1][2], odds[1][3]));
-  if (any && odd0 < odd1)
+  if (odd0 < odd1)
     add_odd_values<D, FP8>(o, c, b, g, __builtin_amdgcn_readfirstlane(odd0),
                            __builtin_amdgcn_readfirstlane(odd1), r);
   l += __shfl_xor(l, 32);
@@ -552,7 +582,20 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   const int d4 = 4 * (threadIdx.x % (D / 4));
   const float* p = a.part + (((int64_t)slot0 * c.Hk + g) * a.splits * kPpRows + rw) * PS;
   Merge acc;
-  for (int s = 0; s < parts; ++s, p += kPpRows * PS) acc.add(p[D], p[D + 1], *(const f32x4*)(p + d4));
+  constexpr int F = 8;  // in flight
+  for (int s0 = 0; s0 < parts; s0 += F) {
+    float2 ml[F];
+    f32x4 o[F];
+#pragma unroll
+    for (int s = 0; s < F; ++s) {
+      const float* ps = p + (int64_t)min(s0 + s, parts - 1) * (kPpRows * PS);
+      ml[s] = *(const float2*)(ps + D);
+      o[s] = *(const f32x4*)(ps + d4);
+    }
+#pragma unroll
+    for (int s = 0; s < F; ++s)
+      if (s0 + s < parts) acc.add(ml[s].x, ml[s].y, o[s]);
+  }
   const int tok = r.row / a.rep;
   store_row(a.out + ((int64_t)(r.s0 + tok) * c.Hk * a.rep + g * a.rep + r.row % a.rep) * D + d4,
             acc.o, acc.den, r.first + tok, r.cap);
@@ -563,31 +606,40 @@ struct PromptShape {
   int splits, split_steps;
 };
 
-// Units of 128 rows, and the splits of the positions that fill the 512
-// workgroups the card holds of them: with few units, down to 16 steps a split;
-// with more, only to even out contexts of very different lengths.
+// Units of 128 rows, and the parts that a long context's steps are cut into.
+// The card holds 512 workgroups (two a CU), so up to 256 units take as many
+// parts as fill them, of 8 steps and an eighth of the units at least: below
+// that, the parts' way through memory and the second launch cost more.  Of
+// more units only contexts of 256 steps are split, to even out the last
+// workgroups.  Measured with 4 KV heads of 128 and 8 q heads each, us:
+//   128 units of 141 steps   67 (4 parts), 82 (8), 125 (one)
+//   128 units of 954         312 (4), 326 (8), 964 (one)
+//    32 units of 36          25 (4), 29 (2), 39 (one)
+//    32 units of 129         40 (16), 52 (4), 116 (2)
+//   252 units of up to 32    37 (one), 44 (two of the longest)
+//   208 units of 69          67 (2), 77 (4), 72 (one)
+//   1024 units of up to 128  194 (one), 231 (up to 8)
 PromptShape prompt_shape(bool ragged, int64_t seqs, int64_t tokens, int64_t rep, int64_t kv_heads) {
   PromptShape s;
   s.slots = ragged ? tokens * rep / kPpRows + seqs
                    : seqs * ((tokens / std::max<int64_t>(seqs, 1) * rep + kPpRows - 1) / kPpRows);
-  const int64_t units = std::max<int64_t>(s.slots * kv_heads, 1);
-  s.splits = (int)std::min<int64_t>(16, std::max<int64_t>(1, (units < 512 ? 1024 : 2048) / units));
-  s.split_steps = units < 512 ? 16 : 128;
+  // (of a ragged batch's slots, about half of those for last rows are there)
+  const int64_t n = std::max<int64_t>(s.slots * kv_heads, 1);
+  const int64_t units = std::max<int64_t>((s.slots - (ragged ? seqs / 2 : 0)) * kv_heads, 1);
+  const int64_t parts = std::min((units <= 256 ? 512 : kPpParts) / units, kPpParts / n);
+  s.splits = (int)std::min<int64_t>(16, std::max<int64_t>(1, parts));
+  s.split_steps = units <= 256 ? (int)std::max<int64_t>(8, units / 8) : 128;
   return s;
 }
 
 }  // namespace
 
+// At least what prompt_shape's parts take, for these sizes and smaller ones.
 int64_t paged_prompt_scratch_bytes(int64_t seqs, int64_t tokens, int64_t q_heads,
                                    int64_t kv_heads) {
-  // (either form of the batch; the wider head)
   const int64_t rep = (q_heads + kv_heads - 1) / kv_heads;
-  int64_t most = 0;
-  for (int ragged = 0; ragged < 2; ++ragged) {
-    if (!ragged && seqs > 0 && tokens % seqs) continue;
-    const PromptShape s = prompt_shape(ragged, seqs, tokens, rep, kv_heads);
-    if (s.splits > 1) most = std::max(most, s.slots * kv_heads * s.splits);
-  }
+  const int64_t n = (tokens * rep / kPpRows + seqs) * kv_heads;  // (more than without starts)
+  const int64_t most = n <= 256 ? std::min<int64_t>(16 * n, 1024) : kPpParts;
   return most * kPpRows * (128 + 4) * 4;
 }
 

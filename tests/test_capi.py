@@ -495,3 +495,17 @@ def test_paged_no_tokens(lib):
     assert _attend(lib, c, tokens=0, q=None, counters=None)[0] == 0
     assert lib.glq_paged_attention_counter_bytes(-1, 1, 1, 1) == -1
     assert lib.glq_paged_attention_scratch_bytes(1, 1, 1, 0) == -1
+
+
+def test_paged_workspace_serves_smaller_sizes():
+    lib = _lib.load()
+    for seqs, kv, rep in ((1, 4, 8), (8, 4, 8), (16, 16, 1), (64, 2, 20)):
+        last = [0, 0]
+        for tokens in [*range(1, 700, 7), *range(700, 40000, 633)]:
+            now = [lib.glq_paged_attention_counter_bytes(seqs, tokens, rep * kv, kv),
+                   lib.glq_paged_attention_scratch_bytes(seqs, tokens, rep * kv, kv)]
+            assert now[0] >= last[0] and now[1] >= last[1]
+            less = [lib.glq_paged_attention_counter_bytes(seqs - 1, tokens, rep * kv, kv),
+                    lib.glq_paged_attention_scratch_bytes(seqs - 1, tokens, rep * kv, kv)]
+            assert less[0] <= now[0] and less[1] <= now[1]
+            last = now
