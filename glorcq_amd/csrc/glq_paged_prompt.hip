@@ -42,12 +42,13 @@ constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running max
 // between two matrix ones; and the maximum of u + 1 and the way of K of u + 3
 // and V of u to LDS with them.  The bytes of two steps more are in flight.
 //
-// Bound by instructions: of a CU's 2700 cycles for two workgroups' steps, 1024
-// are matrix instructions', about as many LDS transfers' and 1300 vector ones'
-// (a step of a workgroup alone on its CU takes 1950, one wave's time to issue
-// it).  4096 tokens of 32 and 4 heads: 196 us, 700 TF/s of what the mask leaves;
-// 512 behind 30000: 314 us, 810 TF/s (a library product of 8192^3 reaches 1143,
-// these matrix instructions alone 1190).
+// Bound by instructions: of a CU's 2600 cycles for two workgroups' steps, 1024
+// are matrix instructions', about as many LDS transfers' and 1200 vector ones'
+// (a step of a workgroup alone on its CU takes 1800, one wave's time to issue
+// it).  4096 tokens of 32 and 4 heads: 177 to 194 us on different cards, 710 to
+// 780 TF/s of what the mask leaves; 512 behind 30000: 281 to 310 us, 820 to 900
+// TF/s (a library product of 8192^3 reaches 1143, these matrix instructions
+// alone 1190).
 //
 // Softmax: the running maximum m of t + e (e the exponent of V's block, as in
 // the first form) follows the scores only when one passes it by more than
@@ -71,54 +72,69 @@ struct PromptStage {
 
   // A wave's pieces of a pass lie in one block, K's and V's in the same, so
   // that addresses are scalars but for a lane's constant part.
+  static constexpr int NB = KP;  // blocks of a step that a wave fetches of
   __device__ int block(int j) const { return KP == 2 ? j : wave >> 1; }
 
-  // Pages and scales of the two blocks of 64 steps, a step a lane: a step finds
-  // its own in registers and waits for none.
+  // What a step needs to know of its two blocks, of 64 steps, a step a lane: a
+  // step finds its own in registers and waits for none.  at: places of the
+  // wave's blocks in the pools, in bytes; ks: scale of the scores; ev: exponent
+  // of V's scale.
   int base;
-  int page[2], ks[2], vs[2];
-  __device__ void look_up(const PagedView& c, int b, int g, int step) {
+  uint32_t at_lo[NB], at_hi[NB];
+  float ks[2], ev[2];
+  __device__ void look_up(const PagedView& c, int b, int g, float scale2, int step) {
     const int s = c.page_shift - 4;
     base = step;
+    int page[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int blk = 2 * (step + (int)(threadIdx.x & 63)) + k;
       const int p = c.table[b * c.table_stride + min(blk >> s, c.max_pages - 1)];
       const bool bad = (unsigned)p >= (unsigned)c.pages;  // page 0 is read, its scores are NaN
       page[k] = bad ? 0 : p;
-      ks[k] = vs[k] = 127;
+      ks[k] = scale2;
+      ev[k] = 0.f;
       if constexpr (FP8) {
         const int64_t at = place(c, g, page[k], blk);
-        ks[k] = c.ks[at];
-        vs[k] = c.vs[at];
+        ks[k] = e8m0_value(c.ks[at]) * scale2;
+        ev[k] = e8m0_exponent(c.vs[at]);
       }
-      if (bad) ks[k] = 255;
+      if (bad) ks[k] = __builtin_nanf("");
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) asm volatile("" : "+v"(ks[k]), "+v"(vs[k]));  // (waits for them)
+    for (int j = 0; j < NB; ++j) {
+      const int blk = 2 * (step + (int)(threadIdx.x & 63)) + block(j);
+      const int64_t at = place(c, g, block(j) ? page[1] : page[0], blk) * (16 * D * S);
+      at_lo[j] = (uint32_t)at;
+      at_hi[j] = (uint32_t)(at >> 32);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) asm volatile("" : "+v"(ks[k]), "+v"(ev[k]));  // (waits for them)
   }
   __device__ static int64_t place(const PagedView& c, int g, int p, int blk) {
     const int s = c.page_shift - 4;
     return ((int64_t)p * c.Hk + g << s) + (blk & ((1 << s) - 1));
   }
-  __device__ int64_t place_of(const PagedView& c, int g, int step, int j) const {
-    const int k = block(j);
-    return place(c, g, __builtin_amdgcn_readlane(k ? page[1] : page[0], step - base), 2 * step + k);
+  __device__ static float lane_value(float x, int lane) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
+  }
+  __device__ const char* block_of(const void* pool, int step, int j) const {
+    const uint32_t lo = __builtin_amdgcn_readlane(at_lo[j], step - base);
+    const uint32_t hi = __builtin_amdgcn_readlane(at_hi[j], step - base);
+    return (const char*)pool + ((uint64_t)hi << 32 | lo);
   }
   template <int SET>
-  __device__ void load_k(const PagedView& c, int g, int step) {
+  __device__ void load_k(const PagedView& c, int step) {
     // (a pass's rows are a block's, or start at a block)
     const unsigned lane = (threadIdx.x / KC & 15) * (D * S) + PB * (threadIdx.x % KC);
 #pragma unroll
-    for (int j = 0; j < KP; ++j)
-      k[SET][j] = *(const Piece*)((const char*)c.k + place_of(c, g, step, j) * (16 * D * S) + lane);
+    for (int j = 0; j < KP; ++j) k[SET][j] = *(const Piece*)(block_of(c.k, step, j) + lane);
   }
   template <int SET>
-  __device__ void load_v(const PagedView& c, int g, int step) {
+  __device__ void load_v(const PagedView& c, int step) {
     const unsigned lane = threadIdx.x % VC * PB;
 #pragma unroll
-    for (int j = 0; j < KP; ++j)
-      v[SET][j] = *(const Piece*)((const char*)c.v + place_of(c, g, step, j) * (16 * D * S) + lane);
+    for (int j = 0; j < KP; ++j) v[SET][j] = *(const Piece*)(block_of(c.v, step, j) + lane);
   }
 
   // LDS places in halves.  K: values 8 d8 .. + 8 of a position at (d8,
@@ -323,8 +339,8 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   auto mask = [&](int j, f32x16& s, float (&ks)[2], float (&ev)[2]) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      ks[k] = e8m0_value(__builtin_amdgcn_readlane(st.ks[k], u0 + j - st.base)) * scale2;
-      ev[k] = e8m0_exponent(__builtin_amdgcn_readlane(st.vs[k], u0 + j - st.base));
+      ks[k] = Stage::lane_value(st.ks[k], u0 + j - st.base);
+      ev[k] = Stage::lane_value(st.ev[k], u0 + j - st.base);
     }
     const int p0 = (u0 + j) * kPpStep;
     if (p0 < r.lo_all || p0 + kPpStep > r.hi_all) {
@@ -386,6 +402,8 @@ void paged_prompt_kernel(PagedAttnArgs a) {
     f16x8 wn[2];
     float sum[2] = {0.f, 0.f}, big[2] = {s1[0], s1[8]};
     s2 = f32x16{};
+    float last = 0.f;
+    int late = 0;
 #pragma unroll
     for (int i = 0; i < kOps; ++i) {
       if (i & 1)
@@ -399,7 +417,9 @@ void paged_prompt_kernel(PagedAttnArgs a) {
         const int k = e >> 3;
         float x = __builtin_amdgcn_exp2f(fmaf(s0[e], ks[k], off[k]));
         asm volatile("" : "+v"(x));  // (in this place)
-        sum[k] += x;
+        sum[late >> 3] += last;      // (of the one before: x takes a while)
+        last = x;
+        late = e;
         wn[k][e & 7] = (_Float16)x;
         if (e & 1) {
           big[k] = fmaxf(fmaxf(big[k], s1[e - 1]), s1[e]);
@@ -408,6 +428,7 @@ void paged_prompt_kernel(PagedAttnArgs a) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    sum[1] += last;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       l = FP8 ? fmaf(sum[k], __builtin_amdgcn_exp2f(-ev[k]), l) : l + sum[k];
@@ -425,11 +446,11 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   // looks for the V of the one before it.  Steps past the last are not fetched:
   // their scores, of what LDS held before, are not used.
   constexpr int kSets = Stage::kSets, kOther = kSets - 1;
-  st.look_up(c, b, g, u0);
+  st.look_up(c, b, g, scale2, u0);
   {
     Stage s2 = st;
-    st.template load_k<0>(c, g, u0);
-    s2.template load_k<0>(c, g, u0 + 1);
+    st.template load_k<0>(c, u0);
+    s2.template load_k<0>(c, u0 + 1);
 #pragma unroll
     for (int i = 0; i < Stage::kParts; ++i) {
       Stage::store_k(buf(0), st.k[0], i);
@@ -438,9 +459,9 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   }
   for (int i = tid; i < 4 * D; i += kPpThreads)
     *(u32x4*)(buf(1) + Stage::kV + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-  st.template load_k<0>(c, g, u0 + 2);
-  if constexpr (kSets == 2) st.template load_k<kOther>(c, g, u0 + 3);
-  st.template load_v<0>(c, g, u0);
+  st.template load_k<0>(c, u0 + 2);
+  if constexpr (kSets == 2) st.template load_k<kOther>(c, u0 + 3);
+  st.template load_v<0>(c, u0);
   __syncthreads();
   scores(sa, 0);
   scores(sb, 1);
@@ -456,8 +477,8 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < Stage::kParts; ++i) Stage::store_k(buf(0), st.k[0], i);
-  st.template load_k<0>(c, g, u0 + 2 + kSets);
-  if constexpr (kSets == 2) st.template load_v<kOther>(c, g, u0 + 1);
+  st.template load_k<0>(c, u0 + 2 + kSets);
+  if constexpr (kSets == 2) st.template load_v<kOther>(c, u0 + 1);
   // steps whose V holds infinities or NaN: the wave's first, one past its last
   int odd0 = 0x7FFFFFFF, odd1 = 0;
   // A step of the workgroup.  One barrier parts the writers and the readers of
@@ -466,7 +487,7 @@ void paged_prompt_kernel(PagedAttnArgs a) {
     // the registers of V of j, and of K of j + 3
     constexpr int VS = decltype(parity)::value % kSets, KS3 = (decltype(parity)::value + 1) % kSets;
     // (of steps j + 1 to j + 5 below)
-    if (u0 + j + 6 > st.base + 64) st.look_up(c, b, g, u0 + j);
+    if (u0 + j + 6 > st.base + 64) st.look_up(c, b, g, scale2, u0 + j);
     __syncthreads();
     uint32_t found = 0;
     // K of j + 3 and V of j to LDS, K of j + 4 and V of j + 1 on their way
@@ -485,18 +506,18 @@ void paged_prompt_kernel(PagedAttnArgs a) {
         if (i == U * part) Stage::store_k(buf(j + 1), st.k[KS3], part);
         if (i == U * (2 + part)) Stage::store_v(buf(j), st.v[VS], part);
       }
-      if (i == U * (Stage::kParts - 1)) st.template load_k<KS3>(c, g, u0 + j + 3 + kSets);
+      if (i == U * (Stage::kParts - 1)) st.template load_k<KS3>(c, u0 + j + 3 + kSets);
       if (i == 4 * U) {
 #pragma unroll
         for (int p = 0; p < Stage::KP; ++p) found |= Stage::odd_in(st.v[VS][p]);
-        st.template load_v<VS>(c, g, u0 + j + kSets);
+        st.template load_v<VS>(c, u0 + j + kSets);
       }
     };
     step(j, s0, s1, s2, other);
     if (__builtin_amdgcn_ballot_w64((found & Stage::kOdd) != 0)) {
-      st.template load_v<VS>(c, g, u0 + j);
+      st.template load_v<VS>(c, u0 + j);
       Stage::store_v_finite(buf(j), st.v[VS]);
-      st.template load_v<VS>(c, g, u0 + j + kSets);
+      st.template load_v<VS>(c, u0 + j + kSets);
       odd0 = min(odd0, u0 + j);
       odd1 = u0 + j + 1;
     }
