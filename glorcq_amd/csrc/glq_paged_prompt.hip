@@ -402,6 +402,8 @@ void paged_prompt_kernel(PagedAttnArgs a) {
     f16x8 wn[2];
     float sum[2] = {0.f, 0.f}, big[2] = {s1[0], s1[8]};
     s2 = f32x16{};
+    // (the CU's other workgroup gets its turn between steps, not within: 5 %)
+    __builtin_amdgcn_s_setprio(1);
     float last = 0.f;
     int late = 0;
 #pragma unroll
@@ -428,6 +430,7 @@ void paged_prompt_kernel(PagedAttnArgs a) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     sum[1] += last;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
