@@ -374,6 +374,12 @@ extern "C" int glq_paged_append(const glq_paged_append_params* p, void* stream) 
               "q_item_rows must be 0 or a multiple of head_dim dividing q_heads * head_dim");
     GLQ_CHECK(q_item_rows > 0 || (q_stride >= q_heads * D && q_stride % 8 == 0),
               "q's row stride must cover the heads and be a multiple of 8");
+    const int64_t row = q_heads * D;
+    const bool own = q_item_rows == 0 && (q_stride == row || tokens == 1);
+    GLQ_CHECK((q == q_out && own) ||
+                  apart(q, ((tokens - 1) * (q_item_rows > 0 ? row : q_stride) + row) * 2, q_out,
+                        tokens * row * 2),
+              "q_out must not overlap q (but for rows side by side, rotated in place)");
   }
   a.q = (const __half*)q; a.k = (const __half*)k; a.v = (const __half*)v;
   a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;

@@ -598,6 +598,8 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
             "workspace of %lld (counters) and %lld bytes (scratch, 256-byte aligned) needed "
             "(got %lld, %lld)", (long long)cnt, (long long)scr, (long long)p->counter_bytes,
             (long long)p->scratch_bytes);
+  GLQ_CHECK(apart(q, tokens * q_heads * D * 2, out, tokens * q_heads * D * 2),
+            "out must not overlap q");
   a.q = (const __half*)q;
   a.out = (__half*)out;
   a.rep = (int)(q_heads / Hk);

@@ -177,7 +177,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     not) and rotated (cos/sin (T or 1, D), None: not) and rounded once to the
     pages' type; with q (T, Hq*D) -- or item-major (n, T, R), a batched GEMV's
     output over R-row slices -- its heads likewise, returned as q_out (T, Hq, D)
-    fp16 (else None).  Rows of k, v and q may be slices of a wider matrix.
+    fp16 (else None; q itself where its rows lie side by side).  Rows of k, v
+    and q may be slices of a wider matrix.
     8-bit pages: a block's scale is the smallest power of two that takes its
     values to e4m3's 448; tokens that a block already had are scaled along when
     it grows.  Infinities and NaN are stored as NaN.  Pages that get tokens must
@@ -278,7 +279,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Causal attention of the new tokens' q (T, Hq, D) fp16 (paged_append's
     result) over their sequences' pages -> (T, Hq*D) fp16 (glq_paged_attention).
     The token at position p attends to (p - window, p], or [0, p] with window
-    0.  `out`: rows behind starts[B] keep what they held.  `workspace`: from
+    0.  `out` (apart from q): rows behind starts[B] keep what they held.  `workspace`: from
     paged_attention_workspace; None takes one of the stream's, or under graph
     capture one of the call's own, so that graphs may be replayed on several
     streams."""

@@ -784,7 +784,9 @@ typedef struct glq_paged_cache {
  * NaN are stored as NaN.  What lies behind a sequence's last token in its block
  * becomes zero.  Rows of k, v and q are k_stride, v_stride and q_stride values
  * apart (multiples of 8); with q_item_rows > 0, q is item-major as in
- * glq_qk_norm_rope.  Pages that get tokens must belong to one sequence.
+ * glq_qk_norm_rope.  q_out may be q itself where q's rows lie side by side, and
+ * must not overlap it otherwise.  Pages that get tokens must belong to one
+ * sequence.
  */
 typedef struct glq_paged_append_params {
   glq_paged_cache cache;
@@ -810,7 +812,9 @@ int glq_paged_append(const glq_paged_append_params* p, void* stream);
  *   out[t][h*D + d] = fp16(sum_p softmax_p(scale * q.k_p) v_p[d]),
  * KV head h / (q_heads / kv_heads), fp32 scores, softmax and sums.  A row
  * without positions (p < 0) is 0; one past the page table NaN.  q (tokens,
- * q_heads, head_dim) fp16, out (tokens, q_heads * head_dim).  workspace: the
+ * q_heads, head_dim) fp16, out (tokens, q_heads * head_dim) apart from it.  The
+ * workspace's sizes never shrink with seqs or tokens; a workspace serves smaller
+ * calls too: the
  * counters (glq_paged_attention_counter_bytes) are zero before their first use
  * and left zero by each call; the scratch (.._scratch_bytes, 256-byte aligned)
  * needs no initialisation (both negative for invalid sizes).  Calls that share

@@ -470,6 +470,9 @@ def test_paged_cache_checks(lib, kw, what):
     (dict(q=P, q_heads=4, q_stride=256, q_out=P), b"row stride"),
     (dict(q=P, q_heads=4, q_item_rows=96, q_out=P), b"q_item_rows"),
     (dict(tokens=1 << 25), b"tokens"), (dict(tokens=3), b"same number"),
+    (dict(q=P, q_heads=4, q_stride=1024, q_out=P), b"overlap"),
+    (dict(q=P, q_heads=4, q_stride=512, q_out=P + 512), b"overlap"),
+    (dict(q=P, q_heads=4, q_item_rows=256, q_out=P), b"overlap"),
 ])
 def test_paged_append_checks(lib, kw, what):
     rc, msg = _append(lib, **kw)
@@ -480,7 +483,7 @@ def test_paged_append_checks(lib, kw, what):
     (dict(q_heads=7), b"q_heads"), (dict(window=-1), b"window"), (dict(out=None), b"null"),
     (dict(q=P + 2), b"aligned"), (dict(counters=None), b"workspace"),
     (dict(counter_bytes=10), b"workspace"), (dict(scratch_bytes=10), b"workspace"),
-    (dict(scratch=P + 64), b"workspace"),
+    (dict(scratch=P + 64), b"workspace"), (dict(out=P), b"overlap"), (dict(out=P + 256), b"overlap"),
 ])
 def test_paged_attention_checks(lib, kw, what):
     rc, msg = _attend(lib, **kw)

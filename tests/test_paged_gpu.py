@@ -627,6 +627,61 @@ def test_other_stream_and_views(gpu):
     assert torch.equal(y, ref)
 
 
+def test_graphs_at_once(gpu):
+    """Captured calls have workspaces of their own: three graphs replayed on
+    streams of their own at once, with eager calls beside them, give the eager
+    results every time."""
+    c = Cache(gpu, 2, 2, 128, 32, FP8, 5100, 34)
+    c.fill([5000, 4000])
+    s, kp, vp = c.pages()
+    calls = []
+    for n in (1, 3, 40):  # merged over workgroups; more rows; a split prompt
+        q = torch.randn(2 * n, 8, 128, generator=c.g).half().to(gpu)
+        calls.append(lambda q=q: kernels.paged_attention(q, kp, vp, c.table, c.lengths, 0.1, **s))
+    want = [f().clone() for f in calls]
+    graphs = []
+    for f in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = f()
+        graphs.append((g, y, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for _, y, _ in graphs:
+            y.zero_()
+        torch.cuda.synchronize()
+        for g, _, st in graphs:
+            with torch.cuda.stream(st):
+                g.replay()
+        eager = [f() for f in calls]
+        torch.cuda.synchronize()
+        for (_, y, _), e, w in zip(graphs, eager, want):
+            assert torch.equal(y, w) and torch.equal(e, w)
+    # a workspace made for more tokens and sequences serves these calls
+    ws = kernels.paged_attention_workspace(torch.empty(3000, 8, 128, dtype=FP16, device=gpu), kp,
+                                           torch.empty(70, 160, dtype=torch.int32, device=gpu))
+    for n, w in zip((1, 3, 40), want):
+        q = calls[(1, 3, 40).index(n)].__defaults__[0]
+        y = kernels.paged_attention(q, kp, vp, c.table, c.lengths, 0.1, workspace=ws, **s)
+        assert torch.equal(y, w)
+
+
+def test_append_q_in_place(gpu):
+    """q_out may be q where its rows lie side by side."""
+    c = Cache(gpu, 2, 2, 64, 16, FP16, 64, 35)
+    c.lengths.fill_(20)
+    k = torch.randn(40, 128, generator=c.g).half().to(gpu)
+    q = torch.randn(40, 4, 64, generator=c.g).half().to(gpu)
+    cos, sin = (x.to(gpu) for x in rope_rows(torch.arange(40), 64))
+    s, kp, vp = c.pages()
+    args = (k, k, kp, vp, c.table, c.lengths)
+    want = kernels.paged_append(*args, cos=cos, sin=sin, q=q, **s)
+    got = kernels.paged_append(*args, cos=cos, sin=sin, q=q, q_out=q, **s)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got.view(want.shape), want)
+    with pytest.raises(RuntimeError, match="overlap"):
+        kernels.paged_attention(q, kp, vp, c.table, c.lengths, 1.0, out=q.view(40, 256), **s)
+
+
 def test_refusals(gpu):
     c = Cache(gpu, 2, 2, 64, 16, FP8, 64, 34)
     s, kp, vp = c.pages()
