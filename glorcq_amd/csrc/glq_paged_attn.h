@@ -11,10 +11,11 @@ constexpr int kPaRows = 16;      // query rows (tokens x the KV head's q heads) 
 constexpr int kPpRows = 128;     // of the second form's
 // A sequence with more rows a KV head takes the second form.  The first one
 // reads a sequence's pages once for each 16 rows; the second once for 128, but
-// computes as if it had them all.  8 sequences of 4000 positions, 8-bit pages,
-// 4 KV heads, us of the first | second form: 32 rows 25 | 31, 64 rows 29 | 35,
-// 128 rows 40 | 40; of 3000 positions and 16 KV heads: 28 | 61, 43 | 64, 137 | 80.
-constexpr int kPaMostRows = 64;
+// computes as if it had them all.  us of the first | second form, 8-bit pages,
+// with 32, 64 and 128 rows: 8 sequences of 4000 positions and 4 KV heads 25 |
+// 24, 30 | 27, 41 | 32; 64 of 1000 29 | 32, 49 | 34, 73 | 37; 8 of 3000 and 16
+// KV heads 28 | 42, 44 | 45, 134 | 53.
+constexpr int kPaMostRows = 32;
 
 struct PagedAttnArgs {
   PagedView c;

@@ -45,8 +45,8 @@ constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running max
 // Bound by instructions: of a CU's 2600 cycles for two workgroups' steps, 1024
 // are matrix instructions', about as many LDS transfers' and 1200 vector ones'
 // (a step of a workgroup alone on its CU takes 1800, one wave's time to issue
-// it).  4096 tokens of 32 and 4 heads: 177 to 194 us on different cards, 710 to
-// 780 TF/s of what the mask leaves; 512 behind 30000: 281 to 310 us, 820 to 900
+// it).  4096 tokens of 32 and 4 heads: 161 to 187 us on different cards, 735 to
+// 855 TF/s of what the mask leaves; 512 behind 30000: 278 to 300 us, 850 to 910
 // TF/s (a library product of 8192^3 reaches 1143, these matrix instructions
 // alone 1190).
 //
@@ -636,13 +636,13 @@ struct PromptShape {
 // that, the parts' way through memory and the second launch cost more.  Of
 // more units only contexts of 256 steps are split, to even out the last
 // workgroups.  Measured with 4 KV heads of 128 and 8 q heads each, us:
-//   128 units of 141 steps   67 (4 parts), 82 (8), 125 (one)
-//   128 units of 954         312 (4), 326 (8), 964 (one)
-//    32 units of 36          25 (4), 29 (2), 39 (one)
-//    32 units of 129         40 (16), 52 (4), 116 (2)
-//   252 units of up to 32    37 (one), 44 (two of the longest)
-//   208 units of 69          67 (2), 77 (4), 72 (one)
-//   1024 units of up to 128  194 (one), 231 (up to 8)
+//   128 units of 141 steps   67 (4 parts), 76 (2), 113 (one)
+//   128 units of 954         302 (4), 376 (2), 672 (one)
+//    32 units of 36          24 (4), 27 (2), 35 (one)
+//    32 units of 129         39 (16), 36 (8), 99 (one)
+//   252 units of up to 32    34 (one), 40 (two of the longest)
+//   288 units of up to 32    37 (one), 45 (two of the longest)
+//   1024 units of up to 128  188 (one), 235 (two of the longest)
 PromptShape prompt_shape(bool ragged, int64_t seqs, int64_t tokens, int64_t rep, int64_t kv_heads) {
   PromptShape s;
   s.slots = ragged ? tokens * rep / kPpRows + seqs
@@ -677,6 +677,9 @@ int paged_prompt_launch(PagedAttnArgs a, int head_dim, hipStream_t stream) {
   const int64_t steps = (((int64_t)a.c.max_pages << a.c.page_shift) + kPpStep - 1) / kPpStep;
   if (steps < 2 * s.split_steps) a.splits = 1;
   const int64_t grid = s.slots * a.c.Hk * a.splits;
+  GLQ_CHECK(a.splits == 1 || grid * kPpRows * (head_dim + 4) * 4 <=
+                                 paged_prompt_scratch_bytes(a.c.B, a.c.T, a.rep * a.c.Hk, a.c.Hk),
+            "paged prompt parts do not fit their scratch");
   GLQ_CHECK(s.slots * 16 < (1ll << 24) && grid < (1ll << 24), "batch of too many query rows");
   const bool fp8 = a.c.ks != nullptr, wide = head_dim == 128;
   auto kern = wide ? (fp8 ? paged_prompt_kernel<128, true> : paged_prompt_kernel<128, false>)

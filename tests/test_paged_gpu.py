@@ -314,6 +314,9 @@ def test_attention_split(gpu, dtype, D, page, Hq, Hk, news, past, window):
 
 @pytest.mark.parametrize("dtype", [FP8, FP16])
 @pytest.mark.parametrize("D,page,Hq,Hk,news,past,window", [
+    (128, 64, 8, 1, [4, 4], [70, 1000], 0),        # 32 rows a sequence
+    (128, 64, 8, 1, [5, 5], [70, 1000], 0),        # 40
+    (64, 16, 4, 2, [16, 17, 1], [40, 700, 90], 0),  # 32, 34 and 2 in a batch
     (128, 64, 8, 1, [8, 8], [70, 1000], 0),        # 64 rows a sequence
     (128, 64, 8, 1, [9, 9], [70, 1000], 0),        # 72
     (64, 16, 4, 2, [32, 33, 1], [40, 700, 90], 0),  # 64, 66 and 2 in a batch
