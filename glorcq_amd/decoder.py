@@ -173,6 +173,8 @@ class GLoRCQQwen3Attention(nn.Module):
         B, S, H = hidden_states.shape
         inner, T, hd = self.inner, B * S, self.head_dim
         q, k, v = self._project(hidden_states.reshape(T, H), qkv_xu)
+        if q.dim() == 3 and q.shape[2] == hd:  # items of a head (one KV head): (T, Hq, D)
+            q = q.transpose(0, 1).contiguous()
         cos, sin = (t.reshape(-1, hd).contiguous() for t in position_embeddings)
         kp, vp, ks, vs = step.cache.layers[self.layer_idx]
         at = dict(page_table=step.page_table, lengths=step.lengths, starts=step.starts,

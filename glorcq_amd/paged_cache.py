@@ -119,8 +119,11 @@ class PagedKVCache:
 
     def workspace(self, q: torch.Tensor):
         """The attention workspace of steps of q's shape, one for all layers:
-        steps of one cache run in order."""
+        steps of one cache run in order.  None for the first one under graph
+        capture (its zeros would be written by replays alone)."""
         ws = self._workspaces.get(q.shape)
+        if ws is None and torch.cuda.is_current_stream_capturing():
+            return None
         if ws is None:
             ws = self._workspaces[q.shape] = kernels.paged_attention_workspace(
                 q, self.layers[0][0], self.page_table)

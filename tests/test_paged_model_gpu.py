@@ -11,8 +11,9 @@ are given back and used again."""
 import pytest
 import torch
 
+from glorcq_amd import kernels
 from glorcq_amd.graph_wrapper import _static_cache
-from glorcq_amd.paged_cache import GLoRCQPagedWrapper, PagedStep, paged_forward
+from glorcq_amd.paged_cache import GLoRCQPagedWrapper, PagedKVCache, PagedStep, paged_forward
 from glorcq_amd.synthetic_model import build_qwen3_moe, qwen3_moe_config
 
 pytestmark = pytest.mark.gpu
@@ -124,3 +125,54 @@ def test_continued_prompts_and_room(gpu):
     assert [len(o) for o in out] == [97, 27]
     with pytest.raises(RuntimeError, match="max_seq_len"):
         w.replay(torch.zeros(2, dtype=torch.long, device=gpu))
+
+
+@pytest.mark.parametrize("batch", [3, 4])
+@torch.no_grad()
+def test_one_kv_head(gpu, batch):
+    """A model of 4 query heads and one KV head: the batched projections' items
+    are heads, as many of them as sequences for a batch of 4."""
+    cfg = qwen3_moe_config(num_hidden_layers=1, vocab_size=VOCAB, max_position_embeddings=512)
+    cfg.num_attention_heads, cfg.num_key_value_heads = 4, 1
+    model = build_qwen3_moe(cfg, gpu, seed=1)[0]
+    prompts = _prompts([9, 40, 3, 17][:batch], gpu)
+    g = torch.Generator().manual_seed(8)
+    cont = torch.randint(0, VOCAB, (3, batch), generator=g).to(gpu)
+    w = GLoRCQPagedWrapper(model, max_batch_size=batch, max_seq_len=64, page_size=16,
+                           cache_dtype=torch.float16)
+    w.capture_graph()
+    got = [w.prefill(prompts).clone()] + [w.replay(t).clone() for t in cont]
+    torch.cuda.synchronize()
+    got = torch.stack(got).float()
+    for b, p in enumerate(prompts):
+        ref = _static_logits(model, p, cont[:, b], gpu)
+        err = float((got[:, b] - ref).abs().max())
+        assert err <= 0.02 * float(ref.abs().max()), (b, err)
+
+
+@torch.no_grad()
+def test_capture_before_any_step(gpu):
+    """A step captured before an eager one of its shape: the eager one's
+    workspace is zeroed all the same."""
+    cache = PagedKVCache(1, 1, 64, 2, 5000, page_size=16, dtype=torch.float16, device=gpu)
+    cache.extend(4800)
+    kp, vp, _, _ = cache.layers[0]
+    g = torch.Generator().manual_seed(4)
+    for x in (kp, vp):
+        x.copy_(torch.randn(x.shape, generator=g))
+    q = torch.randn(2, 4, 64, generator=g).half().to(gpu)
+    step = PagedStep(cache)
+
+    def run():
+        return kernels.paged_attention(q, kp, vp, step.page_table, step.lengths, 0.1,
+                                       workspace=step.workspace(q))
+
+    want = kernels.paged_attention(q, kp, vp, step.page_table, step.lengths, 0.1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run()
+    for _ in range(2):
+        assert torch.equal(run(), want)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
