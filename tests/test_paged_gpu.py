@@ -669,6 +669,53 @@ def test_graphs_at_once(gpu):
         assert torch.equal(y, w)
 
 
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+def test_captured_ragged_batch(gpu, dtype):
+    """One captured step of 200 rows replayed for batches that divide them
+    otherwise, padded ones among them: pages and results are the eager ones,
+    rows behind the last sequence keep what they held."""
+    B, T, Hq, Hk, D, page = 4, 200, 8, 2, 64, 32
+    c = Cache(gpu, B, Hk, D, page, dtype, 700, 36)
+    c.fill([300, 0, 17, 64])
+    gen = torch.Generator().manual_seed(37)
+    mine = [None if x is None else x.clone() for x in c.t]  # the graph's pages
+    st = torch.zeros(B + 1, dtype=torch.int32, device=gpu)
+    x = torch.zeros(T, (Hq + 2 * Hk) * D, dtype=torch.float16, device=gpu)
+    cos, sin = (t.to(gpu) for t in rope_rows(torch.arange(T), D))
+    outs = [torch.zeros(T, Hq * D, dtype=torch.float16, device=gpu) for _ in range(4)]
+
+    def step(t, qo, out):
+        q, k, v = x.split([Hq * D, Hk * D, Hk * D], 1)
+        s = dict(starts=st, k_scales=t[2], v_scales=t[3])
+        q = kernels.paged_append(k, v, t[0], t[1], c.table, c.lengths, cos=cos, sin=sin, q=q,
+                                 q_out=qo, **s)
+        kernels.paged_attention(qo.view(T, Hq, D), t[0], t[1], c.table, c.lengths, 0.1, out=out,
+                                window=250, **s)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(mine, outs[0], outs[1])
+    lens = [300, 0, 17, 64]
+    for news in ([0, 0, 0, 0], [1, 1, 1, 1], [150, 1, 9, 0], [0, 0, 0, 200], [40, 70, 3, 50],
+                 [1, 0, 1, 7]):
+        lens = [a + n for a, n in zip(lens, news)]
+        st.copy_(torch.tensor([0] + news).cumsum(0))
+        c.lengths.copy_(torch.tensor(lens))
+        x.copy_(torch.randn(x.shape, generator=gen))
+        for o in outs:
+            o.fill_(7.0)
+        graph.replay()
+        step(c.t, outs[2], outs[3])
+        torch.cuda.synchronize()
+        n = sum(news)
+        for o in outs:
+            assert (o[n:] == 7.0).all() and not (n and (o[:n] == 7.0).all())
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+        assert outs[1].isfinite().all()
+        for a, b in zip(mine, c.t):
+            assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_append_q_in_place(gpu):
     """q_out may be q where its rows lie side by side."""
     c = Cache(gpu, 2, 2, 64, 16, FP16, 64, 35)
