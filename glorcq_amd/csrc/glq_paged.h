@@ -91,13 +91,13 @@ __device__ __forceinline__ void paged_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Checks a cache and its batch and fills the kernels' view of them (the pages
-// themselves may be null in a batch of no tokens).
 // Whether two ranges of bytes have none in common.
 inline bool apart(const void* a, int64_t an, const void* b, int64_t bn) {
   return (uintptr_t)a + an <= (uintptr_t)b || (uintptr_t)b + bn <= (uintptr_t)a;
 }
 
+// Checks a cache and its batch and fills the kernels' view of them (the pages
+// themselves may be null in a batch of no tokens).
 int paged_view(const glq_paged_cache* c, const int32_t* starts, int64_t tokens, PagedView& view);
 
 }  // namespace glq

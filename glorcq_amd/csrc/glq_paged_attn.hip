@@ -609,17 +609,19 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
   a.count = (unsigned*)p->counters;
   const int64_t rows_each = (int64_t)a.c.each * a.rep;
   GLQ_CHECK(tokens * a.rep < (1ll << 30), "batch of too many (token, head) rows");
+  // (the first form counts its tiles in 32 bits)
+  const int64_t most = (cache->max_pages * cache->page_size + 31) / 32 + 1;
+  GLQ_CHECK((!starts && rows_each > kPaMostRows) ||
+                std::min(tokens * a.rep / kPaRows + cache->seqs,
+                         cache->seqs * ((kPaMostRows + kPaRows - 1) / kPaRows)) * Hk <=
+                    (1ll << 31) / most - 1,
+            "a batch of too many rows for its page table's length");
   // Many rows take the second form, a sequence at a time; where lengths are the
   // device's, both are launched, each passing over the other's sequences.
   if (starts ? tokens * a.rep > kPaMostRows : rows_each > kPaMostRows) {
     if (int rc = paged_prompt_launch(a, (int)D, (hipStream_t)stream)) return rc;
     if (!starts) return GLQ_OK;
   }
-  const int64_t most = (cache->max_pages * cache->page_size + 31) / 32 + 1;
-  GLQ_CHECK(std::min(tokens * a.rep / kPaRows + cache->seqs,
-                     cache->seqs * ((kPaMostRows + kPaRows - 1) / kPaRows)) * Hk <=
-                (1ll << 31) / most - 1,
-            "a batch of too many rows for its page table's length");
   a.slots_each = (int)((rows_each + kPaRows - 1) / kPaRows);
   // (rows of the pieces' places in LDS: of 8, two threads merge a value's parts;
   // a sequence of 60000 positions 30 us, 37 with 16; 64 of 3000 46 and 45)
