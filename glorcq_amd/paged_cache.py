@@ -217,9 +217,9 @@ class GLoRCQPagedWrapper:
     def prefill(self, prompts):
         """The prompts' forward into an empty cache -> the logits after each
         one's last token (batch, vocab)."""
-        lens = [int(p.shape[0]) for p in prompts]
+        lens = [int(p.shape[0]) if p.dim() == 1 else 0 for p in prompts]
         if len(prompts) != self.max_batch_size or min(lens) < 1:
-            raise RuntimeError(f"{self.max_batch_size} prompts of at least one token needed")
+            raise RuntimeError(f"{self.max_batch_size} 1-D prompts of at least one token needed")
         self.cache.reset()
         self.cache.extend(lens)
         starts = torch.tensor([0] + lens).cumsum(0)
@@ -232,6 +232,10 @@ class GLoRCQPagedWrapper:
     def replay(self, input_ids):
         """One decode step: (batch,) ids, the sequences' next tokens -> the
         captured logits buffer (batch, vocab)."""
+        if self.graph is None:
+            raise RuntimeError("no captured step (capture_graph, which empties the cache)")
+        if input_ids.shape != self.static_input_ids.shape:
+            raise RuntimeError(f"input_ids must be ({self.max_batch_size},)")
         self.static_input_ids.copy_(input_ids)
         self.cache.extend(1)
         self.graph.replay()

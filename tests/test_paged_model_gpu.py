@@ -176,3 +176,19 @@ def test_capture_before_any_step(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+def test_wrapper_refusals(gpu):
+    w = GLoRCQPagedWrapper(_model(gpu), max_batch_size=2, max_seq_len=32, page_size=16)
+    a, b = _prompts((4, 5), gpu)
+    for what, call in (
+            ("no captured step", lambda: w.replay(a[:2])),
+            ("2 1-D prompts", lambda: w.prefill([a])),
+            ("2 1-D prompts", lambda: w.prefill([a, b[:0]])),
+            ("2 1-D prompts", lambda: w.prefill([a[None], b])),
+            ("max_seq_len", lambda: w.prefill([a, b.repeat(10)]))):
+        with pytest.raises(RuntimeError, match=what):
+            call()
+    w.capture_graph()
+    with pytest.raises(RuntimeError, match="input_ids must be"):
+        w.replay(a[:1])
