@@ -24,7 +24,7 @@ struct PagedAttnArgs {
   float* part;      // parts of units: o, m, l of a row in D + 4
   unsigned* count;  // [unit], zero between calls (first form)
   int rep, window, slots_each, rows;
-  int slots, splits, split_steps;  // second form
+  int slots, splits, split_steps, fold;  // second form
   float scale2;                    // scale log2(e)
 };
 

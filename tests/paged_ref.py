@@ -98,7 +98,12 @@ def attend(q, k, v, ev, first, scale, window, fp8):
       score: D products summed, 2 D u sum |q k| scale; scale and exponent
              products, sums and exp2: 8 u (|t| + 32 + 1)
       p is rounded to fp16 (2^-11) against the largest weight 2^M of a block's
-      share: 2^-25 absolute where it is subnormal
+      share: 2^-25 absolute where it is subnormal.  With more than 32 rows a
+      KV head the kernel's maximum m is a whole power of two that has followed
+      the scores: m < M + 1 (ceil), so 2^-25 2^m <= 2 2^-25 2^M; and a weight
+      still to be used when m follows is scaled by the power of two and rounded
+      a second time, the first error then no larger than before in units of
+      2^m: two of them, 4 2^-25 2^M at most
       sums over L positions: 2 L u
     """
     n, Hq, D = q.shape
@@ -129,7 +134,7 @@ def attend(q, k, v, ev, first, scale, window, fp8):
             M = (t2 + e).amax(-1, keepdim=True)
             total = torch.exp2(t2 - M).sum(-1, keepdim=True)
             codes = (vv * torch.exp2(-e)[:, None]).abs().sum(0)
-            sub = 2.0 ** -25 * codes / total
+            sub = (4 if n * rep > 32 else 1) * 2.0 ** -25 * codes / total
             tol[i, h * rep:(h + 1) * rep] = (
                 2.0 ** -11 * r.abs() + 2.0 ** -25  # (fp16 subnormal outputs)
                 + (2.0 ** -11 + 2 * d + 2 * L * u + 4 * u) * pv * 1.001 + sub)

@@ -324,6 +324,8 @@ def test_attention_split(gpu, dtype, D, page, Hq, Hk, news, past, window):
     (128, 32, 4, 2, [130, 70], [2600, 1500], 0),
     (64, 128, 8, 1, [33, 20], [4100, 33], 2000),
     (64, 16, 2, 2, [100] * 3, [900, 0, 2500], 0),
+    (64, 64, 64, 64, [640], [0], 0),               # 320 units, two a CU in turn
+    (64, 64, 64, 64, [300, 340], [0, 20], 0),
 ])
 def test_attention_prompt_split(gpu, dtype, D, page, Hq, Hk, news, past, window):
     """Rows about the limit between the two forms, and prompts whose positions
