@@ -99,6 +99,9 @@ struct PromptStage {
         ks[k] = e8m0_value(c.ks[at]) * scale2;
         ev[k] = e8m0_exponent(c.vs[at]);
       }
+      // not 0, which times the -inf of a score that a row does not see is NaN; to
+      // scores, of up to 2^39, 2^-126 is one
+      if (ks[k] < 0x1p-126f) ks[k] = 0x1p-126f;
       if (bad) ks[k] = __builtin_nanf("");
     }
 #pragma unroll

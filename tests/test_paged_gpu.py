@@ -785,3 +785,20 @@ def test_refusals(gpu):
     # nothing to do
     assert kernels.paged_attention(q[:0], kp, vp, scale=1.0, **ok).shape == (0, 256)
     assert kernels.paged_append(k[:0], k[:0], kp, vp, q=q[:0], **ok).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-8, -1e-8, 1e-38, 1e-45])
+@pytest.mark.parametrize("news,past", [([1, 1], [40, 69]), ([40, 33], [0, 70])])
+def test_attention_any_scale(gpu, dtype, D, scale, news, past):
+    """Scales below, at and next to zero, down to the smallest fp32 one, in both
+    forms: blocks that no token has written have the scale 2^-127 in a cache of
+    zeros, and what rows do not see has no weight all the same."""
+    c = Cache(gpu, 2, 2, D, 16, dtype, 140, 38)
+    for x in c.t:
+        if x is not None:
+            x.view(torch.uint8).zero_()
+    c.fill([n + p for n, p in zip(news, past)])
+    q = (torch.randn(sum(news), 4, D, generator=c.g) * 2).half().to(gpu)
+    check_attend(c, q, news, scale)
