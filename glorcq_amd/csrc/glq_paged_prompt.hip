@@ -365,17 +365,21 @@ void paged_prompt_kernel(PagedAttnArgs a) {
       }
     }
   };
-  // m follows where a score has passed it by 2^kPpLag, in whole powers of two,
-  // by which the weights in w can be scaled exactly
+  // m follows where a score has passed it by 2^kPpLag, in whole powers of two.
+  // The weights in w, of up to 2^8, then keep what fp16 has of them: their
+  // factor is applied in two, since as one fp16 value it is 0 from 2^-25 on
+  // (down to 2^-16 it is the first alone; below 2^-40 nothing is left of w).
   auto follow = [&](float mx) {
     if (__builtin_amdgcn_ballot_w64(mx > m + kPpLag)) {  // (-inf + lag: any score passes)
       const float mn = fmaxf(m, ceilf(mx)), mf = mn == -__builtin_inff() ? 0.f : mn;
-      const float f = __builtin_amdgcn_exp2f(m - mf);
-      const _Float16 fh = (_Float16)f;
+      const float d = m - mf, d0 = fmaxf(d, -16.f), d1 = fmaxf(d - d0, -24.f);
+      const float f = __builtin_amdgcn_exp2f(d);
+      const _Float16 f0 = (_Float16)__builtin_amdgcn_exp2f(d0);
+      const _Float16 f1 = (_Float16)__builtin_amdgcn_exp2f(d1);
       m = mn;
       l *= f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) w[k] *= fh;
+      for (int k = 0; k < 2; ++k) w[k] = w[k] * f0 * f1;
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll

@@ -2,6 +2,8 @@
 against its formulas in 64 bits (paged_ref), over formats, head layouts, page
 sizes, lengths and masks; the bounds are paged_ref's, derived there."""
 
+import math
+
 import pytest
 import torch
 
@@ -802,3 +804,26 @@ def test_attention_any_scale(gpu, dtype, D, scale, news, past):
     c.fill([n + p for n, p in zip(news, past)])
     q = (torch.randn(sum(news), 4, D, generator=c.g) * 2).half().to(gpu)
     check_attend(c, q, news, scale)
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rise", [16.0, 24.0, 26.0, 30.0])
+def test_prompt_scores_that_rise(gpu, dtype, D, rise):
+    """Scores that rise by 7.5 (in powers of two), which the running maximum
+    leaves, and then further: the weights of 2^7.5 that wait for their product
+    by then keep what the new maximum leaves of them."""
+    c = Cache(gpu, 1, 1, D, 32, dtype, 160, 39)
+    n, first = 40, 96
+    k = torch.zeros(first + n, 1, D, dtype=torch.float64)
+    v = torch.zeros_like(k)
+    k[32:64, 0, 0] = 7.5
+    k[70, 0, 0] = rise
+    v[32:64, 0, :D - 1] = 1.0
+    v[:, 0, D - 1] = 1.0  # (every block of one scale)
+    c.model.put("k", 0, k)
+    c.model.put("v", 0, v)
+    c.upload()
+    q = torch.zeros(n, 1, D, dtype=torch.float16, device=gpu)
+    q[..., 0] = 1.0
+    check_attend(c, q, [n], math.log(2.0))
