@@ -96,6 +96,15 @@ inline bool apart(const void* a, int64_t an, const void* b, int64_t bn) {
   return (uintptr_t)a + an <= (uintptr_t)b || (uintptr_t)b + bn <= (uintptr_t)a;
 }
 
+// Whether n rows of `row` bytes, `stride` >= row apart, and a range of bytes
+// have none in common.
+inline bool rows_apart(const void* rows, int64_t row, int64_t stride, int64_t n, const void* b,
+                       int64_t bn) {
+  const int64_t lo = (int64_t)((uintptr_t)b - (uintptr_t)rows), hi = lo + bn;
+  const int64_t i = lo < row ? 0 : (lo - row) / stride + 1;  // the first row that ends past lo
+  return i >= n || i * stride >= hi;
+}
+
 // Checks a cache and its batch and fills the kernels' view of them (the pages
 // themselves may be null in a batch of no tokens).
 int paged_view(const glq_paged_cache* c, const int32_t* starts, int64_t tokens, PagedView& view);

@@ -380,6 +380,17 @@ extern "C" int glq_paged_append(const glq_paged_append_params* p, void* stream) 
                   apart(q, ((tokens - 1) * (q_item_rows > 0 ? row : q_stride) + row) * 2, q_out,
                         tokens * row * 2),
               "q_out must not overlap q (but for rows side by side, rotated in place)");
+    // (other waves read these while q_out is written)
+    const int64_t head = D * 2, out_bytes = tokens * row * 2;
+    const int64_t cs_step = cs_stride > 0 ? cs_stride * 2 : head;
+    const int64_t cs_rows = cs_stride > 0 ? tokens : 1;
+    GLQ_CHECK(rows_apart(k, Hk * head, k_stride * 2, tokens, q_out, out_bytes) &&
+                  rows_apart(v, Hk * head, v_stride * 2, tokens, q_out, out_bytes) &&
+                  (!cos || (rows_apart(cos, head, cs_step, cs_rows, q_out, out_bytes) &&
+                            rows_apart(sin, head, cs_step, cs_rows, q_out, out_bytes))) &&
+                  (!q_norm_w || apart(q_norm_w, head, q_out, out_bytes)) &&
+                  (!k_norm_w || apart(k_norm_w, head, q_out, out_bytes)),
+              "q_out must not overlap k, v, cos, sin or the norm weights");
   }
   a.q = (const __half*)q; a.k = (const __half*)k; a.v = (const __half*)v;
   a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;

@@ -177,8 +177,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     not) and rotated (cos/sin (T or 1, D), None: not) and rounded once to the
     pages' type; with q (T, Hq*D) -- or item-major (n, T, R), a batched GEMV's
     output over R-row slices -- its heads likewise, returned as q_out (T, Hq, D)
-    fp16 (else None; q itself where its rows lie side by side).  Rows of k, v
-    and q may be slices of a wider matrix; a 3-D q whose last dimension is D is
+    fp16 (else None; q itself where its rows lie side by side, apart from all
+    other inputs).  Rows of k, v and q may be slices of a wider matrix; a 3-D q whose last dimension is D is
     (T, Hq, D), never item-major.
     8-bit pages: a block's scale is the smallest power of two that takes its
     values to e4m3's 448; tokens that a block already had are scaled along when

@@ -785,8 +785,9 @@ typedef struct glq_paged_cache {
  * becomes zero.  Rows of k, v and q are k_stride, v_stride and q_stride values
  * apart (multiples of 8); with q_item_rows > 0, q is item-major as in
  * glq_qk_norm_rope.  q_out may be q itself where q's rows lie side by side, and
- * must not overlap it otherwise.  Pages that get tokens must belong to one
- * sequence.
+ * must not overlap it otherwise, nor any of the other inputs' values (refused
+ * where it overlaps k, v, cos, sin or a norm weight).  Pages that get tokens must
+ * belong to one sequence.
  */
 typedef struct glq_paged_append_params {
   glq_paged_cache cache;

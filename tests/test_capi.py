@@ -512,3 +512,24 @@ def test_paged_workspace_serves_smaller_sizes():
                     lib.glq_paged_attention_scratch_bytes(seqs - 1, tokens, rep * kv, kv)]
             assert less[0] <= now[0] and less[1] <= now[1]
             last = now
+
+
+# a q of two rows of 4 heads, side by side, far from everything else
+_APART = dict(q=1 << 20, q_heads=4, q_stride=512, k_stride=1024, v_stride=1024, k=P, v=P + 512)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q_out=P), dict(q_out=P + 2048 + 496), dict(q_out=P - 2032), dict(q_out=P + 16),
+    dict(k=1 << 16, q_out=P + 512), dict(k=1 << 16, q_out=P + 2048 + 1008),
+    dict(cos=P * 64, sin=P * 65, q_out=P * 64 + 240), dict(cos=P * 64, sin=P * 65, q_out=P * 65),
+    dict(cos=P * 64, sin=P * 65, cs_stride=128, q_out=P * 65 + 496),
+    dict(q_norm_w=P * 64, q_out=P * 64), dict(k_norm_w=P * 64, q_out=P * 64 - 1024),
+    # one fused row of q, k and v, whose k begins within q
+    dict(tokens=1, seqs=1, q=P, k=P + 1008, v=P * 32, q_out=P),
+])
+def test_paged_append_output_over_an_input(lib, kw):
+    """q_out over something that the launch reads beside q: other waves would
+    read it while it is written."""
+    kw = {**_APART, **kw}
+    rc, msg = _append(lib, dict(seqs=kw.pop("seqs", 2)), **kw)
+    assert rc == 1 and b"overlap" in msg

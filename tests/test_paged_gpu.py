@@ -827,3 +827,39 @@ def test_prompt_scores_that_rise(gpu, dtype, D, rise):
     q = torch.zeros(n, 1, D, dtype=torch.float16, device=gpu)
     q[..., 0] = 1.0
     check_attend(c, q, [n], math.log(2.0))
+
+
+def test_append_output_between_rows(gpu):
+    """q_out may lie between the rows of a strided k and v, and a single token's
+    fused row of q, k and v is rotated in place; over their rows it is refused."""
+    c = Cache(gpu, 2, 2, 64, 16, FP16, 64, 41)
+    c.lengths.fill_(20)
+    T, S = 40, 40000
+    buf = torch.randn(T, S, generator=c.g).half().to(gpu)
+    k, v = buf[:, :128], buf[:, 20000:20128]
+    q = torch.randn(T, 4, 64, generator=c.g).half().to(gpu)
+    cos, sin = (x.to(gpu) for x in rope_rows(torch.arange(T), 64))
+    s, kp, vp = c.pages()
+    args = (kp, vp, c.table, c.lengths)
+
+    def held():  # bits (there is garbage in the pool)
+        return torch.cat([x.view(torch.int16).flatten() for x in (kp, vp)])
+
+    want = kernels.paged_append(k, v, *args, cos=cos, sin=sin, q=q, **s)
+    pages = held()
+    between = buf[3, 128:128 + T * 256].view(T, 4, 64)
+    got = kernels.paged_append(k, v, *args, cos=cos, sin=sin, q=q, q_out=between, **s)
+    assert got.data_ptr() == between.data_ptr() and torch.equal(got, want)
+    assert torch.equal(held(), pages)
+    for bad in (buf[3, :T * 256], buf[3, 19968:19968 + T * 256]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            kernels.paged_append(k, v, *args, q=q, q_out=bad, **s)
+    one = torch.randn(1, 512, generator=c.g).half().to(gpu)
+    q, k, v = one.split([256, 128, 128], 1)
+    args = (kp, vp, c.table[:1], torch.ones(1, dtype=torch.int32, device=gpu))
+    at = dict(cos=cos[5:6], sin=sin[5:6], **s)
+    want = kernels.paged_append(k, v, *args, q=q, **at)
+    pages = held()
+    kernels.paged_append(k, v, *args, q=q, q_out=q, **at)
+    assert torch.equal(q.view(1, 4, 64), want)
+    assert torch.equal(held(), pages)
