@@ -863,3 +863,49 @@ def test_append_output_between_rows(gpu):
     kernels.paged_append(k, v, *args, q=q, q_out=q, **at)
     assert torch.equal(q.view(1, 4, 64), want)
     assert torch.equal(held(), pages)
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+@pytest.mark.parametrize("D,new,past,window", [
+    (64, 640, 3707, 0), (128, 640, 3707, 0),  # 137 steps in one run
+    (64, 640, 7000, 4357), (128, 640, 7000, 4357),  # that begin past 0
+    (64, 640, 8001, 0), (128, 640, 8001, 0),  # 270 steps in two parts
+])
+def test_prompt_long_runs(gpu, dtype, D, new, past, window):
+    """Prompts of 320 units, two a CU: runs of far more steps than a workgroup
+    looks up at once, and a long context's two parts of a unit.  Sampled rows and
+    heads."""
+    Hq, Hk, page = 64, 16, 32
+    L = new + past
+    P = -(-L // page)
+    pool = P + 5
+    g = torch.Generator().manual_seed(40)
+    table = torch.randperm(pool, generator=g)[:P].to(torch.int32)
+    kp, vp, ks, vs = kernels.paged_cache_tensors(pool, Hk, D, page, dtype, gpu)
+    for x in (kp, vp):
+        x.copy_(torch.randn(x.shape, generator=g).to(dtype))
+    if dtype == FP8:  # scales from 2^-2 to 2
+        for x in (ks, vs):
+            x.view(torch.uint8).copy_(torch.randint(125, 129, x.shape, generator=g))
+    q = torch.randn(new, Hq, D, generator=g).half()
+    lengths = torch.tensor([L], dtype=torch.int32, device=gpu)
+    y = kernels.paged_attention(q.to(gpu), kp, vp, table.view(1, P).to(gpu), lengths, 0.1,
+                                k_scales=ks, v_scales=vs, window=window)
+    torch.cuda.synchronize()
+    y = y.cpu().double().view(new, Hq, D)
+    pg = table.long()
+    for h in (0, 7, 15):
+        k = kp.cpu()[pg, h].double()               # (P, page, D)
+        v = vp.cpu()[pg, h].double().mT            # (P, blocks, 16, D)
+        ev = torch.zeros(1, P * page // 16, dtype=torch.int64)
+        if dtype == FP8:
+            ek, ev = (x.view(torch.uint8).cpu()[pg, h].long() - 127 for x in (ks, vs))
+            k = k.view(P, -1, 16, D) * torch.exp2(ek.double())[..., None, None]
+            v = v * torch.exp2(ev.double())[..., None, None]
+            ev = ev.view(1, -1)
+        k, v = (x.reshape(-1, 1, D)[:L] for x in (k, v))
+        for i in (0, 290, new - 12):  # 48 rows of the KV head
+            heads = slice(4 * h, 4 * h + 4)
+            ref, tol = R.attend(q[i:i + 12, heads], k, v, ev, past + i, 0.1, window, dtype == FP8)
+            d = (y[i:i + 12, heads] - ref).abs()
+            assert (d <= tol).all(), (h, i, float((d / tol).max()))
