@@ -11,6 +11,7 @@ are given back and used again."""
 import pytest
 import torch
 
+import paged_ref as R
 from glorcq_amd import kernels
 from glorcq_amd.graph_wrapper import _static_cache
 from glorcq_amd.paged_cache import GLoRCQPagedWrapper, PagedKVCache, PagedStep, paged_forward
@@ -192,3 +193,83 @@ def test_wrapper_refusals(gpu):
     w.capture_graph()
     with pytest.raises(RuntimeError, match="input_ids must be"):
         w.replay(a[:1])
+
+
+class _Rounded:
+    """paged_append for fp16 pages that then hold what 8-bit ones would: each
+    block's values as e4m3 codes of its scale, worked out on the CPU in 64 bits
+    (paged_ref.Model)."""
+
+    def __init__(self, append):
+        self.append, self.layers = append, {}
+
+    def __call__(self, k, v, k_pages, v_pages, page_table, lengths, starts=None, **kw):
+        out = self.append(k, v, k_pages, v_pages, page_table, lengths, starts=starts, **kw)
+        _, Hk, page, D = k_pages.shape
+        B, table = len(lengths), page_table.cpu().long()
+        m = self.layers.setdefault(k_pages.data_ptr(), R.Model(B, Hk, D, page, True, 0, None))
+        st = [i * len(k) // B for i in range(B + 1)] if starts is None else starts.tolist()
+        kp, vp = k_pages.cpu(), v_pages.cpu()
+        for b, L in enumerate(lengths.tolist()):
+            pos = torch.arange(L)
+            pg, at = table[b, pos // page], pos % page
+            fresh = pos >= L - (st[b + 1] - st[b])
+            m.put("k", b, kp[pg, :, at][fresh].double())
+            m.put("v", b, vp[pg, :, at // 16, :, at % 16][fresh].double())
+            kp[pg, :, at] = m.k[b].half()
+            vp[pg, :, at // 16, :, at % 16] = m.v[b].half()
+        k_pages.copy_(kp)
+        v_pages.copy_(vp)
+        return out
+
+
+@torch.no_grad()
+def test_e4m3_pages_cost_their_rounding_alone(gpu, monkeypatch):
+    """The default cache, prompts and captured decode steps: the logits of a run
+    over fp16 pages whose values are rounded as 8-bit ones are, within the other
+    tests' 2 % of their range; and in the first layer, whose inputs are the same
+    bits, codes that are the same or neighbours (a value of the fp16 pages has
+    been rounded before)."""
+    model = _model(gpu)
+    lens = (40, 7, 64)
+    prompts = _prompts(lens, gpu)
+    g = torch.Generator().manual_seed(11)
+    cont = torch.randint(0, VOCAB, (12, 3), generator=g).to(gpu)
+    a = GLoRCQPagedWrapper(model, max_batch_size=3, max_seq_len=80, page_size=32)
+    assert a.cache.layers[0][0].dtype == torch.float8_e4m3fn
+    a.capture_graph()
+    got = [a.prefill(prompts).clone()] + [a.replay(t).clone() for t in cont]
+    b = GLoRCQPagedWrapper(model, max_batch_size=3, max_seq_len=80, page_size=32,
+                           cache_dtype=torch.float16)
+    monkeypatch.setattr(kernels, "paged_append", _Rounded(kernels.paged_append))
+    want = [b.prefill(prompts)]
+    for t in cont:
+        pos = torch.tensor([b.cache.length(i) for i in range(3)], device=gpu)
+        b.cache.extend(1)
+        want.append(paged_forward(model, t, pos, PagedStep(b.cache)))
+    torch.cuda.synchronize()
+    got, want = torch.stack(got).float(), torch.stack(want).float()
+    err = (got - want).abs().amax((0, 2))
+    assert (err <= 0.02 * want.abs().amax((0, 2))).all(), err
+    # 16-token blocks of the sequences' tokens (both caches gave out the same pages)
+    assert torch.equal(a.cache.page_table, b.cache.page_table)
+    (kq, vq, ks, vs), (kf, vf) = a.cache.layers[0], b.cache.layers[0][:2]
+    table = a.cache.page_table.cpu().long()
+    for q, s, f, rows in ((kq, ks, kf, True), (vq, vs, vf, False)):
+        q, s, f = q.cpu().double(), s.cpu().view(torch.uint8).double() - 127, f.cpu().double()
+        q, f = (x.unflatten(2, (2, 16)) if rows else x.mT for x in (q, f))  # (.., blocks, 16, D)
+        step = torch.exp2(s)[..., None, None]
+        q = q * step
+        # one step: 2^-3 of the larger value, 2^-9 of the scale where codes are subnormal
+        # (a scale may differ too, where the largest value was rounded over its border)
+        near = (q - f).abs() <= 2.0 ** -3 * torch.maximum(q.abs(), f.abs()) + 2.0 ** -8 * step
+        same = q == f
+        n = differ = 0
+        for i, L in enumerate(lens):
+            for p in range(L + len(cont)):
+                at = (table[i, p // 32], slice(None), p % 32 // 16, p % 16)
+                assert near[at].all()
+                n, differ = n + same[at].numel(), differ + int((~same[at]).sum())
+        # a value is next to a border of two codes (4 bits) by an fp16 rounding (11
+        # bits) once in 2^7
+        assert differ <= n * 2.0 ** -6, (differ, n)
