@@ -138,8 +138,11 @@ struct RowAttention {
 
   // Online softmax over the tile's positions.  The scale 2^e of a V block goes
   // into the exponent: w = 2^(t + e - m) with m the largest t + e so far, so
-  // that w (fp16 for the product) keeps its bits where the block's share of
-  // the result is largest; the denominator sums w 2^-e in fp32.
+  // that w keeps its bits where the block's share of the result is largest.  It
+  // is rounded to fp16 for the product alone, in which V's codes are exact; the
+  // denominator sums w 2^-e in fp32.  The largest weight is 1 and loses nothing:
+  // outputs are 2.1e-4 to 2.2e-4 off the exact ones (root mean square, relative),
+  // 2.1e-4 of it their own rounding to fp16.
   // `next_k`: fetches the next tile's k into x, whose k has been used by then.
   template <class Next>
   __device__ void step(Tile& x, int tile, Next next_k) {

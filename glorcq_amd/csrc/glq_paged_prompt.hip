@@ -42,18 +42,24 @@ constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running max
 // between two matrix ones; and the maximum of u + 1 and the way of K of u + 3
 // and V of u to LDS with them.  The bytes of two steps more are in flight.
 //
-// Bound by instructions: of a CU's 2600 cycles for two workgroups' steps, 1024
-// are matrix instructions', about as many LDS transfers' and 1200 vector ones'
-// (a step of a workgroup alone on its CU takes 1800, one wave's time to issue
-// it).  4096 tokens of 32 and 4 heads: 161 to 187 us on different cards, 735 to
-// 855 TF/s of what the mask leaves; 512 behind 30000: 278 to 300 us, 850 to 910
-// TF/s (a library product of 8192^3 reaches 1143, these matrix instructions
-// alone 1190).
+// Bound by the waves' instruction streams: of a CU's 2400 to 2700 cycles for two
+// workgroups' steps the matrix pipe is busy for 43 % and the vector unit, with
+// the issue of matrix instructions, for 63 % of each SIMD's, LDS for 38 %, and
+// two waves a SIMD leave gaps between them (a step of a workgroup alone on its
+// CU takes 1800, one wave's time to issue it).  4096 tokens of 32 and 4 heads:
+// 158 to 189 us, 730 to 870 TF/s of what the mask leaves; 512 behind 30000: 271
+// to 301 us, 840 to 940 TF/s (on several cards; on one of them a prompt takes 163
+// us between other work, 177 in a row with its like).  A library product of
+// 8192^3 reaches 1143 TF/s, these matrix instructions alone 1190.
 //
 // Softmax: the running maximum m of t + e (e the exponent of V's block, as in
 // the first form) follows the scores only when one passes it by more than
 // 2^kPpLag: weights up to 2^8 lose nothing, in fp16 or in the fp32 sums, and
-// the 64 sums of O a lane are rarely scaled.
+// the 64 sums of O a lane are rarely scaled.  Weights are rounded to fp16 for
+// the product with V (exact ones would take a second product; V's codes are exact in
+// it), not in the denominator; no weight is 1 here as the largest of the first
+// form is, so this shows: outputs are 2.9e-4 off the exact ones (root mean
+// square, relative), 2.1e-4 of it their own rounding to fp16.
 template <int D, bool FP8>
 struct PromptStage {
   static constexpr int S = FP8 ? 1 : 2;             // bytes of a value

@@ -5,7 +5,9 @@ and MoE blocks as framework ops (its graph wrapper captures them as they are,
 inference/graph_wrapper.py:69-149).  For the Qwen3-MoE-shaped model that is
 ~60 small kernels per layer per decode token (RMSNorm alone is 7), which at
 decode sizes cost more than the projections.  These modules replace them
-with one launch each, keeping the framework's fp16 rounding points:
+with one launch each, keeping the framework's fp16 rounding points (but for the
+paged path, whose append rounds a head once, after norm and rotation, k from
+fp64, and whose 8-bit pages round k and v to e4m3):
 
 * `FusedRMSNorm` -- Qwen3MoeRMSNorm (glq_rmsnorm);
 * `GLoRCQQwen3Attention` -- Qwen3MoeAttention for one decode token against a

@@ -280,10 +280,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Causal attention of the new tokens' q (T, Hq, D) fp16 (paged_append's
     result) over their sequences' pages -> (T, Hq*D) fp16 (glq_paged_attention).
     The token at position p attends to (p - window, p], or [0, p] with window
-    0.  `out` (apart from q): rows behind starts[B] keep what they held.  `workspace`: from
-    paged_attention_workspace; None takes one of the stream's, or under graph
-    capture one of the call's own, so that graphs may be replayed on several
-    streams."""
+    0; scale may be 0 or negative.  Scores, softmax and sums are fp32, the
+    weights in the product with V fp16.  `out` (apart from q): rows behind
+    starts[B] keep what they held.  `workspace`: from paged_attention_workspace;
+    None takes one of the stream's, or under graph capture one of the call's own,
+    so that graphs may be replayed on several streams."""
     lib = _lib.load()
     if not isinstance(q, torch.Tensor) or q.dim() not in (2, 3):
         raise RuntimeError("q must be (T, Hq, D) or (T, Hq*D)")

@@ -4,7 +4,9 @@ The static cache of the graph wrapper holds one position for the whole batch
 and max_seq_len positions a sequence in fp16.  Here every sequence has a length
 of its own, memory is taken a page at a time from one pool a layer, and values
 are e4m3 codes with a power-of-two scale for each 16 tokens of a head (half the
-bytes), or fp16.  No reference counterpart (its model path has the static cache
+bytes), or fp16.  Logits differ from the static cache's by these roundings, and
+with fp16 pages by k's and q's, which are rounded once, after norm and rotation,
+where the static path rounds between them too.  No reference counterpart (its model path has the static cache
 alone, inference/graph_wrapper.py:69-149).
 
 * `PagedKVCache` -- the pools of all layers, the page table and the lengths:

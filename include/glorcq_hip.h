@@ -811,11 +811,12 @@ int glq_paged_append(const glq_paged_append_params* p, void* stream);
  * the row of q at position p of its sequence attends to positions
  * (p - window, p], window 0: [0, p]:
  *   out[t][h*D + d] = fp16(sum_p softmax_p(scale * q.k_p) v_p[d]),
- * KV head h / (q_heads / kv_heads), fp32 scores, softmax and sums.  A row
- * without positions (p < 0) is 0; one past the page table NaN.  q (tokens,
- * q_heads, head_dim) fp16, out (tokens, q_heads * head_dim) apart from it.  The
- * workspace's sizes never shrink with seqs or tokens; a workspace serves smaller
- * calls too: the
+ * KV head h / (q_heads / kv_heads), scale of either sign or 0; fp32 scores,
+ * softmax and sums, but for the softmax's weights in the product with V, which
+ * are fp16 (2^-11 of each).  A row without positions (p < 0) is 0; one past the
+ * page table NaN.  q (tokens, q_heads, head_dim) fp16, out (tokens, q_heads *
+ * head_dim) apart from it.  The workspace's sizes never shrink with seqs or
+ * tokens; a workspace serves smaller calls too: the
  * counters (glq_paged_attention_counter_bytes) are zero before their first use
  * and left zero by each call; the scratch (.._scratch_bytes, 256-byte aligned)
  * needs no initialisation (both negative for invalid sizes).  Calls that share
