@@ -95,7 +95,7 @@ class PagedAttentionParams(ctypes.Structure):
         ("cache", PagedCache), ("starts", _vp), ("tokens", _i64), ("q", _vp), ("out", _vp),
         ("q_heads", _i64), ("window", _i64), ("counters", _vp), ("scratch", _vp),
         ("counter_bytes", _i64), ("scratch_bytes", _i64),
-        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("sinks", ctypes.c_int32),
     ]
 
 

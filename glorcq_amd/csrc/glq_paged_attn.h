@@ -23,7 +23,7 @@ struct PagedAttnArgs {
   __half* out;      // (T, Hq D)
   float* part;      // parts of units: o, m, l of a row in D + 4
   unsigned* count;  // [unit], zero between calls (first form)
-  int rep, window, slots_each, rows;
+  int rep, window, sinks, slots_each, rows;
   int slots, splits, split_steps, fold;  // second form
   float scale2;                    // scale log2(e)
 };
@@ -60,6 +60,32 @@ __device__ __forceinline__ void set_rows(RowSet& r, const PagedView& c, int b, i
   r.lo_all = lo(r.first + r1 / rep);
   r.hi_any = hi(r.first + r1 / rep);
 }
+
+// The n tiles of TP positions of which some row sees one, numbered from `begin`
+// on: those of positions [lo, hi), a window's or all; with SINKS those of the
+// sinks before them, as far as they lie before lo's.  (Without sinks a number is
+// the tile's place: as one kernel for both, calls without took 1.5 to 3.5 % more.)
+template <int TP, bool SINKS>
+struct Span {
+  int begin, n, sink = 0, skip = 0;
+  __device__ Span(int lo, int hi, int sinks) {
+    const int first = lo / TP;
+    begin = first;
+    n = max((hi + TP - 1) / TP - first, 0);
+    if constexpr (SINKS) {
+      begin = 0;
+      sink = min((sinks + TP - 1) / TP, first);
+      skip = first - sink;
+      n += sink;
+    }
+  }
+  __device__ int place(int t) const {
+    if constexpr (SINKS)
+      return t < sink ? t : t + skip;
+    else
+      return t;
+  }
+};
 
 // 4 columns of a row's result to memory.
 __device__ __forceinline__ void store_row(__half* dst, f32x4 v, float den, int pos, int cap) {

@@ -2,6 +2,7 @@
 // (layout and formats: glq_paged.h), a few query rows a KV head at a time.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "glq_paged_attn.h"
 
@@ -24,7 +25,7 @@ constexpr int kPaGrid = 256;
 // 128 KB in flight there.  64 sequences of 3 to 8000 positions, 8-bit pages:
 // 61 us, 4.8 TB/s, what a copy reaches (a read alone 6.1); one sequence of
 // 130000: 36 us, 3.7 TB/s; of 517, 10 us, of which 5 are an empty launch's.
-template <int D, bool FP8>
+template <int D, bool FP8, bool SINKS>
 struct RowAttention {
   // A tile is TP positions, in NS parts of TS; of each part, lane group kb has P
   // consecutive ones, as rows 4 kb + j of the NT products of 16 positions and as
@@ -43,7 +44,7 @@ struct RowAttention {
   };
 
   const PagedView& c;
-  int b, g, li, kb, rep, window;
+  int b, g, li, kb, rep, window, sinks;
   float scale2;
   RowSet r;
   f16x8 q[D / 32];
@@ -147,7 +148,8 @@ struct RowAttention {
   template <class Next>
   __device__ void step(Tile& x, int tile, Next next_k) {
     const int p0 = tile * TP + P * kb;
-    const bool edge = tile * TP < r.lo_all || (tile + 1) * TP > r.hi_all;
+    const bool edge =
+        (tile * TP < r.lo_all && !(SINKS && (tile + 1) * TP <= sinks)) || (tile + 1) * TP > r.hi_all;
     float t[NS][NT][4], ev[NS];
     float mx = m;
 #pragma unroll
@@ -166,7 +168,8 @@ struct RowAttention {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int p = p0 + u * TS + 4 * i + j;
-            if (p < r.lo || p >= r.hi) t[u][i][j] = -__builtin_inff();
+            if ((p < r.lo && !(SINKS && p < sinks)) || p >= r.hi)
+              t[u][i][j] = -__builtin_inff();
           }
         }
 #pragma unroll
@@ -219,13 +222,15 @@ struct RowAttention {
         for (int u = 0; u < NS; ++u) {
           const int pu = p0 + u * TS;
           const int n0 = min(max(lo - pu, 0), P), n1 = min(max(hi - pu, 0), P);
+          const int ns = SINKS ? min(max(sinks - pu, 0), n1) : 0;
           constexpr int E = FP8 ? 4 : 2;  // values of a word
           auto below = [](int n) {        // the bits of its first n values
             return n <= 0 ? 0u : n >= E ? ~0u : (1u << (32 / E * n)) - 1u;
           };
           u32x4 keep;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) keep[e] = below(n1 - E * e) & ~below(n0 - E * e);
+          for (int e = 0; e < 4; ++e)
+            keep[e] = (below(n1 - E * e) & ~below(n0 - E * e)) | below(ns - E * e);
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
             const u32x4 v = x.v[u][i] & keep;
@@ -259,14 +264,11 @@ struct RowAttention {
   }
 };
 
-// Tiles of each of a sequence's units, 0 for a sequence without new tokens (the
-// rows of others are written even where they see nothing: at least 1).
-template <int TP>
-__device__ __forceinline__ int sequence_tiles(const RowSet& r, int window) {
-  if (r.n == 0) return 0;
-  const int lo = window > 0 ? max(r.first - window + 1, 0) : 0;
-  const int hi = min(max(r.first + r.n, 0), r.cap);
-  return max((hi + TP - 1) / TP - lo / TP, 1);
+// The tiles of each of a sequence's units.
+template <int TP, bool SINKS>
+__device__ __forceinline__ Span<TP, SINKS> sequence_span(const RowSet& r, int window, int sinks) {
+  return Span<TP, SINKS>(window > 0 ? max(r.first - window + 1, 0) : 0,
+                         min(max(r.first + r.n, 0), r.cap), sinks);
 }
 
 // The batch's work is a line of tiles: sequence by sequence, unit by unit (KV
@@ -286,7 +288,7 @@ __device__ __forceinline__ int sequence_tiles(const RowSet& r, int window) {
 constexpr int kPaShort = 4;
 
 // The line, as every wave works it out for itself: 64 sequences a step.
-template <int TP>
+template <int TP, bool SINKS>
 struct Line {
   int total, quota, align;
 
@@ -297,7 +299,9 @@ struct Line {
     r.n = max((c.starts ? c.start(b + 1) : r.s0 + c.each) - r.s0, 0);
     r.first = c.length(b) - r.n;
     r.cap = c.max_pages << c.page_shift;
-    tiles = sequence_tiles<TP>(r, a.window);
+    // 0 for a sequence without new tokens (the rows of others are written even
+    // where they see nothing: at least 1)
+    tiles = r.n == 0 ? 0 : max(sequence_span<TP, SINKS>(r, a.window, a.sinks).n, 1);
     // (a sequence of more rows is the second form's)
     units = c.starts && r.n * a.rep > kPaMostRows ? 0 : (r.n * a.rep + kPaRows - 1) / kPaRows * c.Hk;
   }
@@ -362,9 +366,9 @@ struct Line {
   }
 };
 
-template <int D, bool FP8>
+template <int D, bool FP8, bool SINKS>
 __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a) {
-  using RA = RowAttention<D, FP8>;
+  using RA = RowAttention<D, FP8, SINKS>;
   constexpr int TP = RA::TP, PS = D + 4;
   struct Seg {  // a unit's piece that did not stay within its wave
     int b, unit, tiles, ended, line;  // line: of the unit's first tile
@@ -375,7 +379,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
   const PagedView& c = a.c;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int Hq = c.Hk * a.rep;
-  const Line<TP> line(a);
+  const Line<TP, SINKS> line(a);
   const int wg_quota = line.quota * kPaWaves, wg0 = blockIdx.x * wg_quota;
   if (wg0 >= line.total) return;  // uniform
   if (lane < 2) seg[wave][lane].unit = -1;
@@ -384,6 +388,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
   x.scale2 = a.scale2;
   x.rep = a.rep;
   x.window = a.window;
+  x.sinks = a.sinks;
   {
     int off = 0, left = line.quota, pos = wg0 + wave * line.quota;
     int tiles = 0, units = 0, b = line.find(a, pos, off, tiles, units);
@@ -406,26 +411,26 @@ __global__ __launch_bounds__(kPaThreads) void paged_rows_kernel(PagedAttnArgs a)
       x.b = b;
       x.g = unit - qt * c.Hk;
       set_rows<kPaRows>(x.r, c, b, qt * kPaRows, a.rep, a.window, x.li);
-      const int first = (a.window > 0 ? max(x.r.first - a.window + 1, 0) : 0) / TP;
+      const Span<TP, SINKS> span = sequence_span<TP, SINKS>(x.r, a.window, a.sinks);
       // k and v of the next tile are fetched as soon as the present one's have
       // been used, page ids a tile before them
       {
-        const int e = first + t1;
-        int t = first + t0;
+        const int e = span.begin + t1;
+        int t = span.begin + t0;
         typename RA::Tile tile;
-        typename RA::Ids id = x.ids(t), ahead = x.ids(t + 1);
+        typename RA::Ids id = x.ids(span.place(t)), ahead = x.ids(span.place(t + 1));
         x.begin(a.q, Hq);
-        x.load_k(tile, t, id);
-        x.load_v(tile, t, id);
+        x.load_k(tile, span.place(t), id);
+        x.load_v(tile, span.place(t), id);
         for (; t < e; ++t) {
-          x.step(tile, t, [&] {
+          x.step(tile, span.place(t), [&] {
             if (t + 1 < e) {
               id = ahead;
-              ahead = x.ids(t + 2);
-              x.load_k(tile, t + 1, id);
+              ahead = x.ids(span.place(t + 2));
+              x.load_k(tile, span.place(t + 1), id);
             }
           });
-          if (t + 1 < e) x.load_v(tile, t + 1, id);
+          if (t + 1 < e) x.load_v(tile, span.place(t + 1), id);
         }
       }
       x.l += __shfl_xor(x.l, 16);
@@ -582,7 +587,7 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
   GLQ_CHECK(p != nullptr, "null params");
   const glq_paged_cache* cache = &p->cache;
   const int32_t* starts = p->starts;
-  const int64_t tokens = p->tokens, q_heads = p->q_heads, window = p->window;
+  const int64_t tokens = p->tokens, q_heads = p->q_heads, window = p->window, sinks = p->sinks;
   const void* q = p->q;
   void* out = p->out;
   PagedAttnArgs a{};
@@ -590,7 +595,7 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
   const int64_t D = cache->head_dim, Hk = cache->kv_heads;
   GLQ_CHECK(q_heads > 0 && q_heads % Hk == 0 && q_heads <= 8192,
             "q_heads must be a positive multiple of kv_heads (<= 8192)");
-  GLQ_CHECK(window >= 0, "window must be >= 0 (0: none)");
+  GLQ_CHECK(window >= 0 && sinks >= 0, "window and sinks must be >= 0 (0: none)");
   if (tokens == 0 || cache->seqs == 0) return GLQ_OK;
   GLQ_CHECK(q && out && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0,
             "q and out must be non-null and 16-byte aligned");
@@ -606,7 +611,9 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
   a.q = (const __half*)q;
   a.out = (__half*)out;
   a.rep = (int)(q_heads / Hk);
-  a.window = window >= cache->max_pages * cache->page_size ? 0 : (int)window;
+  const int64_t cap = cache->max_pages * cache->page_size;
+  a.window = window >= cap ? 0 : (int)window;
+  a.sinks = a.window > 0 ? (int)std::min(sinks, cap) : 0;
   a.scale2 = p->scale * 1.44269504088896f;
   a.part = (float*)p->scratch;
   a.count = (unsigned*)p->counters;
@@ -630,10 +637,15 @@ extern "C" int glq_paged_attention(const glq_paged_attention_params* p, void* st
   // a sequence of 60000 positions 30 us, 37 with 16; 64 of 3000 46 and 45)
   a.rows = !starts && rows_each <= 8 ? 8 : kPaRows;
   const size_t lds = (size_t)kPaWaves * 2 * a.rows * (D + 4) * 4;
-  auto kern = D == 128 ? (a.c.ks ? paged_rows_kernel<128, true> : paged_rows_kernel<128, false>)
-                       : (a.c.ks ? paged_rows_kernel<64, true> : paged_rows_kernel<64, false>);
-  static size_t attr[4] = {64 * 1024, 64 * 1024, 64 * 1024, 64 * 1024};
-  if (int rc = set_lds_limit(kern, lds, attr[(D == 64) * 2 + !a.c.ks])) return rc;
+  const auto pick = [&](auto sinks_) {
+    constexpr bool S = decltype(sinks_)::value;
+    return D == 128 ? (a.c.ks ? paged_rows_kernel<128, true, S> : paged_rows_kernel<128, false, S>)
+                    : (a.c.ks ? paged_rows_kernel<64, true, S> : paged_rows_kernel<64, false, S>);
+  };
+  auto kern = a.sinks > 0 ? pick(std::true_type()) : pick(std::false_type());
+  static size_t attr[8] = {64 * 1024, 64 * 1024, 64 * 1024, 64 * 1024,
+                           64 * 1024, 64 * 1024, 64 * 1024, 64 * 1024};
+  if (int rc = set_lds_limit(kern, lds, attr[(a.sinks > 0) * 4 + (D == 64) * 2 + !a.c.ks])) return rc;
   kern<<<dim3(kPaGrid), dim3(kPaThreads), lds, (hipStream_t)stream>>>(a);
   GLQ_LAUNCH_CHECK("paged_rows_kernel");
   return GLQ_OK;

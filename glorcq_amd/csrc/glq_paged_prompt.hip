@@ -60,7 +60,7 @@ constexpr float kPpLag = 8.f;  // log2 by which a score may pass the running max
 // it), not in the denominator; no weight is 1 here as the largest of the first
 // form is, so this shows: outputs are 2.9e-4 off the exact ones (root mean
 // square, relative), 2.1e-4 of it their own rounding to fp16.
-template <int D, bool FP8>
+template <int D, bool FP8, bool SINKS>
 struct PromptStage {
   static constexpr int S = FP8 ? 1 : 2;             // bytes of a value
   static constexpr int PB = FP8 && D == 64 ? 8 : 16;  // bytes of a piece
@@ -75,6 +75,9 @@ struct PromptStage {
   static constexpr int kSets = KP * PB / 4 > 4 ? 1 : 2;
   Piece k[kSets][KP], v[kSets][KP];
   int wave;  // uniform
+  using Steps = Span<kPpStep, SINKS>;
+  Steps span;
+  __device__ PromptStage(const Steps& s, int w) : wave(w), span(s) {}
 
   // A wave's pieces of a pass lie in one block, K's and V's in the same, so
   // that addresses are scalars but for a lane's constant part.
@@ -94,7 +97,7 @@ struct PromptStage {
     int page[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int blk = 2 * (step + (int)(threadIdx.x & 63)) + k;
+      const int blk = 2 * span.place(step + (int)(threadIdx.x & 63)) + k;
       const int p = c.table[b * c.table_stride + min(blk >> s, c.max_pages - 1)];
       const bool bad = (unsigned)p >= (unsigned)c.pages;  // page 0 is read, its scores are NaN
       page[k] = bad ? 0 : p;
@@ -112,7 +115,7 @@ struct PromptStage {
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const int blk = 2 * (step + (int)(threadIdx.x & 63)) + block(j);
+      const int blk = 2 * span.place(step + (int)(threadIdx.x & 63)) + block(j);
       const int64_t at = place(c, g, block(j) ? page[1] : page[0], blk) * (16 * D * S);
       at_lo[j] = (uint32_t)at;
       at_hi[j] = (uint32_t)(at >> 32);
@@ -212,13 +215,15 @@ struct PromptStage {
 
 // Adds the infinities and NaN of V that the row of a lane sees, at positions of
 // steps [u0, u1), to its sums: rare, and so a plain walk over the blocks.
-template <int D, bool FP8>
+template <int D, bool FP8, bool SINKS>
 __device__ void add_odd_values(f32x16 (&o)[D / 32], const PagedView& c, int b, int g, int u0,
-                               int u1, const RowSet& r) {
-  using Stage = PromptStage<D, FP8>;
+                               int u1, const RowSet& r, const Span<kPpStep, SINKS>& span,
+                               int sinks) {
+  using Stage = PromptStage<D, FP8, SINKS>;
   constexpr int S = FP8 ? 1 : 2, NG = D / 32;
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  for (int blk = 2 * u0; blk < 2 * u1; ++blk) {
+  for (int i = 2 * u0; i < 2 * u1; ++i) {
+    const int blk = 2 * span.place(i >> 1) + (i & 1);
     const int p = c.page_of(b, blk >> (c.page_shift - 4));
     if (p < 0) continue;  // (the scores are NaN there)
     const char* base = (const char*)c.v + Stage::place(c, g, p, blk) * (16 * D * S);
@@ -239,7 +244,7 @@ __device__ void add_odd_values(f32x16 (&o)[D / 32], const PagedView& c, int b, i
     while (here) {
       const int j = __builtin_ctz(here), pos = 16 * blk + j;
       here &= here - 1;
-      const bool sees = pos >= r.lo && pos < r.hi;
+      const bool sees = (pos >= r.lo || (SINKS && pos < sinks)) && pos < r.hi;
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -266,10 +271,10 @@ __device__ __forceinline__ int split_parts(const PagedAttnArgs& a, int steps) {
   return min(max(steps / a.split_steps, 1), a.splits);
 }
 
-template <int D, bool FP8>
+template <int D, bool FP8, bool SINKS>
 __global__ __launch_bounds__(kPpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_prompt_kernel(PagedAttnArgs a) {
-  using Stage = PromptStage<D, FP8>;
+  using Stage = PromptStage<D, FP8, SINKS>;
   constexpr int NG = D / 32, KS = D / 16, PS = D + 4, kOps = KS + 2 * NG;
   extern __shared__ __align__(16) unsigned char smem[];
   _Float16* bufs = (_Float16*)smem;  // 2 x Stage::kBytes
@@ -300,8 +305,9 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   set_rows<kPpRows>(r, c, b, slot * kPpRows, a.rep, a.window, 0);
   const int rows = r.n * a.rep;
   if (slot < 0 || slot * kPpRows >= rows || (c.starts && rows <= kPaMostRows)) return;  // uniform
-  // the unit's steps, and this split's of them
-  int u0 = r.lo_any / kPpStep, u1 = (r.hi_any + kPpStep - 1) / kPpStep;
+  // the unit's steps, by their number in its span, and this split's of them
+  const typename Stage::Steps span(r.lo_any, r.hi_any, a.sinks);
+  int u0 = span.begin, u1 = span.begin + span.n;
   const int parts = split_parts(a, u1 - u0);
   if (split >= parts) return;  // uniform
   if (parts > 1) {
@@ -334,8 +340,7 @@ void paged_prompt_kernel(PagedAttnArgs a) {
 #pragma unroll
   for (int i = 0; i < NG; ++i) o[i] = f32x16{};
 
-  Stage st;
-  st.wave = wave;
+  Stage st(span, wave);
   auto buf = [&](int j) { return bufs + (j & 1) * (Stage::kBytes / 2); };
   // the scores of a step, 16 of a row on a lane: positions 8 (e / 4) + 4 half + e % 4
   auto scores = [&](f32x16& s, int j) {
@@ -353,8 +358,8 @@ void paged_prompt_kernel(PagedAttnArgs a) {
       ks[k] = Stage::lane_value(st.ks[k], u0 + j - st.base);
       ev[k] = Stage::lane_value(st.ev[k], u0 + j - st.base);
     }
-    const int p0 = (u0 + j) * kPpStep;
-    if (p0 < r.lo_all || p0 + kPpStep > r.hi_all) {
+    const int p0 = span.place(u0 + j) * kPpStep;
+    if ((p0 < r.lo_all && !(SINKS && p0 + kPpStep <= a.sinks)) || p0 + kPpStep > r.hi_all) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const bool bad = ks[k] != ks[k] || ev[k] != ev[k];
@@ -362,7 +367,7 @@ void paged_prompt_kernel(PagedAttnArgs a) {
         for (int e = 0; e < 8; ++e) {
           const int p = p0 + 16 * k + 8 * (e >> 2) + 4 * half + (e & 3);
           if (bad) s[8 * k + e] = __builtin_nanf("");
-          if (p < r.lo || p >= r.hi) s[8 * k + e] = -__builtin_inff();
+          if ((p < r.lo && !(SINKS && p < a.sinks)) || p >= r.hi) s[8 * k + e] = -__builtin_inff();
         }
         if (bad) {
           ks[k] = 1.f;
@@ -567,8 +572,8 @@ void paged_prompt_kernel(PagedAttnArgs a) {
   odd0 = min(min(odds[0][0], odds[0][1]), min(odds[0][2], odds[0][3]));
   odd1 = max(max(odds[1][0], odds[1][1]), max(odds[1][2], odds[1][3]));
   if (odd0 < odd1)
-    add_odd_values<D, FP8>(o, c, b, g, __builtin_amdgcn_readfirstlane(odd0),
-                           __builtin_amdgcn_readfirstlane(odd1), r);
+    add_odd_values<D, FP8, SINKS>(o, c, b, g, __builtin_amdgcn_readfirstlane(odd0),
+                           __builtin_amdgcn_readfirstlane(odd1), r, span, a.sinks);
   l += __shfl_xor(l, 32);
   if (!r.live) return;
   if (parts == 1) {
@@ -615,8 +620,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a) {
   set_rows<kPpRows>(r, c, b, slot * kPpRows, a.rep, a.window, rw);
   const int rows = r.n * a.rep;
   if (slot < 0 || slot * kPpRows >= rows || (c.starts && rows <= kPaMostRows) || !r.live) return;
-  const int parts = split_parts(
-      a, (r.hi_any + kPpStep - 1) / kPpStep - r.lo_any / kPpStep);
+  const int parts = split_parts(a, Span<kPpStep, true>(r.lo_any, r.hi_any, a.sinks).n);
   if (parts == 1) return;
   const int d4 = 4 * (threadIdx.x % (D / 4));
   const float* p = a.part + (((int64_t)slot0 * c.Hk + g) * a.splits * kPpRows + rw) * PS;
@@ -688,8 +692,12 @@ int paged_prompt_launch(PagedAttnArgs a, int head_dim, hipStream_t stream) {
   a.slots_each = a.c.starts ? 0 : (int)(s.slots / a.c.B);
   a.splits = s.splits;
   a.split_steps = s.split_steps;
-  // no context that needs splitting
-  const int64_t steps = (((int64_t)a.c.max_pages << a.c.page_shift) + kPpStep - 1) / kPpStep;
+  // no context that needs splitting: a unit's tokens see the page table's
+  // positions, or a window's each and the sinks
+  int64_t steps = (((int64_t)a.c.max_pages << a.c.page_shift) + kPpStep - 1) / kPpStep;
+  if (a.window > 0)
+    steps = std::min(steps, ((int64_t)a.window + kPpRows / a.rep + 1) / kPpStep + 2 +
+                                (a.sinks + kPpStep - 1) / kPpStep);
   if (steps < 2 * s.split_steps) a.splits = 1;
   const int64_t grid = s.slots * a.c.Hk * a.splits;
   // A CU holds workgroups i and i + 256: where nothing comes after them, the
@@ -702,12 +710,17 @@ int paged_prompt_launch(PagedAttnArgs a, int head_dim, hipStream_t stream) {
             "paged prompt parts do not fit their scratch");
   GLQ_CHECK(s.slots * 16 < (1ll << 24) && grid < (1ll << 24), "batch of too many query rows");
   const bool fp8 = a.c.ks != nullptr, wide = head_dim == 128;
-  auto kern = wide ? (fp8 ? paged_prompt_kernel<128, true> : paged_prompt_kernel<128, false>)
-                   : (fp8 ? paged_prompt_kernel<64, true> : paged_prompt_kernel<64, false>);
-  const size_t lds = 2 * (wide ? PromptStage<128, true>::kBytes : PromptStage<64, true>::kBytes);
-  static size_t attr[2] = {0, 0};
+  const auto pick = [&](auto sinks_) {
+    constexpr bool S = decltype(sinks_)::value;
+    return wide ? (fp8 ? paged_prompt_kernel<128, true, S> : paged_prompt_kernel<128, false, S>)
+                : (fp8 ? paged_prompt_kernel<64, true, S> : paged_prompt_kernel<64, false, S>);
+  };
+  auto kern = a.sinks > 0 ? pick(std::true_type()) : pick(std::false_type());
+  const size_t lds =
+      2 * (wide ? PromptStage<128, true, false>::kBytes : PromptStage<64, true, false>::kBytes);
+  static size_t attr[4] = {0, 0, 0, 0};
   if (wide)
-    if (int rc = set_lds_limit(kern, lds, attr[fp8])) return rc;
+    if (int rc = set_lds_limit(kern, lds, attr[(a.sinks > 0) * 2 + fp8])) return rc;
   kern<<<dim3((unsigned)grid), dim3(kPpThreads), lds, stream>>>(a);
   GLQ_LAUNCH_CHECK("paged_prompt_kernel");
   if (a.splits > 1) {

@@ -276,11 +276,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     starts: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
                     v_scales: torch.Tensor | None = None, window: int = 0,
                     out: torch.Tensor | None = None,
-                    workspace: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+                    workspace: tuple[torch.Tensor, torch.Tensor] | None = None,
+                    sinks: int = 0) -> torch.Tensor:
     """Causal attention of the new tokens' q (T, Hq, D) fp16 (paged_append's
     result) over their sequences' pages -> (T, Hq*D) fp16 (glq_paged_attention).
     The token at position p attends to (p - window, p], or [0, p] with window
-    0; scale may be 0 or negative.  Scores, softmax and sums are fp32, the
+    0, and to the sequence's first `sinks` positions up to its own; pages that
+    lie between need not be there (id -1).  scale may be 0 or negative.  Scores, softmax and sums are fp32, the
     weights in the product with V fp16.  `out` (apart from q): rows behind
     starts[B] keep what they held.  `workspace`: from paged_attention_workspace;
     None takes one of the stream's, or under graph capture one of the call's own,
@@ -298,8 +300,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Hq = width // D
     if Hq == 0 or Hq % Hk:
         raise RuntimeError(f"q's heads ({Hq}) must be a multiple of the KV heads ({Hk})")
-    if window < 0:
-        raise RuntimeError("window must be >= 0 (0: none)")
+    if window < 0 or sinks < 0:
+        raise RuntimeError("window and sinks must be >= 0 (0: none)")
     if out is None:
         out = q.new_empty((T, width))
     else:
@@ -319,5 +321,5 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _check(scratch, "workspace's scratch", dev, torch.uint8)
     _launch(lib.glq_paged_attention, "glq_paged_attention", _attention_params(
         *cache, _ptr(starts), T, q.data_ptr(), out.data_ptr(), Hq, window, counters.data_ptr(),
-        scratch.data_ptr(), counters.numel(), scratch.numel(), scale, 0), dev)
+        scratch.data_ptr(), counters.numel(), scratch.numel(), scale, min(sinks, 0x7FFFFFFF)), dev)
     return out

@@ -808,13 +808,14 @@ int glq_paged_append(const glq_paged_append_params* p, void* stream);
 
 /*
  * Causal attention of the new tokens over the cache (after glq_paged_append):
- * the row of q at position p of its sequence attends to positions
- * (p - window, p], window 0: [0, p]:
+ * the row of q at position p of its sequence attends to the positions of
+ * (p - window, p] and of [0, min(sinks, p + 1)), window 0: [0, p]:
  *   out[t][h*D + d] = fp16(sum_p softmax_p(scale * q.k_p) v_p[d]),
  * KV head h / (q_heads / kv_heads), scale of either sign or 0; fp32 scores,
  * softmax and sums, but for the softmax's weights in the product with V, which
  * are fp16 (2^-11 of each).  A row without positions (p < 0) is 0; one past the
- * page table NaN.  q (tokens, q_heads, head_dim) fp16, out (tokens, q_heads *
+ * page table NaN.  Pages between the sinks and the windows of a sequence's new
+ * tokens need not be there (an id outside [0, pages)).  q (tokens, q_heads, head_dim) fp16, out (tokens, q_heads *
  * head_dim) apart from it.  The workspace's sizes never shrink with seqs or
  * tokens; a workspace serves smaller calls too: the
  * counters (glq_paged_attention_counter_bytes) are zero before their first use
@@ -833,7 +834,7 @@ typedef struct glq_paged_attention_params {
   void *counters, *scratch;
   int64_t counter_bytes, scratch_bytes;
   float scale;
-  int32_t reserved;
+  int32_t sinks;
 } glq_paged_attention_params;
 
 int64_t glq_paged_attention_counter_bytes(int64_t seqs, int64_t tokens, int64_t q_heads,
