@@ -99,6 +99,27 @@ class PagedAttentionParams(ctypes.Structure):
     ]
 
 
+class PagedPools(ctypes.Structure):
+    """glq_paged_pools (include/glorcq_hip.h), field for field."""
+    _fields_ = [*[(n, _vp) for n in ("k_pages", "v_pages", "k_scales", "v_scales")],
+                ("pages", _i64)]
+
+
+class PagedCopyParams(ctypes.Structure):
+    """glq_paged_copy_params (include/glorcq_hip.h), field for field."""
+    _fields_ = [("from_", PagedPools), ("to", PagedPools),
+                *[(n, _i64) for n in ("layers", "kv_heads", "head_dim", "page_size")],
+                *[(n, _vp) for n in ("src", "dst", "tokens")], ("pairs", _i64)]
+
+
+class BeamSelectParams(ctypes.Structure):
+    """glq_beam_select_params (include/glorcq_hip.h), field for field."""
+    _fields_ = [("logits", _vp), ("scores", _vp),
+                *[(n, _i64) for n in ("prompts", "beams", "vocab", "row_stride", "num")],
+                *[(n, _vp) for n in ("out_scores", "out_parents", "out_tokens", "workspace")],
+                ("workspace_bytes", _i64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); must match include/glorcq_hip.h exactly.
 SIGNATURES = {
     "glq_version": (_c_int, []),
@@ -262,6 +283,9 @@ SIGNATURES = {
     "glq_paged_attention_counter_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "glq_paged_attention_scratch_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "glq_paged_attention": (_c_int, [_vp, _vp]),         # params, stream
+    "glq_paged_copy": (_c_int, [_vp, _vp]),              # params, stream
+    "glq_beam_select_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "glq_beam_select": (_c_int, [_vp, _vp]),             # params, stream
 }
 
 _lib = None

@@ -1065,7 +1065,8 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 # the paged key/value cache (it uses the checks and workspaces above)
 from .paged import (paged_append, paged_attention, paged_attention_workspace,  # noqa: E402
-                    paged_cache_tensors)
+                    paged_cache_tensors, paged_copy)
+from .beam import beam_select  # noqa: E402
 
 __all__ += ["paged_append", "paged_attention", "paged_attention_workspace",
-            "paged_cache_tensors"]
+            "paged_cache_tensors", "paged_copy", "beam_select"]

@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from array import array
 
 import torch
 
@@ -38,8 +39,10 @@ _FP8, _FP16, _E8M0 = torch.float8_e4m3fn, torch.float16, torch.float8_e8m0fnu
 _CACHE = "6P7q"
 _append_params = struct.Struct(_CACHE + "Pq3P5q4PqPfi").pack
 _attention_params = struct.Struct(_CACHE + "Pq2P2q2P2qfi").pack
+_copy_params = struct.Struct("4Pq4Pq4q3Pq").pack
 assert struct.calcsize(_CACHE + "Pq3P5q4PqPfi") == ctypes.sizeof(_lib.PagedAppendParams)
 assert struct.calcsize(_CACHE + "Pq2P2q2P2qfi") == ctypes.sizeof(_lib.PagedAttentionParams)
+assert struct.calcsize("4Pq4Pq4q3Pq") == ctypes.sizeof(_lib.PagedCopyParams)
 
 # attention counters: (device index, stream handle) -> zero-filled uint8 tensor
 _counters: dict = {}
@@ -47,9 +50,11 @@ _ws_bytes: dict = {}
 
 
 def paged_cache_tensors(pages: int, kv_heads: int, head_dim: int = 128, page_size: int = 64,
-                        dtype: torch.dtype = torch.float8_e4m3fn, device="cuda"):
+                        dtype: torch.dtype = torch.float8_e4m3fn, device="cuda",
+                        layers: int | None = None):
     """Zero-filled (k_pages, v_pages, k_scales, v_scales) of one layer's cache
-    (the scales None for fp16 pages)."""
+    (the scales None for fp16 pages), or of `layers` layers, one behind the other
+    (layers, pages, ...)."""
     if page_size < BLOCK or page_size > 1024 or page_size & (page_size - 1):
         raise RuntimeError(f"page_size must be a power of two in [16, 1024] (got {page_size})")
     if dtype not in (torch.float16, torch.float8_e4m3fn):
@@ -58,14 +63,15 @@ def paged_cache_tensors(pages: int, kv_heads: int, head_dim: int = 128, page_siz
     size = 1 if dtype == torch.float8_e4m3fn else 2
 
     def zeros(*shape):  # (fp8 types have no fill of their own everywhere)
-        return torch.zeros(*shape[:-1], shape[-1] * size, dtype=torch.uint8,
+        return torch.zeros(*stack, *shape[:-1], shape[-1] * size, dtype=torch.uint8,
                            device=device).view(dtype)
 
+    stack = () if layers is None else (layers,)
     k = zeros(pages, kv_heads, page_size, head_dim)
     v = zeros(pages, kv_heads, blocks, head_dim, BLOCK)
     if size == 2:
         return k, v, None, None
-    ks, vs = (torch.zeros(pages, kv_heads, blocks, dtype=torch.uint8, device=device)
+    ks, vs = (torch.zeros(*stack, pages, kv_heads, blocks, dtype=torch.uint8, device=device)
               .view(torch.float8_e8m0fnu) for _ in range(2))
     return k, v, ks, vs
 
@@ -323,3 +329,74 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         *cache, _ptr(starts), T, q.data_ptr(), out.data_ptr(), Hq, window, counters.data_ptr(),
         scratch.data_ptr(), counters.numel(), scratch.numel(), scale, min(sinks, 0x7FFFFFFF)), dev)
     return out
+
+
+def _pools(k_pages, v_pages, k_scales, v_scales, name):
+    """Pools of one layer or of several: (the C ABI's 5 values, layers, KV heads,
+    head width, page size, type, device index)."""
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() not in (4, 5):
+        raise RuntimeError(f"{name}: k_pages must be ([layers,] pages, Hk, page, D)")
+    dtype, dev = k_pages.dtype, k_pages.get_device()
+    if dtype is not _FP8 and dtype is not _FP16:
+        raise RuntimeError(f"{name}: k_pages must be float16 or float8_e4m3fn (got {dtype})")
+    if dev < 0:
+        raise RuntimeError(f"{name}: k_pages must be a GPU tensor (glorcq_amd runs on the GPU only)")
+    _check(k_pages, "k_pages", dev, dtype)
+    _check(v_pages, "v_pages", dev, dtype)
+    *stack, pages, Hk, page, D = k_pages.shape
+    blocks = (*stack, pages, Hk, page // BLOCK)
+    if v_pages.shape != (*blocks, D, BLOCK):
+        raise RuntimeError(f"{name}: v_pages must be {(*blocks, D, BLOCK)}")
+    if dtype is _FP16:
+        if k_scales is not None or v_scales is not None:
+            raise RuntimeError(f"{name}: fp16 pages have no scales")
+    else:
+        for s, n in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            if s is None:
+                raise RuntimeError(f"{name}: 8-bit pages need {n}")
+            _check(s, n, dev, _E8M0)
+            if s.shape != blocks:
+                raise RuntimeError(f"{name}: {n} must be {blocks}")
+    return ((k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), pages),
+            (stack[0] if stack else 1, Hk, D, page), dtype, dev)
+
+
+def _numbers(x, name):
+    try:
+        if isinstance(x, torch.Tensor):
+            if x.is_cuda:
+                raise RuntimeError(f"{name} must be in host memory")
+            x = x.tolist()
+        return array("i", x)
+    except (TypeError, OverflowError) as e:
+        raise RuntimeError(f"{name} must hold page or token numbers: {e}") from None
+
+
+def paged_copy(k_pages: torch.Tensor, v_pages: torch.Tensor, src, dst,
+               k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
+               tokens=None, to=None) -> None:
+    """Copies pages in all layers at once, one launch for 256 of them
+    (glq_paged_copy): page dst[i] becomes page src[i], the blocks of its first
+    tokens[i] tokens (None: all of it).  Pools are one layer's, or those of
+    several, one behind the other (layers, pages, ...); `to`: (k_pages, v_pages,
+    k_scales, v_scales) of the same layers and heads that get the pages, None:
+    the pools themselves.  src, dst and tokens are lists of numbers on the host
+    (a captured copy copies the same pages at every replay); a page must not be
+    written twice, nor written and read."""
+    lib = _lib.load()
+    pools, shape, dtype, dev = _pools(k_pages, v_pages, k_scales, v_scales, "pools")
+    into = pools
+    if to is not None:
+        if len(to) != 4:
+            raise RuntimeError("to must be (k_pages, v_pages, k_scales, v_scales)")
+        into, *like = _pools(*to, "to")
+        if like != [shape, dtype, dev]:
+            raise RuntimeError("to must have the layers, heads, page size, type and GPU of the pools")
+    src, dst = _numbers(src, "src"), _numbers(dst, "dst")
+    tokens = None if tokens is None else _numbers(tokens, "tokens")
+    n = len(src)
+    if len(dst) != n or (tokens is not None and len(tokens) != n):
+        raise RuntimeError("src, dst and tokens must be of one length")
+    _launch(lib.glq_paged_copy, "glq_paged_copy", _copy_params(
+        *pools, *into, *shape, src.buffer_info()[0], dst.buffer_info()[0],
+        0 if tokens is None else tokens.buffer_info()[0], n), dev)

@@ -843,6 +843,63 @@ int64_t glq_paged_attention_scratch_bytes(int64_t seqs, int64_t tokens, int64_t 
                                           int64_t kv_heads);
 int glq_paged_attention(const glq_paged_attention_params* p, void* stream);
 
+/*
+ * Copies pages, in all layers of a cache at once: page dst[i] of `to` becomes
+ * page src[i] of `from`, its first ceil(tokens[i] / 16) blocks (tokens NULL: all
+ * of it; 0: none), scales with them.  A cache's pools are those of its layers
+ * one behind the other, (layers, pages, ...).  src, dst and tokens are `pairs`
+ * int32 in HOST memory, read before the call returns (a captured graph copies
+ * the same pages at every replay).  Refused: page numbers out of range, a page
+ * that is written twice, and, where from and to are one cache, a page that is
+ * both written and read; two caches must not share memory.
+ */
+typedef struct glq_paged_pools {
+  void* k_pages;
+  void* v_pages;
+  void* k_scales;  /* NULL with v_scales: fp16 pages */
+  void* v_scales;
+  int64_t pages;   /* of a layer */
+} glq_paged_pools;
+
+typedef struct glq_paged_copy_params {
+  glq_paged_pools from, to;
+  int64_t layers, kv_heads, head_dim, page_size;
+  const int32_t *src, *dst, *tokens;
+  int64_t pairs;
+} glq_paged_copy_params;
+
+int glq_paged_copy(const glq_paged_copy_params* p, void* stream);
+
+/*
+ * The best continuations of each of `prompts` prompts over its `beams` beams and
+ * the vocabulary:
+ *   c[b][k][v] = scores[b][k] + x[b][k][v] - log sum_u exp(x[b][k][u]),
+ * x rows of `vocab` logits (dtype 0: fp16, 1: bf16, 2: fp32), row_stride values
+ * apart, beam after beam; scores (prompts, beams) fp32.  The `num` largest of
+ * each prompt in falling order, the lowest k vocab + v first among equal ones,
+ * compared in fp64 (to 1e-10): out_scores (prompts, num) fp32, out_parents and
+ * out_tokens (prompts, num) int64, their k and v.  A logit or a score of -inf
+ * makes -inf, which is chosen after everything else; all continuations of a beam
+ * with a NaN or +inf among its logits or as its score are NaN, which are chosen
+ * before everything else.  beams <= 64, num <= 128, num <= beams * vocab.  The
+ * workspace (glq_beam_select_workspace_bytes, negative for invalid sizes;
+ * 16-byte aligned) needs no initialisation.
+ */
+typedef struct glq_beam_select_params {
+  const void* logits;
+  const float* scores;
+  int64_t prompts, beams, vocab, row_stride, num;
+  float* out_scores;
+  int64_t *out_parents, *out_tokens;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t dtype;
+  int32_t reserved;
+} glq_beam_select_params;
+
+int64_t glq_beam_select_workspace_bytes(int64_t prompts, int64_t beams, int64_t vocab, int64_t num);
+int glq_beam_select(const glq_beam_select_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
