@@ -116,8 +116,9 @@ class BeamSelectParams(ctypes.Structure):
     """glq_beam_select_params (include/glorcq_hip.h), field for field."""
     _fields_ = [("logits", _vp), ("scores", _vp),
                 *[(n, _i64) for n in ("prompts", "beams", "vocab", "row_stride", "num")],
-                *[(n, _vp) for n in ("out_scores", "out_parents", "out_tokens", "workspace")],
-                ("workspace_bytes", _i64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+                *[(n, _vp) for n in ("out_scores", "out_parents", "out_tokens", "counters",
+                                     "scratch")],
+                ("counter_bytes", _i64), ("scratch_bytes", _i64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 # name -> (restype, argtypes); must match include/glorcq_hip.h exactly.
@@ -284,7 +285,8 @@ SIGNATURES = {
     "glq_paged_attention_scratch_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "glq_paged_attention": (_c_int, [_vp, _vp]),         # params, stream
     "glq_paged_copy": (_c_int, [_vp, _vp]),              # params, stream
-    "glq_beam_select_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "glq_beam_select_counter_bytes": (_i64, [_i64, _i64]),
+    "glq_beam_select_scratch_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "glq_beam_select": (_c_int, [_vp, _vp]),             # params, stream
 }
 

@@ -10,13 +10,15 @@ import struct
 import torch
 
 from .. import _lib
-from . import workspace as _stream_scratch
-from .paged import _check, _launch
+from . import _zeroed_buffer, workspace as _stream_scratch
+from .paged import _check, _launch, _new_workspace
 
-_FORMAT = "2P5q4Pq2i"
+_FORMAT = "2P5q5P2q2i"
 _params = struct.Struct(_FORMAT).pack
 assert struct.calcsize(_FORMAT) == ctypes.sizeof(_lib.BeamSelectParams)
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+# counters: (device index, stream handle) -> zero-filled uint8 tensor
+_counters: dict = {}
 _ws_bytes: dict = {}
 
 
@@ -52,16 +54,19 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num: int):
         raise RuntimeError("logits must have contiguous rows, the same distance apart")
     need = _ws_bytes.get((B, K, V, num))
     if need is None:
-        need = lib.glq_beam_select_workspace_bytes(B, K, V, num)
-        if need >= 0:
-            _ws_bytes[(B, K, V, num)] = need
-    out = scores.new_empty((B, max(num, 0)))
-    parents, tokens = torch.empty((2, B, max(num, 0)), dtype=torch.int64, device=scores.device)
+        need = (max(lib.glq_beam_select_counter_bytes(B, K), 1),
+                max(lib.glq_beam_select_scratch_bytes(B, K, V, num), 1))
+        _ws_bytes[(B, K, V, num)] = need
+    n = max(num, 0)
+    out = scores.new_empty((B, n))
+    parents, tokens = torch.empty((2, B, n), dtype=torch.int64, device=scores.device)
     if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=scores.device)
+        counters, scratch = _new_workspace(need, scores.device)
     else:
-        ws = _stream_scratch(scores.device, max(need, 1))
+        counters = _zeroed_buffer(_counters, scores.device, need[0])
+        scratch = _stream_scratch(scores.device, need[1])
     _launch(lib.glq_beam_select, "glq_beam_select", _params(
         logits.data_ptr(), scores.data_ptr(), B, K, V, row, num, out.data_ptr(),
-        parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), dtype, 0), dev)
+        parents.data_ptr(), tokens.data_ptr(), counters.data_ptr(), scratch.data_ptr(),
+        counters.numel(), scratch.numel(), dtype, 0), dev)
     return out, parents, tokens

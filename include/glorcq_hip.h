@@ -881,9 +881,11 @@ int glq_paged_copy(const glq_paged_copy_params* p, void* stream);
  * out_tokens (prompts, num) int64, their k and v.  A logit or a score of -inf
  * makes -inf, which is chosen after everything else; all continuations of a beam
  * with a NaN or +inf among its logits or as its score are NaN, which are chosen
- * before everything else.  beams <= 64, num <= 128, num <= beams * vocab.  The
- * workspace (glq_beam_select_workspace_bytes, negative for invalid sizes;
- * 16-byte aligned) needs no initialisation.
+ * before everything else.  beams <= 64, num <= 128, num <= beams * vocab.  Outputs
+ * must not overlap the logits or the scores.  The counters (.._counter_bytes) are
+ * zero before their first use and left zero by each call; the scratch
+ * (.._scratch_bytes, 16-byte aligned) needs no initialisation (both negative for
+ * invalid sizes).  Calls that share either must not overlap.
  */
 typedef struct glq_beam_select_params {
   const void* logits;
@@ -891,13 +893,14 @@ typedef struct glq_beam_select_params {
   int64_t prompts, beams, vocab, row_stride, num;
   float* out_scores;
   int64_t *out_parents, *out_tokens;
-  void* workspace;
-  int64_t workspace_bytes;
+  void *counters, *scratch;
+  int64_t counter_bytes, scratch_bytes;
   int32_t dtype;
   int32_t reserved;
 } glq_beam_select_params;
 
-int64_t glq_beam_select_workspace_bytes(int64_t prompts, int64_t beams, int64_t vocab, int64_t num);
+int64_t glq_beam_select_counter_bytes(int64_t prompts, int64_t beams);
+int64_t glq_beam_select_scratch_bytes(int64_t prompts, int64_t beams, int64_t vocab, int64_t num);
 int glq_beam_select(const glq_beam_select_params* p, void* stream);
 
 #ifdef __cplusplus

@@ -172,6 +172,17 @@ def test_extreme_logits(gpu):
         assert torch.allclose(a.cpu().double(), rs, rtol=1e-6)
 
 
+def test_large_logits(gpu):
+    """Values beside which a shift by a few hundred rounds to nothing: of 3000
+    logits two count, so that each has a half."""
+    for size, tol in ((1e9, 1e-6), (1e12, 1e-3)):  # (fp64's steps there: 1e-7 and 1e-4)
+        x = torch.zeros(1, 3000, device=gpu)
+        x[0, 5], x[0, 2500] = size, size
+        a, _, t = kernels.beam_select(x, torch.full((1, 1), -1.0, device=gpu), 2)
+        assert t[0].tolist() == [5, 2500]
+        assert ((a[0].double() + 1 + math.log(2)).abs() < tol + 2.0 ** -23).all()
+
+
 def test_subnormal_logits_keep_their_order(gpu):
     x = torch.zeros(1, 3000, dtype=torch.float16, device=gpu)
     x[0, 2000], x[0, 1000], x[0, 500] = 3 * 2.0 ** -24, 2 * 2.0 ** -24, 2.0 ** -24

@@ -69,8 +69,8 @@ def test_copy_of_nothing(lib):
 
 def _beam(lib, **kw):
     a = dict(logits=P, scores=2 * P, prompts=2, beams=4, vocab=1000, row_stride=1000, num=8,
-             out_scores=3 * P, out_parents=4 * P, out_tokens=5 * P, workspace=6 * P,
-             workspace_bytes=1 << 20)
+             out_scores=3 * P, out_parents=4 * P, out_tokens=5 * P, counters=6 * P, scratch=7 * P,
+             counter_bytes=1 << 20, scratch_bytes=1 << 20)
     p = _lib.BeamSelectParams(**{**a, **kw})
     return lib.glq_beam_select(ctypes.byref(p), None), lib.glq_last_error()
 
@@ -84,8 +84,10 @@ def _beam(lib, **kw):
     (dict(logits=None), b"null"), (dict(scores=None), b"null"), (dict(out_tokens=None), b"null"),
     (dict(logits=P + 1), b"aligned"), (dict(logits=P + 2, dtype=2), b"aligned"),
     (dict(scores=P + 2), b"aligned"), (dict(out_parents=P + 4), b"aligned"),
-    (dict(workspace=None), b"workspace"), (dict(workspace_bytes=100), b"workspace"),
-    (dict(workspace=P + 8), b"workspace"), (dict(out_scores=2 * P), b"overlap"),
+    (dict(counters=None), b"workspace"), (dict(scratch=None), b"workspace"),
+    (dict(counter_bytes=4), b"workspace"), (dict(scratch_bytes=100), b"workspace"),
+    (dict(scratch=P + 8), b"workspace"), (dict(counters=P + 2), b"workspace"),
+    (dict(out_scores=P + 8000), b"overlap"), (dict(out_scores=2 * P), b"overlap"),
     (dict(out_tokens=2 * P + 24), b"overlap"), (dict(out_parents=2 * P - 120), b"overlap"),
 ])
 def test_beam_checks(lib, kw, what):
@@ -96,7 +98,9 @@ def test_beam_checks(lib, kw, what):
 def test_beam_of_nothing_and_workspace(lib):
     assert lib.glq_beam_select(None, None) == 1
     assert _beam(lib, prompts=0, logits=None)[0] == 0
-    size = lib.glq_beam_select_workspace_bytes
+    assert lib.glq_beam_select_counter_bytes(-1, 4) == lib.glq_beam_select_counter_bytes(1, 0) == -1
+    assert lib.glq_beam_select_counter_bytes(3, 4) >= 60
+    size = lib.glq_beam_select_scratch_bytes
     assert size(0, 4, 1000, 8) == 0 and 0 < size(1, 4, 1000, 8) <= size(8, 4, 1000, 8)
     for bad in ((-1, 4, 1000, 8), (1, 0, 1000, 8), (1, 65, 1000, 8), (1, 4, 0, 8), (1, 4, 1000, 0),
                 (1, 4, 1000, 129), (1, 4, 1 << 25, 8)):
