@@ -184,7 +184,8 @@ class GLoRCQQwen3Attention(nn.Module):
         qr = kernels.paged_append(k, v, kp, vp, cos=cos, sin=sin, q=q,
                                   q_norm_w=inner.q_norm.weight, k_norm_w=inner.k_norm.weight,
                                   eps=inner.q_norm.variance_epsilon, **at)
-        a = kernels.paged_attention(qr, kp, vp, scale=self.scaling, window=self.window,
+        window, sinks = step.visible(self.window)
+        a = kernels.paged_attention(qr, kp, vp, scale=self.scaling, window=window, sinks=sinks,
                                     workspace=step.workspace(qr), **at)
         return inner.o_proj(a).reshape(B, S, -1), None
 
