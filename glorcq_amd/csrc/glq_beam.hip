@@ -129,23 +129,25 @@ __device__ __forceinline__ double value_of(uint64_t k) {
 }
 
 
-// Of a wave: a number that q lanes' x are not below, the largest but for its last 12
-// bits; -inf where there are no such lanes.  (A bit a step, by counting lanes.)
-__device__ __forceinline__ float wave_nth(float x, int q) {
-  const uint32_t k = ordered(x);
-  uint32_t t = 0;
+// Of a wave: a number that q lanes' x are not below, the largest but for its last 16
+// bits, and -inf where there are no such lanes; the same of r lanes' y.  (A bit a
+// step, by counting lanes.)
+__device__ __forceinline__ float2 wave_nth(float x, int q, float y, int r) {
+  const uint32_t k = ordered(x), l = ordered(y);
+  uint32_t t = 0, u = 0;
 #pragma unroll
-  for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
+  for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
     if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(k >= (t | bit))) >= q) t |= bit;
-  return t > ordered(kNone) ? value_of(t) : kNone;
+    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(l >= (u | bit))) >= r) u |= bit;
+  }
+  return float2{t > ordered(kNone) ? value_of(t) : kNone, u > ordered(kNone) ? value_of(u) : kNone};
 }
-// Of a wave: at most the key of its num-th best, by its lanes' two largest keys.
-__device__ __forceinline__ float wave_least(int num, float mx, float second) {
-  return num <= 64 ? wave_nth(mx, num) : wave_nth(second, (num + 1) / 2);  // uniform
-}
-// The same, and that of which the waves of a workgroup have num together.
+// At most the key of a wave's num-th best, by its lanes' two largest keys; and a key
+// of which the waves of a workgroup have num together, at most the smallest of it.
 __device__ __forceinline__ float2 waves_least(int num, float mx, float second) {
-  return float2{wave_least(num, mx, second), wave_nth(mx, (num + kBmWaves - 1) / kBmWaves)};
+  const bool one = num <= 64;  // an element a lane will do
+  return wave_nth(one ? mx : second, one ? num : (num + 1) / 2, mx,
+                  (num + kBmWaves - 1) / kBmWaves);
 }
 // At most the key of the workgroup's num-th best, and above -inf.
 __device__ __forceinline__ float workgroup_least(const float2 (&of)[kBmWaves]) {
@@ -469,8 +471,8 @@ static_assert(2 * kBmMost <= kBmThreads, "as many places as may be taken and nee
 // A part's elements in LDS: 64-bit numbers that are larger for the better one,
 // the value's order above its place's.
 struct PartLds {
-  static constexpr int kMost = 64 * kBmEach + kBmMost;  // of a wave: a chunk's and the best before
-  uint64_t key[kBmWaves][kMost + 4];
+  static constexpr int kChunk = 64 * kBmEach, kMost = 768;  // of a wave: a chunk's, all
+  uint64_t key[kBmWaves][kMost + 4], kept[kBmWaves][kBmMost];
   float2 least[kBmWaves];
   int count[kBmWaves];
 };
@@ -481,29 +483,23 @@ __device__ __forceinline__ float next_up(float x) {
   return __uint_as_float((int)b < 0 ? b - 1 : b + 1);
 }
 
-// Keeps the num best of a wave's list of n keys, at its front.
-__device__ __noinline__ int keep_best(uint64_t* list, int n, int num) {
-  constexpr int R = (PartLds::kMost + 63) / 64;
+// Keeps the num best of a wave's list of n keys, at its front.  (Rare: values that
+// rise along the row.)
+__device__ __forceinline__ void keep_best(uint64_t* list, uint64_t* kept, int n, int num) {
   const int lane = threadIdx.x & 63;
   paged_lds_sync();
-  uint64_t key[R];
-  int rank[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    key[r] = lane + 64 * r < n ? list[lane + 64 * r] : 0;
-    rank[r] = 0;
-  }
-  for (int j = 0; j < n; ++j) {
-    const uint64_t o = list[j];
-#pragma unroll
-    for (int r = 0; r < R; ++r) rank[r] += o > key[r];
+#pragma unroll 1
+  for (int i = lane; i < n; i += 64) {
+    const uint64_t key = list[i];
+    int rank = 0;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) rank += list[j] > key;
+    if (rank < num) kept[rank] = key;
   }
   paged_lds_sync();
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (lane + 64 * r < n && rank[r] < num) list[rank[r]] = key[r];
+#pragma unroll 1
+  for (int i = lane; i < num; i += 64) list[i] = kept[i];
   paged_lds_sync();
-  return min(n, num);
 }
 
 // One workgroup a part of a row, in chunks of 2048 values that pass through
@@ -605,8 +601,10 @@ __global__ __launch_bounds__(kBmThreads) void beam_kernel(BeamArgs a) {
   float cut = -__FLT_MAX__;  // what is below is none of the best
   int mine = 0;              // keys of the wave's list
   auto collect = [&](int c) {
-    if (mine + kBmEach * __builtin_popcountll(__builtin_amdgcn_ballot_w64(mx >= cut)) > s.kMost)
-      mine = keep_best(s.key[wave], mine, num);
+    if (mine > s.kMost - s.kChunk) {
+      keep_best(s.key[wave], s.kept[wave], mine, num);
+      mine = num;
+    }
 #pragma unroll
     for (int e = 0; e < kBmEach; ++e) {
       const bool in = x[e] >= cut;
@@ -625,8 +623,8 @@ __global__ __launch_bounds__(kBmThreads) void beam_kernel(BeamArgs a) {
     const int hits = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mx >= cut));
     if (hits == 0) return;  // uniform
     float least = kNone;
-    if (hits > 24) {
-      least = wave_least(num, top1, top2);
+    if (2 * hits > num) {
+      least = waves_least(num, top1, top2).x;
       cut = fmaxf(cut, least);
     }
     collect(c);
