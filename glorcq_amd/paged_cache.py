@@ -279,7 +279,7 @@ class PagedStep:
     def visible(self, window: int) -> tuple[int, int]:
         """Window and sinks of a layer whose own window is this (0: none)."""
         c = self.cache
-        return (c.window, c.sinks) if c.window and not 0 < window <= c.window else (window, 0)
+        return (c.window, c.sinks) if c.window and not 0 < window < c.window else (window, 0)
 
     def workspace(self, q):
         # (a step whose sequences bring one token each, as decode steps do, is

@@ -109,6 +109,50 @@ def test_sorted_rows(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("num", [1, 16, 128])
+@pytest.mark.parametrize("how", ["random", "rising", "falling", "equal", "steps", "late", "masked",
+                                 "jumps"])
+def test_many_rows(gpu, dtype, num, how):
+    """Rows in parts of several chunks of 2048: what stands in a later chunk, or
+    only there; values that rise along the row, so that each chunk is better than
+    those before; equal ones; sums whose largest term comes 1000 above the rest."""
+    B, K, V = 12, 8, 49160
+    x, s = make(gpu, B, K, V, dtype, 16)
+    at = torch.arange(V, device=gpu, dtype=torch.float32)
+    if how in ("rising", "falling"):
+        x = ((at if how == "rising" else at.flip(0)) / 512 - 40).expand(B * K, -1)
+    elif how == "equal":
+        x = torch.full((B * K, V), 0.5, device=gpu)
+    elif how == "steps":
+        x = (at // 1000 % 7).expand(B * K, -1)
+    elif how == "late":
+        x = x.float() - 20 * (at < 47000)
+    elif how == "masked":  # all of the first chunks of every part
+        x = x.float().masked_fill((at % 6145) < 4500, -INF)
+    elif how == "jumps":
+        x = x.float() + 1000 * (at % 6145 > 6000) * (torch.arange(B * K, device=gpu) % 2)[:, None]
+    x = x.to(dtype).contiguous()
+    a, p, t = kernels.beam_select(x, s, num)
+    # the formula in fp64, on the GPU
+    y = x.double().view(B, K, V)
+    c = (s.double()[..., None] + torch.log_softmax(y, -1)).view(B, K * V)
+    v, i = c.sort(dim=1, descending=True, stable=True)
+    v, i = v[:, :num], i[:, :num]
+    assert torch.equal(p, i // V) and torch.equal(t, i % V)
+    assert ((a.double() - v).abs() <= 2.0 ** -24 * v.abs() + 1e-10).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nan_in_a_later_chunk(gpu, dtype):
+    x, s = make(gpu, 12, 8, 49160, dtype, 17)
+    x[3, 5000], x[11, 49159], x[20, 3000] = NAN, INF, -INF
+    a, p, t = kernels.beam_select(x, s, 6)
+    for b, k in ((0, 3), (1, 3)):
+        assert a[b].isnan().all() and (p[b] == k).all() and t[b].tolist() == list(range(6))
+    assert torch.isfinite(a[2:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("left", [0, 1, 5, 40, 3000])
 def test_masked(gpu, dtype, left):
     """Few tokens allowed (none, in some beams): -inf comes last, by place."""

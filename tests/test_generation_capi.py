@@ -95,6 +95,16 @@ def test_beam_checks(lib, kw, what):
     assert rc == 1 and what in msg
 
 
+def test_attention_refuses_negative_sinks(lib):
+    cache = _lib.PagedCache(k_pages=P, v_pages=P, page_table=P, lengths=P, seqs=2, max_pages=4,
+                            table_stride=4, pages=8, kv_heads=2, head_dim=128, page_size=64)
+    p = _lib.PagedAttentionParams(cache=cache, tokens=2, q=P, out=2 * P, q_heads=8, window=4,
+                                  sinks=-1, scale=1.0, counters=P, scratch=P,
+                                  counter_bytes=1 << 30, scratch_bytes=1 << 30)
+    assert lib.glq_paged_attention(ctypes.byref(p), None) == 1
+    assert b"sinks" in lib.glq_last_error()
+
+
 def test_beam_of_nothing_and_workspace(lib):
     assert lib.glq_beam_select(None, None) == 1
     assert _beam(lib, prompts=0, logits=None)[0] == 0

@@ -137,6 +137,7 @@ def test_window_frees_pages(window, sinks):
     # (the 33 tokens of one step see no less than window + 32 positions)
     assert most <= -(-sinks // 16) + (window + 33) // 16 + 3
     assert PagedStep(c).visible(0) == (window, sinks)
+    assert PagedStep(c).visible(window) == (window, sinks)
     assert PagedStep(c).visible(window + 1) == (window, sinks)
     if window > 1:
         assert PagedStep(c).visible(window - 1) == (window - 1, 0)
