@@ -26,9 +26,8 @@ constexpr float kNone = -__builtin_inff();
 // e^d for |d| < 700, in fp64 and to 6e-11: 2^(n + f), n from the low bits
 // of d log2(e) + 1.5 2^52, 2^f by its Chebyshev series of degree 7 on [-1/2, 1/2].
 // Two continuations of different beams compare by sums over the vocabulary, so
-// fp32 (1e-7) would put some in the wrong order; the vector fp64 rate is that of
-// unpacked fp32.
-// N of them side by side, so that one has not to wait for itself.
+// fp32 (1e-7) would put some in the wrong order; fp64 fma runs at fp32's rate
+// (5.2 and 4.7 cycles a wave's).  N side by side, so that none waits for itself.
 template <int N>
 __device__ __forceinline__ void exp_of(double (&d)[N]) {
   constexpr double kLog2e = 1.4426950408889634, kBig = 6755399441055744.0;
@@ -506,11 +505,10 @@ __device__ __forceinline__ void keep_best(uint64_t* list, uint64_t* kept, int n,
 // registers, so that memory is read once: the sum of its exponentials, and its
 // best.  The last workgroup of a prompt to arrive goes on with all of its parts'.
 //
-// Many rows are bound by the vector unit: 26 instructions a value, 14 of them the
-// exponential's fp64 ones: 128 rows of 151936 fp16 values 34 us (16 of them the
-// chunks' instructions at a full rate; a copy would take 8).  Few rows are bound
-// by the way of one part, a row's and a prompt's last workgroup, about 2 us each:
-// 4 rows 12.4 us with the launch.
+// Many rows are bound by instructions: 30 vector ones a value, 15 of them fp64,
+// and the cut's scalar ones: 128 rows of 151936 fp16 values 31 us (1.2 TB/s; a
+// copy's rate would be 8).  Few rows are bound by the way of one part (5 us) and
+// of a prompt's last workgroup (5 us): 4 rows 11.9 us with the launch.
 //
 // A thread sums its exponentials over the first value that it saw (or a later one
 // 600 above it: fp64 has the room).  A wave collects what is not below the num-th
@@ -732,7 +730,7 @@ constexpr int64_t kBmFew = 256, kBmMany = 1024;
 // Parts of a row and their length, in chunks: so many workgroups as the card holds
 // at once, but two chunks each where a CU would get a second workgroup.  4 rows of
 // 151936 values: 11.6 us in parts of two chunks, 13.3 of one; 128 rows 34 us in 8
-// parts each, 36 in 7, 10 or 15.
+// parts each, 36 in 7, 10 or 15 (both of one build, before the last ones).
 void beam_parts(int64_t rows, int64_t vocab, int64_t& parts, int64_t& part) {
   const int64_t chunk = kBmThreads * kBmEach, chunks = (vocab + chunk - 1) / chunk;
   const int64_t all = std::max<int64_t>(rows, 1) * chunks;

@@ -32,6 +32,10 @@ struct CopyArgs {
 // 8 KB of a run, 8 loads of 16 bytes a lane in flight, and the first piece's
 // wave the run's scales.  Everything but a lane's constant offset is uniform:
 // the grid is (pieces of k and v, layers, pairs), and the pairs are arguments.
+//
+// Bound by memory: 97 pages of 24 layers to another pool (1.2 GB read and written)
+// 240 us, 5.1 TB/s, what a large copy reaches; 56 part pages of 48 layers 39 us.
+// Three part pages of 48 layers: 4.2 us, a launch.
 __global__ __launch_bounds__(kCpThreads) void paged_copy_kernel(CopyArgs a) {
   constexpr int N = kCpPiece / 1024;
   const int lane = threadIdx.x & 63;
