@@ -64,12 +64,9 @@ __device__ __forceinline__ double below(float a, float b) {
 
 // An element: its value and its place k 2^24 + v; the better one has the larger
 // value, or the lower place.
-template <class V>
 struct Element {
-  V v;
+  float v;
   uint32_t at;
-  // (without branches: both are in registers, or read at once)
-  __device__ bool over(const Element& b) const { return (v > b.v) | ((v == b.v) & (at < b.at)); }
 };
 
 // x of the lane o away (o = 1, 2, 16, 32) or of one of the other half of 2 o
@@ -130,7 +127,6 @@ __device__ __forceinline__ double value_of(uint64_t k) {
   return __builtin_bit_cast(double, k ^ (k >> 63 ? 0x8000000000000000ull : ~0ull));
 }
 
-
 // Of a wave: a number that q lanes' x are not below, the largest but for its last 16
 // bits, and -inf where there are no such lanes; the same of r lanes' y.  (A bit a
 // step, by counting lanes.)
@@ -166,6 +162,67 @@ __device__ __forceinline__ float workgroup_least(const float2 (&of)[kBmWaves]) {
 __device__ __forceinline__ int place_in(uint64_t mask) {
   return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
                                         __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// Keeps the num best of a wave's list of n > num keys (PLACES: of the same ones the
+// lowest in `at`), at its front, and returns what the others' keys were below, or the
+// num-th key: a bit a step, by counting lanes.  (Values that rise along the row or
+// are mostly the same, beams far apart, num above 64.  By comparing all pairs 128
+// rows of 151936 values, most of them -65504, took 1970 us, now 50.)
+template <int MOST, bool PLACES>
+__device__ __forceinline__ uint64_t keep_best(uint64_t* list, uint32_t* at, int n, int num) {
+  constexpr int kEach = MOST / 64;
+  const int lane = threadIdx.x & 63;
+  paged_lds_sync();
+  uint64_t key[kEach];
+  uint32_t place[kEach];  // (its complement)
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    key[i] = i * 64 + lane < n ? list[i * 64 + lane] : 0;
+    if constexpr (PLACES) place[i] = i * 64 + lane < n ? ~at[i * 64 + lane] : 0;
+  }
+  uint64_t t = 0;
+  int count = n;  // not below t
+#pragma unroll 1
+  for (uint64_t bit = 1ull << 63; bit && count > num; bit >>= 1) {
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] >= (t | bit)));
+    if (above >= num) {
+      t |= bit;
+      count = above;
+    }
+  }
+  uint32_t u = 0;  // of the keys that are t
+  if constexpr (PLACES) {
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit && count > num; bit >>= 1) {
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(
+            (key[i] > t) | ((key[i] == t) & (place[i] >= (u | bit)))));
+      if (above >= num) {
+        u |= bit;
+        count = above;
+      }
+    }
+  }
+  int kept = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    bool in = key[i] >= t;
+    if constexpr (PLACES) in = (key[i] > t) | ((key[i] == t) & (place[i] >= u));
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+    if (in) {
+      list[kept + place_in(mask)] = key[i];
+      if constexpr (PLACES) at[kept + place_in(mask)] = ~place[i];
+    }
+    kept += __builtin_popcountll(mask);
+  }
+  paged_lds_sync();
+  return t;
 }
 
 // Ranks the waves' lists (n[w] keys, behind them four zeros) as one: put(rank, w,
@@ -215,89 +272,77 @@ struct LastLds {
   uint64_t key[kBmWaves][kMost + 4];
   uint32_t at[kBmWaves][kMost + 4];
   float2 least[kBmWaves];
-  Element<double> best[kBmWaves];
   int count[kBmWaves];
 };
 
 // The num best of the workgroup's elements above -inf, each passed with its rank
-// to `put` by one thread; returns how many there are (num at most).  each(f)
-// calls f(value, place) for every element of a thread, the same ones each time;
-// `mx`: the largest key of a thread's elements, key(v) a float that never falls
-// where v grows, and above -inf where v is.
+// to `put` by one thread; returns how many there are (num at most).  each(add)
+// calls add(value, place, whether the list may be full) for all elements that matter,
+// a wave at a time; it returns whether the wave has taken any, and where it has not
+// there is no need to call it with lower ones.  `mx`: the largest key of some of a
+// thread's elements, key(v) a float that never falls where v grows, and above -inf
+// where v is.
 //
 // What is not below the num-th of the lanes' best (of a wave, or a quarter of them
 // in each), not many more elements than num of random ones, is collected in LDS, a
-// list a wave, and ranked by counting.  Where that does not fit (values most of
-// which are equal), the best are taken one by one.
+// list a wave, and ranked by counting.  A list that is full keeps its num best.
 template <class Each, class Key, class Put>
-__device__ int top_n(int num, LastLds& s, float mx, Each each, Key key, Put put) {
-  using E = Element<double>;
-  const int tid = threadIdx.x, wave = tid >> 6;
+__device__ __forceinline__ int top_n(int num, LastLds& s, float mx, Each each, Key key, Put put) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float2 least_of = waves_least(num, mx, kNone);
-  if ((tid & 63) == 0) s.least[wave] = least_of;
+  if (lane == 0) s.least[wave] = least_of;
   __syncthreads();
   const float least = workgroup_least(s.least);
+  uint64_t low = 0;
   int mine = 0;  // uniform
-  each([&](double v, uint32_t at) {
-    const bool in = key(v) >= least;
+  auto add = [&](double v, uint32_t at, bool may_fill) {
+    const bool in = (key(v) >= least) & (ordered(v) >= low);
     const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-    if (mask) {
-      const int i = mine + place_in(mask);
-      if (in && i < s.kMost) {
-        s.key[wave][i] = ordered(v);
-        s.at[wave][i] = at;
-      }
-      mine += __builtin_popcountll(mask);
+    if (!mask) return false;
+    if (may_fill && __builtin_expect(mine > s.kMost - 64, 0)) {
+      low = keep_best<LastLds::kMost, true>(s.key[wave], s.at[wave], mine, num);
+      mine = num;
     }
-  });
-  if ((tid & 63) < 4 && mine <= s.kMost) s.key[wave][mine + (tid & 3)] = 0;
-  if ((tid & 63) == 0) s.count[wave] = mine;
+    if (in) {
+      const int i = mine + place_in(mask);
+      s.key[wave][i] = ordered(v);
+      s.at[wave][i] = at;
+    }
+    mine += __builtin_popcountll(mask);
+    return true;
+  };
+  each(add);
+  if (__builtin_expect(mine > max(num, 64), 0)) {
+    keep_best<LastLds::kMost, true>(s.key[wave], s.at[wave], mine, num);
+    mine = num;
+  }
+  if (lane < 4) s.key[wave][mine + lane] = 0;
+  if (lane == 0) s.count[wave] = mine;
   __syncthreads();
-  int n[kBmWaves], all = 0, most = 0;
+  int n[kBmWaves], all = 0;
 #pragma unroll
   for (int w = 0; w < kBmWaves; ++w) {
     n[w] = __builtin_amdgcn_readfirstlane(s.count[w]);
     all += n[w];
-    most = max(most, n[w]);
   }
-  if (most <= s.kMost) {
-    rank_lists(
-        s.key, n, all,
-        [&](int w, int i, int of, int len, int same) {
-          int better = 0;
-          same += (int)other_half<1>((uint32_t)same);
-          same += (int)other_half<2>((uint32_t)same);
-          if (__builtin_amdgcn_ballot_w64(same > 1))  // equal values: by place
-            for (int j = 0; j < len; ++j)
-              better += (s.key[of][j] == s.key[w][i]) & (s.at[of][j] < s.at[w][i]);
-          return better;
-        },
-        [&](int rank, int w, int i) {
-          if (rank < num) put(rank, E{value_of(s.key[w][i]), s.at[w][i]});
-        });
-    return min(all, num);
-  }
-  E last{(double)__builtin_inff(), 0u};
-  for (int r = 0; r < num; ++r) {  // (more than num of them are there)
-    E b{(double)kNone, 0xFFFFFFFFu};
-    each([&](double v, uint32_t at) {
-      const E e{v, at};
-      if (v > (double)kNone && e.over(b) && (r == 0 || last.over(e))) b = e;
-    });
+  rank_lists(
+      s.key, n, all,
+      [&](int w, int i, int of, int len, int same) {
+        int better = 0;
+        same += (int)other_half<1>((uint32_t)same);
+        same += (int)other_half<2>((uint32_t)same);
+        if (__builtin_amdgcn_ballot_w64(same > 1))  // equal values: by place
+          for (int j = 0; j < len; j += 4)
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const E e{__shfl_xor(b.v, o), (uint32_t)__shfl_xor((int)b.at, o)};
-      if (e.over(b)) b = e;
-    }
-    __syncthreads();
-    if ((tid & 63) == 0) s.best[wave] = b;
-    __syncthreads();
-    last = s.best[0];
-    for (int w = 1; w < kBmWaves; ++w)
-      if (s.best[w].over(last)) last = s.best[w];
-    if (tid == 0) put(r, last);
-  }
-  return num;
+            for (int k = 0; k < 4; ++k)
+              better += (s.key[of][j + k] == s.key[w][i]) & (s.at[of][j + k] < s.at[w][i]);
+        return better;
+      },
+      [&](int rank, int w, int i) {
+        if (rank < num) put(rank, value_of(s.key[w][i]), s.at[w][i]);
+      });
+  return min(all, num);
 }
 
 __device__ __forceinline__ float to_float(__half x) { return (float)(_Float16)x; }
@@ -319,8 +364,8 @@ struct BeamArgs {
 __device__ __forceinline__ uint64_t pack(float v, uint32_t at) {
   return (uint64_t)at << 32 | __float_as_uint(v);
 }
-__device__ __forceinline__ Element<float> unpack(uint64_t x) {
-  return Element<float>{__uint_as_float((uint32_t)x), (uint32_t)(x >> 32)};
+__device__ __forceinline__ Element unpack(uint64_t x) {
+  return Element{__uint_as_float((uint32_t)x), (uint32_t)(x >> 32)};
 }
 
 // The last workgroup of a prompt to arrive: its beams' normalizers, then the best
@@ -399,7 +444,7 @@ __device__ void beam_last(const BeamArgs& a, int b, LastLds& top) {
   const uint64_t of_nan = __builtin_amdgcn_ballot_w64(lane < a.K && lk != lk);
   double c[R];
   float mx = kNone;
-  auto value = [&](Element<float> e) {
+  auto value = [&](Element e) {
     const int k = e.at >> kBmVocab;
     return (double)score[k] + ((double)e.v - lse[k]);
   };
@@ -410,9 +455,6 @@ __device__ void beam_last(const BeamArgs& a, int b, LastLds& top) {
   for (int i = 0; i < R; ++i) {
     c[i] = tid + i * kBmThreads < total ? value(unpack(mine[i])) : (double)kNone;
     mx = fmaxf(mx, key(c[i]));
-  }
-  for (int i = tid + R * kBmThreads; i < total; i += kBmThreads) {
-    mx = fmaxf(mx, key(value(unpack(handoff_get(best + i)))));
   }
   const int64_t out = (int64_t)b * a.num;
   auto put = [&](int r, double v, int k, int token) {
@@ -437,19 +479,28 @@ __device__ void beam_last(const BeamArgs& a, int b, LastLds& top) {
   if (num == 0) return;  // uniform
   const int found = top_n(
       num, top, mx,
-      [&](auto f) {
+      [&](auto add) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) f(c[i], (uint32_t)(mine[i] >> 32));
-        // (all lanes of a wave, for its ballots)
-        for (int i = R * kBmThreads; i < total; i += kBmThreads) {
-          const Element<float> e = unpack(handoff_get(best + min(i + tid, total - 1)));
-          f(i + tid < total ? value(e) : (double)kNone, e.at);
-        }
+        for (int i = 0; i < R; ++i) add(c[i], (uint32_t)(mine[i] >> 32), R * 64 > LastLds::kMost);
+        // the others: 64 parts a wave (all lanes, for its ballots), their first ones,
+        // their second ones, until none is taken: a part's are in order
+        const int of_all = a.K * a.parts, r0 = R * kBmThreads / of_all;
+        if (r0 < a.num)
+          for (int p0 = wave * 64; p0 < of_all; p0 += kBmThreads) {
+            const int p = min(p0 + lane, of_all - 1);
+            uint64_t next = handoff_get(best + r0 * of_all + p);
+            for (int r = r0; r < a.num; ++r) {
+              const Element e = unpack(next);
+              next = handoff_get(best + min(r + 1, a.num - 1) * of_all + p);
+              const bool other = p0 + lane < of_all && r * of_all + p >= R * kBmThreads;
+              if (!add(other ? value(e) : (double)kNone, e.at, true) && r > r0) break;  // uniform
+            }
+          }
       },
       key,
-      [&](int rank, Element<double> e) {
-        put(first + rank, e.v, e.at >> kBmVocab, e.at & ((1 << kBmVocab) - 1));
-        taken[rank] = e.at;
+      [&](int rank, double v, uint32_t at) {
+        put(first + rank, v, at >> kBmVocab, at & ((1 << kBmVocab) - 1));
+        taken[rank] = at;
       });
   if (found == num) return;  // uniform
   // The rest are -inf: the lowest places of the other beams that are not among
@@ -474,7 +525,7 @@ static_assert(2 * kBmMost <= kBmThreads, "as many places as may be taken and nee
 // the value's order above its place's.
 struct PartLds {
   static constexpr int kChunk = 64 * kBmEach, kMost = 768;  // of a wave: a chunk's, all
-  uint64_t key[kBmWaves][kMost + 4], kept[kBmWaves][kBmMost];
+  uint64_t key[kBmWaves][kMost + 4];
   float2 least[kBmWaves];
   int count[kBmWaves];
 };
@@ -485,25 +536,6 @@ __device__ __forceinline__ float next_up(float x) {
   return __uint_as_float((int)b < 0 ? b - 1 : b + 1);
 }
 
-// Keeps the num best of a wave's list of n keys, at its front.  (Rare: values that
-// rise along the row.)
-__device__ __forceinline__ void keep_best(uint64_t* list, uint64_t* kept, int n, int num) {
-  const int lane = threadIdx.x & 63;
-  paged_lds_sync();
-#pragma unroll 1
-  for (int i = lane; i < n; i += 64) {
-    const uint64_t key = list[i];
-    int rank = 0;
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) rank += list[j] > key;
-    if (rank < num) kept[rank] = key;
-  }
-  paged_lds_sync();
-#pragma unroll 1
-  for (int i = lane; i < num; i += 64) list[i] = kept[i];
-  paged_lds_sync();
-}
-
 // One workgroup a part of a row, in chunks of 2048 values that pass through
 // registers, so that memory is read once: the sum of its exponentials, and its
 // best.  The last workgroup of a prompt to arrive goes on with all of its parts'.
@@ -511,7 +543,7 @@ __device__ __forceinline__ void keep_best(uint64_t* list, uint64_t* kept, int n,
 // Many rows are bound by instructions: 30 vector ones a value, 15 of them fp64,
 // and the cut's scalar ones: 128 rows of 151936 fp16 values 31 us (1.2 TB/s; a
 // copy's rate would be 8).  Few rows are bound by the way of one part (5 us) and
-// of a prompt's last workgroup (5 us): 4 rows 11.9 us with the launch.
+// of a prompt's last workgroup (5 us): 4 rows 12.3 us with the launch.
 //
 // A thread sums its exponentials over the first value that it saw (or a later one
 // 600 above it: fp64 has the room).  A wave collects what is not below the num-th
@@ -586,7 +618,7 @@ __global__ __launch_bounds__(kBmThreads) void beam_kernel(BeamArgs a) {
       const float to = mx > ref + 600.f ? mx : ref;
       double d[1] = {below(ref, to)};
       exp_of(d);
-      sum *= d[0];
+      sum = mx > ref + 600.f ? sum * d[0] : sum;
       ref = to;
     }
     const double m = ref;
@@ -602,8 +634,9 @@ __global__ __launch_bounds__(kBmThreads) void beam_kernel(BeamArgs a) {
   float cut = -__FLT_MAX__;  // what is below is none of the best
   int mine = 0;              // keys of the wave's list
   auto collect = [&](int c) {
-    if (mine > s.kMost - s.kChunk) {
-      keep_best(s.key[wave], s.kept[wave], mine, num);
+    if (__builtin_expect(mine > s.kMost - s.kChunk, 0)) {
+      const uint64_t least = keep_best<PartLds::kMost, false>(s.key[wave], nullptr, mine, num);
+      cut = fmaxf(cut, next_up(value_of((uint32_t)(least >> 32))));
       mine = num;
     }
 #pragma unroll
@@ -680,6 +713,10 @@ __global__ __launch_bounds__(kBmThreads) void beam_kernel(BeamArgs a) {
     }
     cut = fmaxf(cut, least);
     collect(c);
+    if (__builtin_expect(mine > max(num, 64), 0)) {
+      keep_best<PartLds::kMost, false>(s.key[wave], nullptr, mine, num);
+      mine = num;
+    }
     if (lane < 4) s.key[wave][mine + lane] = 0;
     if (lane == 0) s.count[wave] = mine;
   }
