@@ -614,11 +614,14 @@ __global__ __launch_bounds__(kBmThreads) void beam_kernel(BeamArgs a) {
     } else {
       top1 = fmaxf(top1, mx);
     }
-    if (__builtin_amdgcn_ballot_w64(mx > ref + 600.f)) {  // (-inf: any value is)
-      const float to = mx > ref + 600.f ? mx : ref;
+    // (by the difference, which fp32 has exactly where the two are near: ref + 600
+    // may round to ref + 1024; over -inf any value is, and inf - inf, NaN, is not)
+    const bool shift = mx - ref > 600.f;
+    if (__builtin_amdgcn_ballot_w64(shift)) {
+      const float to = shift ? mx : ref;
       double d[1] = {below(ref, to)};
       exp_of(d);
-      sum = mx > ref + 600.f ? sum * d[0] : sum;
+      sum = shift ? sum * d[0] : sum;
       ref = to;
     }
     const double m = ref;

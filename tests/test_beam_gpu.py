@@ -259,6 +259,29 @@ def test_large_logits(gpu):
         assert ((a[0].double() + 1 + math.log(2)).abs() < tol + 2.0 ** -23).all()
 
 
+@pytest.mark.parametrize("base", [2.0 ** 33, 1e10, 14e6 * 1024, -1e10, -(2.0 ** 34 - 2048), -2.0 ** 33])
+@pytest.mark.parametrize("num", [4, 100])
+def test_large_logits_in_later_chunks(gpu, base, num):
+    """Logits that grow by 1024 along a part of several chunks, where 1024 is
+    fp32's step: the largest are the whole sum.  They and their differences are
+    exact in fp64, so a score is off by the fp64 rounding of lse, half a step of
+    values up to 2^34 (2^-20), where log 2 comes in, once in each side, and the
+    fp32 rounding of what is given."""
+    B, K, V = 12, 8, 49160
+    x = torch.full((B * K, V), base, device=gpu)
+    at = torch.arange(V, device=gpu)
+    x[:, at % 6145 > 5000] = base - 2048
+    ones, twos = torch.arange(0, B * K, 2, device=gpu), torch.arange(1, B * K, 2, device=gpu)
+    x[ones, 40001 + ones] = base + 1024   # one that counts
+    x[twos, 9001 + twos] = base + 1024    # two, in different parts
+    x[twos, 47003 + twos] = base + 1024
+    s = -2 * torch.arange(K, device=gpu, dtype=torch.float32).expand(B, -1).contiguous()
+    a, p, t = kernels.beam_select(x, s, num)
+    rs, rp, rt = reference(x, s, num)
+    assert torch.equal(p.cpu(), rp) and torch.equal(t.cpu(), rt)
+    assert ((a.cpu().double() - rs).abs() <= 2.0 ** -24 * rs.abs() + 2 * 2.0 ** -20 + 3e-10).all()
+
+
 def test_subnormal_logits_keep_their_order(gpu):
     x = torch.zeros(1, 3000, dtype=torch.float16, device=gpu)
     x[0, 2000], x[0, 1000], x[0, 500] = 3 * 2.0 ** -24, 2 * 2.0 ** -24, 2.0 ** -24
