@@ -67,6 +67,8 @@ class PagedKVCache:
         self._own: list[list[int]] = [[] for _ in range(max_seqs)]
         self._refs = [0] * self.pages
         self._free = list(range(self.pages - 1, -1, -1))
+        # the first page behind the sinks that a window has not left yet
+        self._behind = [-(-sinks // page_size)] * max_seqs
 
     @classmethod
     def for_model(cls, model, max_seqs: int, max_seq_len: int, **kwargs):
@@ -100,7 +102,7 @@ class PagedKVCache:
         if len(new) != self.max_seqs or min(new) < 0:
             raise RuntimeError(f"new must hold {self.max_seqs} token counts >= 0")
         size = self.page_size
-        need, behind, copied = [], {}, []  # behind: (sequence, index) -> page
+        need, behind, copied = [], [], []  # behind: (sequence, first page, the one after the last)
         left = Counter()                   # references given up
         for b, n in enumerate(new):
             own, L = self._own[b], self._len[b]
@@ -109,10 +111,11 @@ class PagedKVCache:
                                    f"(max_seq_len {self.max_seq_len})")
             need.append(max(0, -(-(L + n) // size) - len(own)))
             if n and self.window:
-                for i in range(-(-self.sinks // size), max(0, L + 1 - self.window) // size):
-                    if own[i] >= 0:
-                        behind[b, i] = own[i]
-                        left[own[i]] += 1
+                first, end = self._behind[b], (L + 1 - self.window) // size
+                for i in range(first, end):
+                    left[own[i]] += 1
+                if first < end:
+                    behind.append((b, first, end))
             if n and L % size:
                 page = own[-1]
                 if self._refs[page] - left[page] > 1:  # (the last one that has it keeps it)
@@ -125,8 +128,10 @@ class PagedKVCache:
         self._free.extend(given)
         for p, n in left.items():
             self._refs[p] -= n
-        for b, i in behind:
-            self._own[b][i] = self._table[b, i] = -1
+        for b, first, end in behind:
+            self._own[b][first:end] = [-1] * (end - first)
+            self._table[b, first:end] = -1
+            self._behind[b] = end
         if copied:
             pairs = [(self._own[b][-1], self._take_page(b, len(self._own[b]) - 1),
                       self._len[b] % size) for b in copied]
@@ -176,6 +181,7 @@ class PagedKVCache:
         self._give_back(reversed(self._own[seq]))
         self._own[seq] = []
         self._len[seq] = 0
+        self._behind[seq] = -(-self.sinks // self.page_size)
         self._table[seq].fill_(-1)
         self.page_table.copy_(self._table)
         self._upload_lengths()
@@ -193,7 +199,7 @@ class PagedKVCache:
         for p in self._own[src]:
             if p >= 0:
                 self._refs[p] += 1
-        self._len[dst] = self._len[src]
+        self._len[dst], self._behind[dst] = self._len[src], self._behind[src]
         self._set_row(dst, self._own[src])
         self.page_table.copy_(self._table)
         self._upload_lengths()
@@ -218,6 +224,7 @@ class PagedKVCache:
             self._give_back(pages)
         for b, pages in own.items():
             self._set_row(b, pages)
+        self._behind = [self._behind[p] for p in parents]
         self.page_table.copy_(self._table)
         if lens != self._len:
             self._len = lens
@@ -250,6 +257,7 @@ class PagedKVCache:
             self._give_back(reversed(self._own[b]))
             self._own[b] = []
         self._len = [0] * self.max_seqs
+        self._behind = [-(-self.sinks // self.page_size)] * self.max_seqs
         self._table.fill_(-1)
         self.page_table.copy_(self._table)
         self.lengths.zero_()

@@ -267,3 +267,53 @@ def test_beam_bookkeeping(K, eos, penalty, steps):
             text, score = _search(table, first[p], K, steps, eos, penalty)
             assert math.isclose(values[p], score, rel_tol=1e-12)
             assert tuple(texts[p]) == text
+
+
+class _Visits(list):
+    """A list that counts the entries that are looked at."""
+    seen = 0
+
+    def __getitem__(self, i):
+        _Visits.seen += len(range(len(self))[i]) if isinstance(i, slice) else 1
+        return super().__getitem__(i)
+
+    def __iter__(self):
+        for i in range(len(self)):
+            yield self[i]
+
+
+def test_a_window_walks_each_page_once():
+    """A step looks at the pages that leave the window with it, however many left
+    before: of long sequences, their forks, and those that others became."""
+    c = Tokens(max_seqs=4, max_seq_len=100000, pages=60, window=100, sinks=20)
+
+    def visited(new):
+        for b in range(4):
+            c._own[b] = _Visits(c._own[b])
+        _Visits.seen = 0
+        c.extend(new)
+        return _Visits.seen
+
+    for _ in range(500):
+        c.extend([100, 0, 0, 0])
+    assert c.length(0) == 50000 and c.pages - c.free_pages <= 2 + 9 + 7
+    # (a step of 100 tokens is followed by one that leaves (100 + 15) // 16 pages)
+    assert visited([1, 0, 0, 0]) <= 7 + 1
+    assert max(visited([1, 0, 0, 0]) for _ in range(39)) <= 2
+    c.fork(0, 1)
+    assert max(visited([1, 1, 0, 0]) for _ in range(40)) <= 4
+    c.reorder([3, 1, 0, 1])
+    assert [c.length(b) for b in range(4)] == [0, 50080, 50080, 50080]
+    assert max(visited([0, 1, 1, 1]) for _ in range(40)) <= 6
+    # a sequence that begins again frees what it has then
+    c.release(1)
+    for _ in range(30):
+        c.extend([0, 20, 0, 0])
+        kept = [i for i, p in enumerate(c.page_table[1].tolist()) if p >= 0]
+        L = c.length(1)
+        assert kept == [i for i in range(-(-L // 16))
+                        if i < 2 or i >= max(0, L - 20 + 1 - 100) // 16]
+    c.resize(50)
+    assert visited(1) <= 16
+    c.reset()
+    assert c.free_pages == 50
