@@ -213,17 +213,26 @@ class PagedKVCache:
         moved = [b for b, p in enumerate(parents) if p != b]
         if not moved:
             return
-        was = [self._own[b] for b in moved]
-        own = {b: list(self._own[parents[b]]) for b in moved}
         lens = [self._len[p] for p in parents]
-        for pages in own.values():
-            for p in pages:
-                if p >= 0:
-                    self._refs[p] += 1
-        for pages in was:
+        # a sequence that several become, once for each beyond the first, beside
+        # one that nobody does: the pages that both begin with (beams, their
+        # prompt's) are had as often as before
+        children = Counter(parents)
+        more = [p for p in sorted(children) for _ in range(children[p] - 1)]
+        gone = [b for b in range(self.max_seqs) if b not in children]
+        tails = []
+        for p, b in zip(more, gone):
+            n = _same(self._own[p], self._own[b])
+            for page in self._own[p][n:]:
+                if page >= 0:
+                    self._refs[page] += 1
+            tails.append(self._own[b][n:])
+        for pages in tails:
             self._give_back(pages)
-        for b, pages in own.items():
-            self._set_row(b, pages)
+        own = [list(self._own[parents[b]]) for b in moved]
+        for b, pages in zip(moved, own):
+            self._own[b] = pages
+        self._table[moved] = self._table[[parents[b] for b in moved]]
         self._behind = [self._behind[p] for p in parents]
         self.page_table.copy_(self._table)
         if lens != self._len:
@@ -273,6 +282,18 @@ class PagedKVCache:
             ws = self._workspaces[q.shape] = kernels.paged_attention_workspace(
                 q, self.layers[0][0], self.page_table)
         return ws
+
+
+def _same(a: list, b: list) -> int:
+    """How many entries two lists have in common at their front."""
+    lo, hi = 0, min(len(a), len(b))
+    while lo < hi:
+        mid = (lo + hi + 1) // 2
+        if a[lo:mid] == b[lo:mid]:
+            lo = mid
+        else:
+            hi = mid - 1
+    return lo
 
 
 class PagedStep:

@@ -317,3 +317,45 @@ def test_a_window_walks_each_page_once():
     assert visited(1) <= 16
     c.reset()
     assert c.free_pages == 50
+
+
+@pytest.mark.parametrize("window", [0, 70])
+def test_reordering_touches_what_differs(window):
+    """Beams that share a long prompt change places: references are counted for
+    the pages in which they differ, not for the prompt's."""
+    c = Tokens(max_seqs=6, max_seq_len=10000, pages=660, window=window, sinks=20 if window else 0)
+    c.extend([9990, 0, 0, 0, 0, 0])
+    c.texts[0] = list(range(9990))
+    c.held = {(p, i): 16 * j + i for j, p in enumerate(c._own[0]) for i in range(16)}
+    c.names = 10000
+    for b in range(1, 6):
+        c.fork(0, b)
+        c.texts[b] = list(c.texts[0])
+    c.step(1)
+    r = random.Random(window)
+    for parents in ([1, 0, 3, 2, 5, 4], [5, 0, 1, 2, 3, 4], [0, 0, 1, 1, 4, 4], [3] * 6,
+                    [0, 1, 2, 3, 4, 5], [2, 2, 2, 0, 4, 1], [5, 4, 5, 4, 5, 4]):
+        c._refs = _Visits(c._refs)
+        _Visits.seen = 0
+        c.reorder(parents)
+        # (a sequence's own pages are its last two; their references, before and after)
+        assert _Visits.seen <= 6 * 8
+        c._refs = list.copy(c._refs)
+        c.texts = [list(c.texts[p]) for p in parents]
+        c.check()
+        c.step([r.choice((0, 1)) for _ in range(6)])
+        c.reorder(range(6))
+    for b in (3, 0, 5, 1, 2):
+        c.release(b)
+        c.texts[b] = []
+        c.check()
+    # sequences of other lengths, and empty ones
+    c.step([3, 0, 40, 0, 0, 17])
+    for parents in ([4, 0, 0, 1, 2, 5], [0, 3, 3, 0, 4, 4], [4] * 6, [3, 0, 1, 1, 1, 1]):
+        c.reorder(parents)
+        c.texts = [list(c.texts[p]) for p in parents]
+        c.check()
+        try:
+            c.step(1)
+        except RuntimeError as e:
+            assert "max_seq_len" in str(e)
