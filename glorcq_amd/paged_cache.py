@@ -101,33 +101,35 @@ class PagedKVCache:
         new = [new] * self.max_seqs if uniform else [int(n) for n in new]
         if len(new) != self.max_seqs or min(new) < 0:
             raise RuntimeError(f"new must hold {self.max_seqs} token counts >= 0")
-        size = self.page_size
-        need, behind, copied = [], [], []  # behind: (sequence, first page, the one after the last)
-        left = Counter()                   # references given up
-        for b, n in enumerate(new):
-            own, L = self._own[b], self._len[b]
-            if L + n > self.max_seq_len:
-                raise RuntimeError(f"sequence {b} would have {L + n} tokens "
-                                   f"(max_seq_len {self.max_seq_len})")
-            need.append(max(0, -(-(L + n) // size) - len(own)))
-            if n and self.window:
-                first, end = self._behind[b], (L + 1 - self.window) // size
-                for i in range(first, end):
-                    left[own[i]] += 1
+        # (on the path of every decode step: without windows and forks, sums and
+        # compares of a few numbers a sequence)
+        size, window, refs = self.page_size, self.window, self._refs
+        lens = [L + n for L, n in zip(self._len, new)]
+        if max(lens) > self.max_seq_len:
+            b = next(b for b, L in enumerate(lens) if L > self.max_seq_len)
+            raise RuntimeError(f"sequence {b} would have {lens[b]} tokens "
+                               f"(max_seq_len {self.max_seq_len})")
+        need = [-(-L // size) - len(own) for L, own in zip(lens, self._own)]
+        behind, copied = [], []  # behind: (sequence, first page, the one after the last)
+        left = {}                # references given up
+        for b, L in enumerate(self._len):
+            if window and new[b]:
+                first, end = self._behind[b], (L + 1 - window) // size
                 if first < end:
                     behind.append((b, first, end))
-            if n and L % size:
-                page = own[-1]
-                if self._refs[page] - left[page] > 1:  # (the last one that has it keeps it)
-                    copied.append(b)
-                    left[page] += 1
-        given = [p for p, n in left.items() if self._refs[p] == n]
+                    for page in self._own[b][first:end]:
+                        left[page] = left.get(page, 0) + 1
+            if L % size and refs[page := self._own[b][-1]] > 1 and new[b] \
+                    and refs[page] - left.get(page, 0) > 1:  # (the last one that has it keeps it)
+                copied.append(b)
+                left[page] = left.get(page, 0) + 1
+        given = [p for p, n in left.items() if refs[p] == n]
         wanted, there = sum(need) + len(copied), len(self._free) + len(given)
         if wanted > there:
             raise RuntimeError(f"{wanted} pages needed, {there} free")
         self._free.extend(given)
         for p, n in left.items():
-            self._refs[p] -= n
+            refs[p] -= n
         for b, first, end in behind:
             self._own[b][first:end] = [-1] * (end - first)
             self._table[b, first:end] = -1
@@ -136,11 +138,12 @@ class PagedKVCache:
             pairs = [(self._own[b][-1], self._take_page(b, len(self._own[b]) - 1),
                       self._len[b] % size) for b in copied]
             self._copy_pages(*map(list, zip(*pairs)))
-        for b, n in enumerate(new):
-            for _ in range(need[b]):
-                self._take_page(b, len(self._own[b]))
-            self._len[b] += n
-        if any(need) or behind or copied:
+        if wanted:
+            for b, n in enumerate(need):
+                for _ in range(n):
+                    self._take_page(b, len(self._own[b]))
+        self._len = lens
+        if wanted or behind:
             self.page_table.copy_(self._table)
         if uniform:
             self.lengths.add_(new[0])
