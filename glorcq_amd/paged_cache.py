@@ -60,6 +60,7 @@ class PagedKVCache:
         self._table = torch.full((max_seqs, each), -1, dtype=torch.int32)
         self.page_table = self._table.to(self.device)
         self.lengths = torch.zeros(max_seqs, dtype=torch.int32, device=self.device)
+        self._changed = [False, False]  # page table and lengths, since they were uploaded
         self._workspaces: dict = {}
         self._len = [0] * max_seqs
         # pages of each sequence's positions (-1: freed behind the window), and
@@ -144,11 +145,12 @@ class PagedKVCache:
                     self._take_page(b, len(self._own[b]))
         self._len = lens
         if wanted or behind:
-            self.page_table.copy_(self._table)
-        if uniform:
+            self._changed[0] = True
+        if uniform and not self._changed[1]:
             self.lengths.add_(new[0])
         else:
-            self._upload_lengths()
+            self._changed[1] = True
+        self._upload()
 
     def _take_page(self, seq: int, i: int) -> int:
         """A free page as the sequence's i-th."""
@@ -175,23 +177,36 @@ class PagedKVCache:
         if own:
             self._table[seq, :len(own)] = torch.tensor(own, dtype=torch.int32)
 
-    def _upload_lengths(self):
-        self.lengths.copy_(torch.tensor(self._len, dtype=torch.int32))
+    def _upload(self) -> None:
+        """Brings the device the page table and the lengths, where they changed."""
+        table, lens = self._changed
+        if table:
+            self.page_table.copy_(self._table)
+        if lens:
+            self.lengths.copy_(torch.tensor(self._len, dtype=torch.int32))
+        self._changed = [False, False]
 
     def release(self, seq: int) -> None:
         """Gives a sequence's pages back (those that it shares stay the others');
         its length is 0 again."""
+        self._release(seq)
+        self._upload()
+
+    def _release(self, seq):
         self._give_back(reversed(self._own[seq]))
         self._own[seq] = []
         self._len[seq] = 0
         self._behind[seq] = -(-self.sinks // self.page_size)
         self._table[seq].fill_(-1)
-        self.page_table.copy_(self._table)
-        self._upload_lengths()
+        self._changed = [True, True]
 
     def fork(self, src: int, dst: int) -> None:
         """Makes the empty sequence dst one with src's tokens.  They share its
         pages; the last one is copied when either gets a token."""
+        self._fork(src, dst)
+        self._upload()
+
+    def _fork(self, src, dst):  # (without the upload: the next extend's will do)
         for b in (src, dst):
             if not 0 <= b < self.max_seqs:
                 raise RuntimeError(f"no sequence {b}")
@@ -204,12 +219,15 @@ class PagedKVCache:
                 self._refs[p] += 1
         self._len[dst], self._behind[dst] = self._len[src], self._behind[src]
         self._set_row(dst, self._own[src])
-        self.page_table.copy_(self._table)
-        self._upload_lengths()
+        self._changed = [True, True]
 
     def reorder(self, parents) -> None:
         """Sequence b becomes what sequence parents[b] was (parents: one a
         sequence); pages that nobody has any more are freed."""
+        self._reorder(parents)
+        self._upload()
+
+    def _reorder(self, parents):
         parents = [int(p) for p in parents]
         if len(parents) != self.max_seqs or not all(0 <= p < self.max_seqs for p in parents):
             raise RuntimeError(f"parents must hold {self.max_seqs} sequences")
@@ -237,10 +255,10 @@ class PagedKVCache:
             self._own[b] = pages
         self._table[moved] = self._table[[parents[b] for b in moved]]
         self._behind = [self._behind[p] for p in parents]
-        self.page_table.copy_(self._table)
+        self._changed[0] = True
         if lens != self._len:
             self._len = lens
-            self._upload_lengths()
+            self._changed[1] = True
 
     def resize(self, pages: int) -> None:
         """Moves the pages that sequences have to the front of new pools of
@@ -258,7 +276,8 @@ class PagedKVCache:
         self._free = list(range(pages - 1, len(live) - 1, -1))
         for b, own in enumerate(self._own):
             self._set_row(b, [place.get(p, -1) for p in own])
-        self.page_table.copy_(self._table)
+        self._changed[0] = True
+        self._upload()
 
     def _move_pages(self, src, pools) -> None:
         k, v, ks, vs = self.pools
@@ -271,8 +290,8 @@ class PagedKVCache:
         self._len = [0] * self.max_seqs
         self._behind = [-(-self.sinks // self.page_size)] * self.max_seqs
         self._table.fill_(-1)
-        self.page_table.copy_(self._table)
-        self.lengths.zero_()
+        self._changed = [True, True]
+        self._upload()
 
     def workspace(self, q: torch.Tensor):
         """The attention workspace of steps of q's shape, one for all layers:
@@ -415,6 +434,10 @@ class GLoRCQPagedWrapper:
     def replay(self, input_ids):
         """One decode step: (batch,) ids, the sequences' next tokens -> the
         captured logits buffer (batch, vocab)."""
+        return self._replay(input_ids, 1)
+
+    def _replay(self, input_ids, new):
+        """replay, with what cache.extend takes."""
         if self.graph is None:
             raise RuntimeError("no captured step (capture_graph, which empties the cache)")
         if self._graph_pools is not self.cache.pools:
@@ -423,7 +446,7 @@ class GLoRCQPagedWrapper:
         if input_ids.shape != self.static_input_ids.shape:
             raise RuntimeError(f"input_ids must be ({self.max_batch_size},)")
         self.static_input_ids.copy_(input_ids)
-        self.cache.extend(1)
+        self.cache.extend(new)
         self.graph.replay()
         return self.static_logits
 
@@ -480,12 +503,26 @@ class GLoRCQPagedWrapper:
         P, vocab = logits.shape
         if vocab < 2 * K:
             raise RuntimeError(f"a vocabulary of {vocab} has no {2 * K} continuations")
-        for p in range(P):
-            for j in range(1, K):
-                self.cache.fork(p * K, p * K + j)
         search = _Beams(P, K, eos_token_id, length_penalty)
         room = self.max_seq_len - max(int(p.shape[0]) for p in prompts)
-        steps = min(max_new_tokens, room + 1)
+        try:
+            step = self._search(search, logits, min(max_new_tokens, room + 1))
+        finally:
+            self.cache._upload()
+        texts, values = search.best(step)
+        t1 = time.time()
+        self.last_timing = {"beams_s": t1 - t0, "steps": step}
+        out = [torch.cat([p.to(self.device), torch.tensor(t, dtype=torch.long).to(self.device)])
+               for p, t in zip(prompts, texts)]
+        return out, values, t1 - t0
+
+    def _search(self, search, logits, steps):
+        """A beam search from the prompts' logits on; the steps it took.  (Forks
+        and moves reach the device with the tokens of the step after them.)"""
+        P, K = search.P, search.K
+        for p in range(P):
+            for j in range(1, K):
+                self.cache._fork(p * K, p * K + j)
         scores = logits.new_zeros((P, 1), dtype=torch.float32)
         for step in range(1, steps + 1):
             best = kernels.beam_select(logits, scores, 2 * K)
@@ -495,15 +532,10 @@ class GLoRCQPagedWrapper:
             if step == steps or search.done():
                 break
             if step > 1:  # (a first step's beams are all their prompt's)
-                self.cache.reorder(parents)
+                self.cache._reorder(parents)
             scores = torch.tensor(search.scores, dtype=torch.float32).to(self.device)
-            logits = self.replay(torch.tensor(search.tokens).to(self.device))
-        texts, values = search.best(step)
-        t1 = time.time()
-        self.last_timing = {"beams_s": t1 - t0, "steps": step}
-        out = [torch.cat([p.to(self.device), torch.tensor(t, dtype=torch.long).to(self.device)])
-               for p, t in zip(prompts, texts)]
-        return out, values, t1 - t0
+            logits = self._replay(torch.tensor(search.tokens).to(self.device), 1)
+        return step
 
 
 class _Beams:

@@ -8,7 +8,8 @@ import random
 import pytest
 import torch
 
-from glorcq_amd.paged_cache import PagedKVCache, PagedStep, _Beams
+from glorcq_amd import kernels
+from glorcq_amd.paged_cache import GLoRCQPagedWrapper, PagedKVCache, PagedStep, _Beams
 
 
 class Tokens(PagedKVCache):
@@ -359,3 +360,84 @@ def test_reordering_touches_what_differs(window):
             c.step(1)
         except RuntimeError as e:
             assert "max_seq_len" in str(e)
+
+
+class _Device(torch.Tensor):
+    """A tensor that counts what is uploaded to it."""
+    uploads = 0
+
+    def copy_(self, *args, **kw):
+        _Device.uploads += 1
+        return super().copy_(*args, **kw)
+
+
+class _Wrapper(GLoRCQPagedWrapper):
+    """Beam search's host side alone: a cache on the CPU, and a chain of tokens
+    (logits by the token before) in the model's place."""
+
+    def __init__(self, table, batch, **kw):
+        self.max_batch_size, self.max_seq_len = batch, kw.get("max_seq_len", 150)
+        self.cache = Tokens(max_seqs=batch, **kw)
+        for name in ("page_table", "lengths"):  # (on the CPU it would be the host's own)
+            setattr(self.cache, name, getattr(self.cache, name).clone().as_subclass(_Device))
+        self.device = torch.device("cpu")
+        self.static_input_ids = torch.zeros(batch, dtype=torch.long)
+        self.table = table
+        self.steps = []  # (sequences' lengths, uploads since the last step)
+
+    def _ready(self):
+        pass
+
+    def _prefill(self, prompts, each):
+        self.cache.reset()
+        new = [n for p in prompts for n in [len(p)] + [0] * (each - 1)]
+        self.cache.extend(new)
+        _Device.uploads = 0
+        return self.table[torch.stack([p[-1] for p in prompts])]
+
+    def _replayed(self):
+        """What the graph reads is what the host has."""
+        c = self.cache
+        assert c.page_table.tolist() == c._table.tolist()
+        assert c.lengths.tolist() == [c.length(b) for b in range(c.max_seqs)]
+        self.steps.append((c.lengths.tolist(), _Device.uploads))
+        _Device.uploads = 0
+
+    def _replay(self, input_ids, new):
+        self.cache.extend(new)
+        self._replayed()
+        return self.table[input_ids]
+
+
+def _select(logits, scores, num):
+    """kernels.beam_select in fp64 on the CPU."""
+    B, K = scores.shape
+    c = scores.double()[..., None] + torch.log_softmax(logits.double(), -1).view(B, K, -1)
+    v, i = c.flatten(1).sort(dim=1, descending=True, stable=True)
+    v, i, V = v[:, :num], i[:, :num], c.shape[2]
+    return v.float(), i // V, i % V
+
+
+def test_beams_upload_a_table_a_step(monkeypatch):
+    """A step of a beam search brings the device the page table and the lengths
+    once, however many sequences fork or change places."""
+    monkeypatch.setattr(kernels, "beam_select", _select)
+    g = torch.Generator().manual_seed(1)
+    w = _Wrapper(2 * torch.randn(40, 40, generator=g), 12)
+    prompts = [torch.tensor([3] * 20), torch.tensor([5] * 37), torch.tensor([9])]
+    w.generate_beams(prompts, 4, max_new_tokens=30)
+    assert len(w.steps) == 29
+    assert w.steps[0][0] == [21] * 4 + [38] * 4 + [2] * 4
+    assert all(n <= 2 for _, n in w.steps)
+    # forks, moves and ends by themselves bring theirs at once
+    w.cache.reset()
+    w.cache.extend([20] + [0] * 11)
+    for f in (lambda c: c.fork(0, 3), lambda c: c.reorder([3, 0] + [0] * 10),
+              lambda c: c.release(2), lambda c: c.resize(30)):
+        f(w.cache)
+        w._replayed()
+    # a search that the pool has no room for leaves the device what the host has
+    w = _Wrapper(w.table, 8, pages=6)
+    with pytest.raises(RuntimeError, match="pages needed"):
+        w.generate_beams([torch.tensor([3] * 40)] * 1 + [torch.tensor([7])], 4, max_new_tokens=30)
+    w._replayed()
