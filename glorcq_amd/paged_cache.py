@@ -489,7 +489,7 @@ class GLoRCQPagedWrapper:
         they are among the first num_beams; the others go on, num_beams of them,
         sharing their pages with their parents.  A prompt is done when it has
         num_beams finished ones and its best beam, as it is, scores below all of
-        them.  All stop at max_new_tokens, or where the longest reaches
+        them; its pages are the other prompts' from then on.  All stop at max_new_tokens, or where the longest reaches
         max_seq_len."""
         K = num_beams
         if K < 1 or 2 * K > 128 or self.max_batch_size % K:
@@ -533,8 +533,13 @@ class GLoRCQPagedWrapper:
                 break
             if step > 1:  # (a first step's beams are all their prompt's)
                 self.cache._reorder(parents)
+            new = [0 if d else 1 for d in search.ended for _ in range(K)]
+            for b in range(P * K):
+                if new[b] == 0 and self.cache.length(b):
+                    self.cache._release(b)
             scores = torch.tensor(search.scores, dtype=torch.float32).to(self.device)
-            logits = self._replay(torch.tensor(search.tokens).to(self.device), 1)
+            logits = self._replay(torch.tensor(search.tokens).to(self.device),
+                                  new if any(search.ended) else 1)
         return step
 
 
@@ -547,19 +552,24 @@ class _Beams:
         self.tokens = [0] * (prompts * beams)
         self._texts = [None] * (prompts * beams)  # (text before, token)
         self._finished = [[] for _ in range(prompts)]  # (score, text), the best first
-        self._done = [False] * prompts
+        self.ended = [False] * prompts
 
     def advance(self, found, step):
         """found: of each prompt, its 2 K best continuations' scores, parents and
-        tokens, one behind the other.  Returns each sequence's parent."""
+        tokens, one behind the other.  Returns each sequence's parent.  (A prompt
+        that is done stays as it is, whatever is found of it.)"""
         K, parents, texts = self.K, [], []
         for p, row in enumerate(found):
+            if self.ended[p]:
+                parents += range(p * K, p * K + K)
+                texts += self._texts[p * K:p * K + K]
+                continue
             n = len(row) // 3
             live = []
             for i in range(n):
                 score, parent, token = row[i], p * K + int(row[n + i]), int(row[2 * n + i])
                 if token == self.eos:
-                    if i < K and not self._done[p]:
+                    if i < K:
                         self._finish(p, score, (self._texts[parent], token), step)
                 elif len(live) < K:
                     live.append((score, parent, token))
@@ -570,7 +580,7 @@ class _Beams:
                 texts.append((self._texts[parent], token))
             done = self._finished[p]
             if len(done) == K and done[-1][0] >= self._value(live[0][0], step):
-                self._done[p] = True
+                self.ended[p] = True
         self._texts = texts
         return parents
 
@@ -584,14 +594,14 @@ class _Beams:
         del done[self.K:]
 
     def done(self):
-        return all(self._done)
+        return all(self.ended)
 
     def best(self, step):
         """Texts and scores; beams that are still going count as they are."""
         texts, values = [], []
         for p in range(self.P):
             all_of = list(self._finished[p])
-            if not self._done[p]:
+            if not self.ended[p]:
                 all_of += [(self._value(s, step), self._texts[p * self.K + j])
                            for j, s in enumerate(self.scores[p])]
             value, text = max(all_of, key=lambda x: x[0])

@@ -185,3 +185,32 @@ def test_refusals(gpu):
             w.generate_beams(*args, **kw)
     out, _, _ = w.generate_beams(prompts, 2, max_new_tokens=1)
     assert [len(x) for x in out] == [6, 7]
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+@torch.no_grad()
+def test_a_done_prompt_leaves_the_others_as_they_are(gpu, monkeypatch, dtype):
+    """One of two prompts ends in its first steps, and the graph is replayed with
+    its sequences empty: the other's text and score are those beside a prompt
+    that goes on, and its beams have the pages."""
+    K, n, eos = 3, 40, 5
+    forward = PC.paged_forward
+    likes = torch.zeros(2, 1, VOCAB, device=gpu)
+    likes[0, :, eos], likes[1, :, eos] = 30, -math.inf
+
+    def biased(model, ids, positions, step, last=None):
+        x = forward(model, ids, positions, step, last)
+        return (x.view(2, -1, VOCAB) + likes.to(x.dtype)).view(x.shape)
+
+    monkeypatch.setattr(PC, "paged_forward", biased)
+    model = _model(gpu)
+    prompts = _prompts((60, 21), gpu)
+    w = _wrapper(model, 2 * K, cache_dtype=dtype)
+    texts, scores, _ = w.generate_beams(prompts, K, max_new_tokens=n)
+    # the prompts' 4 and 2 pages, of which each beam copies the last one; of the
+    # long search 4 pages each in the end, the first one shared
+    small = _wrapper(model, 2 * K, cache_dtype=dtype, pages=6 + 2 * (K - 1) + 1)
+    out, got, _ = small.generate_beams(prompts, K, max_new_tokens=n, eos_token_id=eos)
+    assert len(out[0]) < 60 + 5 and int(out[0][-1]) == eos
+    assert torch.equal(out[1], texts[1]) and got[1] == scores[1]
+    assert [small.cache.length(b) for b in range(2 * K)] == [0] * K + [21 + n - 1] * K

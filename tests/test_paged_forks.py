@@ -441,3 +441,38 @@ def test_beams_upload_a_table_a_step(monkeypatch):
     with pytest.raises(RuntimeError, match="pages needed"):
         w.generate_beams([torch.tensor([3] * 40)] * 1 + [torch.tensor([7])], 4, max_new_tokens=30)
     w._replayed()
+
+
+def test_prompts_that_are_done_give_their_pages_back(monkeypatch):
+    """Two prompts end early; the third's long search has their pages, and finds
+    what it finds alone.  Nobody's results change when another one ends."""
+    monkeypatch.setattr(kernels, "beam_select", _select)
+    g = torch.Generator().manual_seed(2)
+    V, eos = 40, 0
+    table = torch.randn(V, V, generator=g)
+    table[:20, 20:] = table[20:, :20] = -50  # two groups of tokens:
+    table[:20, eos] += 9                     # one ends soon, one never
+    prompts = [torch.tensor([3] * 50), torch.tensor([25] * 20), torch.tensor([7] * 33)]
+    K, n = 3, 80
+    # 7 pages of prompts, each of whose beams copies one; the long search's beams
+    # at 100 tokens have 7 pages each, but the prompt's first, which they share
+    w = _Wrapper(table, 3 * K, pages=1 + K * 6 + 1)
+    out, scores, _ = w.generate_beams(prompts, K, max_new_tokens=n, eos_token_id=eos)
+    assert len(w.steps) == n - 1 and [len(t) for t in out][1] == 20 + n
+    ends = [next(i for i, (lens, _) in enumerate(w.steps) if lens[b * K:b * K + K] == [0] * K)
+            for b in (0, 2)]
+    assert max(ends) < 20
+    for lens, _ in w.steps[max(ends):]:
+        assert lens[:K] == lens[2 * K:] == [0] * K and min(lens[K:2 * K]) > 0
+    for b, p in enumerate(prompts):
+        one = _Wrapper(table, K)
+        text, score, _ = one.generate_beams([p], K, max_new_tokens=n, eos_token_id=eos)
+        assert torch.equal(text[0], out[b]) and score[0] == scores[b]
+    logp = torch.log_softmax(table.double(), -1)
+    for p, t, s in zip(prompts, out, scores):
+        want, value = _search(logp, logp[int(p[-1])], K, n, eos, 1.0)
+        assert tuple(t[len(p):].tolist()) == want
+        assert math.isclose(s, value, rel_tol=n * 2.0 ** -23)
+    # all of the cache can be used again
+    w.cache.reset()
+    assert w.cache.free_pages == w.cache.pages
