@@ -214,3 +214,36 @@ def test_a_done_prompt_leaves_the_others_as_they_are(gpu, monkeypatch, dtype):
     assert len(out[0]) < 60 + 5 and int(out[0][-1]) == eos
     assert torch.equal(out[1], texts[1]) and got[1] == scores[1]
     assert [small.cache.length(b) for b in range(2 * K)] == [0] * K + [21 + n - 1] * K
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+@torch.no_grad()
+def test_beam_scores_are_their_steps(gpu, dtype):
+    """The score of a text is the sum of its tokens' log-probabilities in a cache
+    that is replayed with that text alone, in 64 bits: the same kernels on the
+    same rows, so what differs is the rounding of each step's sum to fp32, 2^-24
+    of it (it grows, so of the last one), and the selection's 3e-10."""
+    model = _model(gpu)
+    prompts = _prompts((21, 50), gpu)
+    K, n = 4, 15
+    w = _wrapper(model, 2 * K, cache_dtype=dtype)
+    out, scores, _ = w.generate_beams(prompts, K, max_new_tokens=n)
+    assert len({tuple(t[-n:].tolist()) for t in out}) == 2
+    w = _wrapper(model, 2 * K, cache_dtype=dtype)
+    w.capture_graph()
+    # each prompt's K sequences all have the text (the prompts' forward with the
+    # search's rows: other numbers of rows take other kernels)
+    x = w._prefill(prompts, K).repeat_interleave(K, 0)
+    for b in range(2 * K):
+        if b % K:
+            w.cache.fork(b - b % K, b)
+    total = [0.0, 0.0]
+    for i in range(n):
+        logp = torch.log_softmax(x.double(), -1)
+        token = torch.stack([t[len(p) + i] for p, t in zip(prompts, out)]).repeat_interleave(K)
+        for p in range(2):
+            total[p] += float(logp[p * K, token[p * K]])
+        if i < n - 1:
+            x = w.replay(token)
+    for score, t in zip(scores, total):
+        assert abs(score - t / n) <= (n * 2.0 ** -24 * abs(t) + n * 3e-10) / n
