@@ -23,6 +23,7 @@ alone, inference/graph_wrapper.py:69-149).
 from __future__ import annotations
 
 import time
+import weakref
 from collections import Counter
 
 import torch
@@ -53,6 +54,7 @@ class PagedKVCache:
         self.pages = max_seqs * each if pages is None else pages
         if self.pages < 1:
             raise RuntimeError("a cache needs a page")
+        self._wrappers = weakref.WeakSet()  # whose captured steps run over the pools
         self._shape = (kv_heads, head_dim, page_size, dtype, device, layers)
         self._take_pools(kernels.paged_cache_tensors(self.pages, *self._shape))
         self.device = self.pools[0].device
@@ -80,8 +82,9 @@ class PagedKVCache:
                    device=next(model.parameters()).device, **kwargs)
 
     def _take_pools(self, pools) -> None:
-        """All layers' pools, one behind the other, and each layer's."""
-        self.pools = pools
+        """All layers' pools, one behind the other, and each layer's; `pools_key`
+        is theirs alone."""
+        self.pools, self.pools_key = pools, object()
         self.layers = [tuple(None if x is None else x[i] for x in pools)
                        for i in range(pools[0].shape[0])]
 
@@ -262,8 +265,9 @@ class PagedKVCache:
 
     def resize(self, pages: int) -> None:
         """Moves the pages that sequences have to the front of new pools of
-        `pages` pages each, and lets the old ones go (graphs that were captured
-        over those are captured again)."""
+        `pages` pages each, and lets the old ones go, with wrappers' steps that
+        were captured over them (GLoRCQPagedWrapper.capture_graph(keep=True)
+        captures them again)."""
         live = sorted({p for own in self._own for p in own if p >= 0})
         if pages < max(len(live), 1):
             raise RuntimeError(f"{len(live)} pages are in use")
@@ -271,6 +275,10 @@ class PagedKVCache:
         self._move_pages(live, pools)
         place = {p: i for i, p in enumerate(live)}
         self._take_pools(pools)
+        if self._wrappers:
+            torch.cuda.synchronize(self.device)  # (no replay is under way)
+        for w in self._wrappers:
+            w.graph = w.static_logits = None
         self.pages = pages
         self._refs = [self._refs[p] for p in live] + [0] * (pages - len(live))
         self._free = list(range(pages - 1, len(live) - 1, -1))
@@ -383,7 +391,7 @@ class GLoRCQPagedWrapper:
         self.device = self.cache.device
         self.static_input_ids = torch.zeros(max_batch_size, dtype=torch.long, device=self.device)
         self.static_logits = None
-        self.graph = None
+        self.graph = self._graph_pools = None
         self.graph_stream = torch.cuda.Stream(device=self.device)
         self.last_timing = {}
 
@@ -392,21 +400,33 @@ class GLoRCQPagedWrapper:
                              PagedStep(self.cache))
 
     @torch.no_grad()
-    def capture_graph(self):
+    def capture_graph(self, keep=False):
         """Warm-up steps on a side stream, then one decode step captured.  The
-        cache is empty meanwhile (a token before position 0 is written nowhere)."""
+        cache is emptied, or with `keep` its sequences stay; meanwhile they have
+        no tokens (one before position 0 is written nowhere)."""
         self.model.eval()
-        self.cache.reset()
-        s = torch.cuda.Stream(device=self.device)
-        s.wait_stream(torch.cuda.current_stream(self.device))
-        with torch.cuda.stream(s):
-            for _ in range(3):
-                self._step()
-        torch.cuda.current_stream(self.device).wait_stream(s)
-        torch.cuda.synchronize(self.device)
-        self.graph, self._graph_pools = torch.cuda.CUDAGraph(), self.cache.pools
-        with torch.cuda.graph(self.graph, stream=self.graph_stream):
-            self.static_logits = self._step()
+        cache = self.cache
+        if keep:
+            cache.lengths.zero_()
+        else:
+            cache.reset()
+        try:
+            s = torch.cuda.Stream(device=self.device)
+            s.wait_stream(torch.cuda.current_stream(self.device))
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    self._step()
+            torch.cuda.current_stream(self.device).wait_stream(s)
+            torch.cuda.synchronize(self.device)
+            self.graph, graph = None, torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=self.graph_stream):
+                self.static_logits = self._step()
+            self.graph, self._graph_pools = graph, cache.pools_key
+            cache._wrappers.add(self)
+        finally:
+            if keep:
+                cache._changed[1] = True
+                cache._upload()
 
     @torch.no_grad()
     def prefill(self, prompts):
@@ -438,11 +458,11 @@ class GLoRCQPagedWrapper:
 
     def _replay(self, input_ids, new):
         """replay, with what cache.extend takes."""
+        if self._graph_pools not in (None, self.cache.pools_key):
+            raise RuntimeError("the step was captured over pools that the cache no longer has "
+                               "(capture_graph; with keep=True the sequences stay)")
         if self.graph is None:
             raise RuntimeError("no captured step (capture_graph, which empties the cache)")
-        if self._graph_pools is not self.cache.pools:
-            raise RuntimeError("the step was captured over pools that the cache no longer has "
-                               "(capture_graph, which empties it)")
         if input_ids.shape != self.static_input_ids.shape:
             raise RuntimeError(f"input_ids must be ({self.max_batch_size},)")
         self.static_input_ids.copy_(input_ids)
@@ -451,7 +471,7 @@ class GLoRCQPagedWrapper:
         return self.static_logits
 
     def _ready(self):
-        if self.graph is None or self._graph_pools is not self.cache.pools:
+        if self.graph is None or self._graph_pools is not self.cache.pools_key:
             self.capture_graph()
 
     @torch.no_grad()

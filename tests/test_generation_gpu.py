@@ -247,3 +247,47 @@ def test_beam_scores_are_their_steps(gpu, dtype):
             x = w.replay(token)
     for score, t in zip(scores, total):
         assert abs(score - t / n) <= (n * 2.0 ** -24 * abs(t) + n * 3e-10) / n
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+@torch.no_grad()
+def test_sequences_go_on_after_a_resize(gpu, dtype):
+    """Steps, a pool of another size, a step captured over it with the sequences
+    kept, and so on: bit for bit the steps of a cache that stays as it is."""
+    model = _model(gpu)
+    prompts = _prompts((40, 7, 64), gpu)
+    a, b = (_wrapper(model, 3, cache_dtype=dtype, pages=30) for _ in range(2))
+    for w in (a, b):
+        w.capture_graph()
+    assert torch.equal(a.prefill(prompts), b.prefill(prompts))
+    g = torch.Generator().manual_seed(9)
+    for pages in (None, 16, 50):
+        if pages:
+            a.cache.resize(pages)
+            with pytest.raises(RuntimeError, match="captured over"):
+                a.replay(torch.zeros(3, dtype=torch.long, device=gpu))
+            a.capture_graph(keep=True)
+        assert a.cache.lengths.tolist() == b.cache.lengths.tolist()
+        for i in range(12):
+            t = torch.randint(0, VOCAB, (3,), generator=g).to(gpu)
+            assert torch.equal(a.replay(t).clone(), b.replay(t)), (pages, i)
+    a.capture_graph()  # (as before: an empty cache)
+    assert a.cache.free_pages == 50 and a.cache.lengths.tolist() == [0] * 3
+
+
+@torch.no_grad()
+def test_a_resize_gives_memory_back(gpu):
+    """A wrapper with a captured step does not keep the pools that it was
+    captured over, nor the step."""
+    model = _model(gpu)
+    w = _wrapper(model, 2, pages=4000)
+    w.generate(_prompts((5, 9), gpu), max_new_tokens=3)
+    w.cache.reset()
+    size = lambda: sum(t.numel() * t.element_size() for t in w.cache.pools)  # noqa: E731
+    torch.cuda.synchronize()
+    was, held = size(), torch.cuda.memory_allocated(gpu)
+    w.cache.resize(40)
+    torch.cuda.synchronize()
+    assert w.graph is None and torch.cuda.memory_allocated(gpu) <= held - (was - size())
+    out, _ = w.generate(_prompts((5, 9), gpu), max_new_tokens=3)  # captured again
+    assert [len(t) for t in out] == [8, 12]
