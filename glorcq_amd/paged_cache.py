@@ -22,6 +22,7 @@ alone, inference/graph_wrapper.py:69-149).
 
 from __future__ import annotations
 
+import operator
 import time
 import weakref
 from collections import Counter
@@ -517,6 +518,11 @@ class GLoRCQPagedWrapper:
                                f"({self.max_batch_size})")
         if max_new_tokens < 1:
             raise RuntimeError("max_new_tokens must be positive")
+        if eos_token_id is not None:
+            try:
+                eos_token_id = operator.index(eos_token_id)
+            except TypeError:
+                raise RuntimeError(f"eos_token_id must be one token (got {eos_token_id!r})") from None
         self._ready()
         t0 = time.time()
         logits = self._prefill(prompts, K)

@@ -476,3 +476,17 @@ def test_prompts_that_are_done_give_their_pages_back(monkeypatch):
     # all of the cache can be used again
     w.cache.reset()
     assert w.cache.free_pages == w.cache.pages
+
+
+def test_an_end_is_one_token(monkeypatch):
+    """A list of them would never be found among the tokens: it is refused."""
+    monkeypatch.setattr(kernels, "beam_select", _select)
+    g = torch.Generator().manual_seed(3)
+    w = _Wrapper(torch.randn(20, 20, generator=g), 2)
+    prompt = [torch.tensor([4, 5])]
+    for bad in ([2], [2, 3], (1,), 2.0, "2", torch.tensor([1, 2])):
+        with pytest.raises(RuntimeError, match="eos_token_id"):
+            w.generate_beams(prompt, 2, max_new_tokens=4, eos_token_id=bad)
+    a = w.generate_beams(prompt, 2, max_new_tokens=9, eos_token_id=7)
+    b = w.generate_beams(prompt, 2, max_new_tokens=9, eos_token_id=torch.tensor(7))
+    assert torch.equal(a[0][0], b[0][0]) and a[1] == b[1]
