@@ -105,7 +105,7 @@ extern "C" int glq_paged_copy(const glq_paged_copy_params* p, void* stream) {
                         L * t.pages * (j < 2 ? page_bytes : page_scales)),
                   "caches that share some of their memory must be one");
   }
-  // every page is written once, and none that is read
+  // every page is written once, and none that is read (by pairs that copy anything)
   bool whole = true;
   {
     unsigned char* seen = (unsigned char*)calloc((size_t)(t.pages / 8 + 1), 1);
@@ -118,6 +118,8 @@ extern "C" int glq_paged_copy(const glq_paged_copy_params* p, void* stream) {
         what = "page out of range";
       else if (n < 0 || n > page)
         what = "tokens must be in [0, page_size]";
+      else if (n == 0)
+        continue;
       else if (seen[d / 8] >> (d % 8) & 1)
         what = "a page is written twice";
       else
@@ -126,7 +128,8 @@ extern "C" int glq_paged_copy(const glq_paged_copy_params* p, void* stream) {
     }
     if (same && !what)
       for (i = 0; i < p->pairs && !what; ++i)
-        if (seen[p->src[i] / 8] >> (p->src[i] % 8) & 1) what = "a page that is read is written";
+        if ((!p->tokens || p->tokens[i]) && (seen[p->src[i] / 8] >> (p->src[i] % 8) & 1))
+          what = "a page that is read is written";
     free(seen);
     GLQ_CHECK(!what, "pair %lld: %s", (long long)i - 1, what);
   }

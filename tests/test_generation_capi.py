@@ -115,3 +115,15 @@ def test_beam_of_nothing_and_workspace(lib):
     for bad in ((-1, 4, 1000, 8), (1, 0, 1000, 8), (1, 65, 1000, 8), (1, 4, 0, 8), (1, 4, 1000, 0),
                 (1, 4, 1000, 129), (1, 4, 1 << 25, 8)):
         assert size(*bad) == -1
+
+
+def test_copy_pairs_of_no_tokens(lib):
+    """They neither write nor read: the same page twice, or another pair's."""
+    assert _copy(lib, src=[0, 1], dst=[2, 2], tokens=[0, 0])[0] == 0  # (no launch)
+    assert _copy(lib, src=[0, 2, 3], dst=[2, 3, 3], tokens=[0, 0, 0])[0] == 0
+    for src, dst, tokens, what in (([8, 0], [1, 2], [0, 0], b"pair 0: page out of range"),
+                                   ([0, 1], [8, 2], [0, 0], b"pair 0: page out of range"),
+                                   ([0, 1, 3], [2, 2, 2], [0, 4, 4], b"pair 2: a page is written twice"),
+                                   ([0, 2], [2, 3], [1, 1], b"pair 1: a page that is read is written")):
+        rc, msg = _copy(lib, src=src, dst=dst, tokens=tokens)
+        assert rc == 1 and what in msg

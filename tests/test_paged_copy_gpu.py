@@ -178,3 +178,10 @@ def test_refusals(gpu):
             kernels.paged_copy(*x, [0], [1], **kw)
     for x, y in zip(raw(t), before):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [FP8, FP16])
+def test_pairs_of_no_tokens_beside_others(gpu, dtype):
+    """A page that one pair writes may be another's that copies nothing."""
+    check(gpu, 3, 9, 2, 64, 64, dtype, [0, 1, 5, 2, 6], [5, 5, 7, 0, 6], tokens=[20, 0, 0, 0, 0])
+    check(gpu, 3, 9, 2, 64, 64, dtype, [0, 1, 2], [5, 5, 6], tokens=[64, 0, 64], other=8)
