@@ -134,7 +134,7 @@ static int check_codec_shape(int64_t N, int64_t K, int bits) {
 
 extern "C" {
 
-int glq_version(void) { return 100; }
+int glq_version(void) { return 200; }
 
 const char* glq_last_error(void) { return g_err; }
 

@@ -49,7 +49,11 @@ extern "C" {
 #define GLQ_ERR_INVALID 1   /* argument check failed (the TORCH_CHECK analogue) */
 #define GLQ_ERR_HIP 2       /* a HIP runtime call or kernel launch failed       */
 
-/* Library version (major*10000 + minor*100 + patch). */
+/*
+ * Library version (major*10000 + minor*100 + patch).  0.2.0: the last field of
+ * glq_paged_attention_params, which 0.1.0 had as `reserved` and did not read, is
+ * `sinks`: callers written for 0.1.0 that leave it unset set it to 0.
+ */
 int glq_version(void);
 
 /* Message of the last error raised on the calling thread ("" if none). */

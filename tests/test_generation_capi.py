@@ -127,3 +127,9 @@ def test_copy_pairs_of_no_tokens(lib):
                                    ([0, 2], [2, 3], [1, 1], b"pair 1: a page that is read is written")):
         rc, msg = _copy(lib, src=src, dst=dst, tokens=tokens)
         assert rc == 1 and what in msg
+
+
+def test_version_tells_the_sinks_apart(lib):
+    """glq_paged_attention_params has sinks where a library before 0.2.0 had a
+    field that it did not read."""
+    assert lib.glq_version() >= 200
