@@ -39,7 +39,8 @@ class PagedKVCache:
     tokens attend to their last `window` positions and to the first `sinks` of
     their sequence (in layers whose own window is not smaller), and `extend`
     frees the pages that lie between: a sequence then needs about sinks + window
-    tokens' pages, however long it gets (prompts, all of theirs)."""
+    tokens' pages, however long it gets up to max_seq_len (prompts, all of
+    theirs).  Positions stay the sequence's own, in the model's rotation too."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, max_seqs: int, max_seq_len: int,
                  page_size: int = 64, pages: int | None = None,

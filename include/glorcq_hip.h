@@ -881,7 +881,7 @@ int glq_paged_copy(const glq_paged_copy_params* p, void* stream);
  * x rows of `vocab` logits (dtype 0: fp16, 1: bf16, 2: fp32), row_stride values
  * apart, beam after beam; scores (prompts, beams) fp32.  The `num` largest of
  * each prompt in falling order, the lowest k vocab + v first among equal ones,
- * compared in fp64 (to 3e-10): out_scores (prompts, num) fp32, out_parents and
+ * compared in fp64 (to 3e-10; of values past 2^17 to fp64's own rounding): out_scores (prompts, num) fp32, out_parents and
  * out_tokens (prompts, num) int64, their k and v.  A logit or a score of -inf
  * makes -inf, which is chosen after everything else; all continuations of a beam
  * with a NaN or +inf among its logits or as its score are NaN, which are chosen
