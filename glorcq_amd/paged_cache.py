@@ -276,10 +276,11 @@ class PagedKVCache:
         pools = kernels.paged_cache_tensors(pages, *self._shape)
         self._move_pages(live, pools)
         place = {p: i for i, p in enumerate(live)}
+        over = [w for w in self._wrappers if w._graph_pools is self.pools_key]
         self._take_pools(pools)
-        if self._wrappers:
+        if over:
             torch.cuda.synchronize(self.device)  # (no replay is under way)
-        for w in self._wrappers:
+        for w in over:
             w.graph = w.static_logits = None
         self.pages = pages
         self._refs = [self._refs[p] for p in live] + [0] * (pages - len(live))

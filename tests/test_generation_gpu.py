@@ -291,3 +291,25 @@ def test_a_resize_gives_memory_back(gpu):
     assert w.graph is None and torch.cuda.memory_allocated(gpu) <= held - (was - size())
     out, _ = w.generate(_prompts((5, 9), gpu), max_new_tokens=3)  # captured again
     assert [len(t) for t in out] == [8, 12]
+
+
+@torch.no_grad()
+def test_a_resize_takes_its_own_steps_alone(gpu):
+    """A wrapper that went over to another cache keeps its step when the first
+    one is resized, and is asked for a new one when its own is."""
+    model = _model(gpu)
+    w, other = _wrapper(model, 2, pages=20), _wrapper(model, 2, pages=20)
+    w.capture_graph()
+    first, w.cache = w.cache, other.cache
+    t = torch.tensor([1, 2], device=gpu)
+    with pytest.raises(RuntimeError, match="captured over"):
+        w.replay(t)
+    w.capture_graph()
+    first.resize(10)
+    w.prefill(_prompts((5, 9), gpu))
+    a = w.replay(t).clone()
+    w.cache.resize(10)
+    assert w.graph is None
+    other.capture_graph()
+    other.prefill(_prompts((5, 9), gpu))
+    assert torch.equal(a, other.replay(t))
